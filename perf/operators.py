@@ -41,7 +41,8 @@ byte's low half, a record is
 
 A block with largest magnitude a takes the least scale with a <= 7 scale, each
 value the code nearest to it (ties to the even code; 7 scale is as far from
-the largest code as 5 scale is from the two next to it).
+the largest code as 5 scale is from the two next to it); bytes go from 2 to 252,
+where every value is an ordinary number.
 """
 import math
 
@@ -215,7 +216,7 @@ def _codes(x):
     """Blocks of 32 values [..., 32] as codes 0 .. 15 and a scale byte each."""
     a = x.abs().amax(-1)
     bits = a.view(torch.int32)
-    e = ((bits >> 23) - 2 + ((bits & 0x7FFFFF) > 0x600000).to(torch.int32)).clamp(min=2)
+    e = ((bits >> 23) - 2 + ((bits & 0x7FFFFF) > 0x600000).to(torch.int32)).clamp(2, 252)
     y = x * ((254 - e) << 23).view(torch.float32).unsqueeze(-1)
     m = y.abs()
     # a tie goes to the even code: the borders 0.25, 1.25, 2.5 and 5 stay below
