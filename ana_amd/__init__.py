@@ -86,6 +86,16 @@ SIGNATURES = {
     "ana_trace": (C.c_int, [C.c_void_p, C.c_uint32]),
     "ana_trace_read": (C.c_int, [C.c_void_p, _u32p, C.c_size_t, _u32p]),
     "ana_probe_reread": (C.c_int, [C.c_int, C.c_uint64, C.c_uint32, C.POINTER(C.c_double)]),
+    "ana_kv4_bytes": (C.c_uint64, [C.c_uint32] * 4),
+    "ana_kv4_write": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ana_kv4_read": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ana_kv4_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_uint32, C.c_float, C.c_void_p,
+                                 C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
+    "ana_kv4_attend_ws": (C.c_uint64, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint64]),
+    "ana_row_logprobs": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p,
+                                   C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                   C.c_void_p, C.c_uint64, C.c_void_p]),
+    "ana_row_logprobs_ws": (C.c_uint64, [C.c_uint32] * 3),
     "ana_bpe_open": (C.c_int, [C.c_char_p, C.POINTER(C.c_void_p)]),
     "ana_bpe_bytes": (C.c_int, [C.POINTER(C.c_void_p)]),
     "ana_bpe_close": (None, [C.c_void_p]),

@@ -211,6 +211,16 @@ static int fail(ana_ctx* c, int code, const char* fmt, ...) {
   return code;
 }
 
+int ana::fail_call(int code, const char* fmt, ...) {
+  char buf[1024];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  g_open_err = buf;
+  return code;
+}
+
 #define HIPCHK(ctx, x)                                                                  \
   do {                                                                                  \
     hipError_t e_ = (x);                                                                \

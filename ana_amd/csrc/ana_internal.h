@@ -34,6 +34,9 @@ std::string read_ftc2(const char* path, Ftc2* out);
 // the manifest alone ("" or the reason it could not be read)
 std::string read_manifest(const char* path, ana_manifest* out);
 
+// the message of a call without a context, for ana_error(NULL); answers code
+int fail_call(int code, const char* fmt, ...);
+
 // ---------------------------------------------------------------- kernels
 // Every kernel computes in IEEE f32 with products and sums rounded
 // separately (compiled with -ffp-contract=off) and exp/log through double,

@@ -1,0 +1,70 @@
+// Keys and values held in 4 bits (MXFP4: E2M1 codes, an E8M0 scale a block of
+// 32 values along a head): the cache's records and what the kernels take.
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+namespace ana {
+
+// A cache: per sequence and head, ceil(slots / 32) records of 34 hd bytes,
+// 32 slots each. A record is laid out as the attention's lanes read it (lane
+// 16 j + m of a wave), so that a wave loads one as whole consecutive pieces:
+//   keys    [4 j][16 m][2 h][hd / 8 bytes]   slot 16 h + m, dims j hd / 4 ..
+//   values  [4 j][16 m][8 e][hd / 32 bytes]  slot 16 (e / 4) + 4 j + e % 4, dims m hd / 16 ..
+//   key scales    [hd / 32 blocks][16 m][2 h]
+//   value scales  [hd / 32 blocks][4 j][8 e]
+// A slot's codes and scales are whole bytes of its own, so two tokens that
+// are written at once never share a byte.
+struct Kv4 {
+  uint8_t* data;
+  uint32_t seqs, slots, tiles, heads, hd;
+};
+__host__ __device__ inline uint32_t kv4_record(uint32_t hd) { return 34 * hd; }
+
+// The rows of a call: sequence i (cache place seq[i], or i) has rows off[i]
+// .. off[i + 1] - 1 (or row i alone) at positions from pos[i].
+struct Kv4Rows {
+  const uint32_t *seq, *pos, *off;
+  uint32_t n, rows;
+};
+// a tensor [rows][heads][hd]: strides in elements, hd consecutive
+struct Kv4Mat {
+  void* p;
+  uint64_t row, head;
+};
+
+enum ElemType : int { ET_F32 = 0, ET_BF16 = 1, ET_F16 = 2 };
+
+// the head sizes and element types that the kernels take
+inline bool kv4_fits(uint32_t hd) { return hd == 32 || hd == 64 || hd == 128; }
+
+// k and v into the cache. With gk, k is qk-normed first, and with q (f32) the
+// query rows are normed in place with gq (one launch for a decoder layer).
+hipError_t launch_kv4_write(const Kv4& c, const Kv4Rows& r, int type, const Kv4Mat& k, const Kv4Mat& v,
+                            const float* gk, const float* gq, const Kv4Mat* q, uint32_t qheads, hipStream_t st);
+// the values that the cache holds for the rows
+hipError_t launch_kv4_read(const Kv4& c, const Kv4Rows& r, int type, const Kv4Mat& k, const Kv4Mat& v,
+                           hipStream_t st);
+
+struct Kv4Attend {
+  Kv4 c;
+  Kv4Rows r;
+  Kv4Mat q, o;
+  uint32_t hq;
+  float scale;
+  const float* sink;   // [hq] or nullptr
+  float* part;         // partials [rows][hq][nsplit][hd + 2], when nsplit > 1
+  uint32_t nsplit, tps;  // pieces of the slots, tiles each but the last
+};
+// how a call's slots are split (live: the most positions a sequence holds
+// after the call, as far as the caller knows; 0: the ring's slots), and the
+// floats of partials that takes
+void kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live, uint32_t* nsplit,
+               uint32_t* tps);
+inline uint64_t kv4_part_floats(uint32_t rows, uint32_t hq, uint32_t hd, uint32_t nsplit) {
+  return nsplit > 1 ? (uint64_t)rows * hq * nsplit * (hd + 2) : 0;
+}
+hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st);
+
+}  // namespace ana

@@ -1,0 +1,415 @@
+// Log probabilities of given tokens, their ranks, the entropy and the top
+// alternatives of rows of logits (gfx950).
+//
+// One pass over a row: a workgroup keeps its piece of the row in registers,
+// so the maximum m, then l = sum e^(x - m) and w = sum e^(x - m) (x - m), the
+// given token's rank and the alternatives all come from one read.
+//   lp(t) = x_t - m - log l        H = log l - w / l
+// The entries at the maximum are counted (c), not summed: log l is
+// log1p(c - 1 + sum of the others), which keeps a probability next to 1 and
+// an entropy next to 0 to their own last bits.
+//
+// Alternatives: logits are ordered by value, then by the lower index (a NaN
+// after every number), so an order key (value bits, ~index) is unique. The
+// k-th largest of 64 group maxima is a bound that at least k logits reach and
+// few more do; those go to LDS, where each counts the keys above its own.
+// Where ties (or rows of few numbers) make them too many, or too few, k
+// rounds of a maximum over the registers find the same.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kv4.h"
+#include "logprobs.h"
+#include "mfma.h"
+#include "wave.h"
+
+namespace ana {
+
+namespace {
+
+typedef unsigned long long u64;
+
+constexpr uint32_t kHead = 8;   // a piece's words before its keys: m, c, l, w, rank, bad
+
+// a logit's order as a whole number: larger for larger ones, -0 as +0, 0 for NaN
+__device__ __forceinline__ uint32_t order_of(float x) {
+  if (x != x) return 0;
+  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
+  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+}
+__device__ __forceinline__ float value_of(uint32_t o) {
+  if (o == 0) return __builtin_nanf("");
+  return __builtin_bit_cast(float, (o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
+__device__ __forceinline__ u64 key_of(float x, uint32_t i) { return (u64)order_of(x) << 32 | (0xFFFFFFFFu - i); }
+
+__device__ __forceinline__ u64 wave_max64(u64 v) {
+#pragma unroll
+  for (int k = 32; k >= 1; k >>= 1) {
+    const u64 o = __shfl_xor(v, k, 64);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void load_vec(const T* p, float* x) {
+  typedef T vecw __attribute__((ext_vector_type(W)));
+  const vecw v = *reinterpret_cast<const vecw*>(p);
+#pragma unroll
+  for (int e = 0; e < W; e++) x[e] = (float)v[e];
+}
+
+// a row's results from its sums (bad: a NaN or +inf among the logits)
+struct RowSums {
+  float m, c, l, w;
+  bool bad;
+  // log of the sum over e^m, and of a logit
+  __device__ __forceinline__ float log_sum() const { return log1pf((c - 1.0f) + l); }
+  __device__ __forceinline__ float lp(float x, float ls) const {
+    if (bad || x != x) return __builtin_nanf("");
+    if (x == -INFINITY) return x;
+    return (x - m) - ls;
+  }
+  __device__ __forceinline__ float entropy(float ls) const {
+    if (bad) return __builtin_nanf("");
+    return m == -INFINITY ? 0.0f : ls - w / (c + l);
+  }
+};
+
+// Piece z of row r, elements z C .. (C a multiple of 16 bytes of elements, at
+// most NT V W). The row may start anywhere: whole 16-byte vectors from its
+// first border on, the elements before and after them one each for the first
+// threads. Alone (one piece) it writes the row's results, else its sums and
+// keys.
+template <typename T, int NT, int V>
+__global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint32_t S) {
+  constexpr int W = 16 / sizeof(T), NW = NT / 64, CAP = 512;
+  __shared__ float tmax[NW][64];
+  __shared__ float red[NW][3];
+  __shared__ uint32_t redu[NW][2];
+  __shared__ float bound_s;
+  __shared__ uint32_t ncand;
+  __shared__ u64 cand[CAP], best[kLpMaxTop], wred[NW];
+  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
+  const uint32_t r = blockIdx.x / S, z = blockIdx.x % S;
+  const T* row = (const T*)a.logits + (uint64_t)r * a.ld;
+  const uint32_t e0 = z * C, cnt = min(C, a.vocab - e0);
+  const T* p = row + e0;
+  const uint32_t head = min((uint32_t)((16 - (uintptr_t)p % 16) % 16 / sizeof(T)), cnt);
+  const uint32_t nvec = (cnt - head) / W, tail0 = head + nvec * W;
+  const uint32_t k = a.top;
+  float x[V][W];
+#pragma unroll
+  for (int u = 0; u < V; u++) {
+    const uint32_t v = u * NT + tid;
+    if (v < nvec) {
+      load_vec<T, W>(p + head + v * W, x[u]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < W; e++) x[u][e] = -INFINITY;
+    }
+  }
+  // this thread's element before or after the vectors
+  const uint32_t edge = tid < head ? tid : tail0 + (tid - head);
+  const bool has_edge = tid < head || edge < cnt;
+  const float xe = has_edge ? (float)p[edge] : -INFINITY;
+  const uint32_t tk = a.tok ? a.tok[r] : 0xFFFFFFFFu;
+  const bool given = tk < a.vocab;
+  const float xt = given ? (float)row[tk] : 0.0f;
+  if (tid == 0) ncand = 0;
+
+  float m = xe == xe ? xe : -INFINITY;
+  bool bad = !(xe < INFINITY);
+#pragma unroll
+  for (int u = 0; u < V; u++)
+#pragma unroll
+    for (int e = 0; e < W; e++) {
+      bad |= !(x[u][e] < INFINITY);
+      m = fmaxf(m, x[u][e]);
+    }
+  const float tm = m;
+  tmax[wv][lane] = tm;
+  __syncthreads();
+  // group l: lane l of every wave
+  float gm = tmax[0][lane];
+#pragma unroll
+  for (int i = 1; i < NW; i++) gm = fmaxf(gm, tmax[i][lane]);
+  m = wmax(gm);
+  if (wv == 0 && k) {
+    // the group maximum that k of them reach
+    uint32_t above = 0;
+    for (int i = 0; i < 64; i++) {
+      const float o = lane_f(gm, i);
+      above += o > gm || (o == gm && i < (int)lane);
+    }
+    if (above == k - 1) bound_s = gm;
+  }
+  // (+inf: the row's results are NaN whatever the sums)
+  const float ms = m == -INFINITY || m == INFINITY ? 0.0f : m;
+  float l = 0.0f, w = 0.0f, c = 0.0f;
+  uint32_t above = 0;
+  constexpr float log2e = 1.4426950408889634f;
+  // an entry's terms; far below the maximum (and for -inf) both are 0
+  auto term = [&](float v, bool skip_top) {
+    const float d = fmaxf(v - ms, -200.0f);
+    const float t = __builtin_amdgcn_exp2f(d * log2e);
+    l += skip_top && v == m ? 0.0f : t;
+    w = fmaf(t, d, w);
+  };
+  if (__any(tm == m)) {
+    term(xe, true);
+    c += xe == m && has_edge ? 1.0f : 0.0f;
+#pragma unroll
+    for (int u = 0; u < V; u++) {
+      const bool in = (uint32_t)u * NT + tid < nvec;
+#pragma unroll
+      for (int e = 0; e < W; e++) {
+        term(x[u][e], true);
+        c += x[u][e] == m && in ? 1.0f : 0.0f;
+      }
+    }
+  } else {
+    term(xe, false);
+#pragma unroll
+    for (int u = 0; u < V; u++)
+#pragma unroll
+      for (int e = 0; e < W; e++) term(x[u][e], false);
+  }
+  if (given) {
+    const uint32_t ot = order_of(xt);
+    auto over = [&](float v, uint32_t i, bool in) {
+      // (a NaN is above nothing; every number is above a NaN)
+      const bool gt = v > xt || (ot == 0 && v == v);
+      const bool eq = v == xt || (ot == 0 && v != v);
+      above += in && (gt || (eq && i < tk)) ? 1u : 0u;
+    };
+    over(xe, e0 + edge, has_edge);
+#pragma unroll
+    for (int u = 0; u < V; u++) {
+      const uint32_t v = u * NT + tid;
+#pragma unroll
+      for (int e = 0; e < W; e++) over(x[u][e], e0 + head + v * W + e, v < nvec);
+    }
+  }
+  float s3[3] = {l, w, c};
+  wsum_n(s3);
+  uint32_t ab = above;
+#pragma unroll
+  for (int mk = 32; mk >= 1; mk >>= 1) ab += __shfl_xor(ab, mk, 64);
+  const uint32_t anybad = __any(bad);
+  if (lane == 0) {
+    red[wv][0] = s3[0];
+    red[wv][1] = s3[1];
+    red[wv][2] = s3[2];
+    redu[wv][0] = ab;
+    redu[wv][1] = anybad;
+  }
+  __syncthreads();
+  if (k) {
+    const float bound = bound_s;
+    auto offer = [&](float v, uint32_t i, bool in) {
+      if (in && v >= bound) {
+        const uint32_t at = atomicAdd(&ncand, 1u);
+        if (at < CAP) cand[at] = key_of(v, i);
+      }
+    };
+    if (__any(tm >= bound)) {
+      offer(xe, e0 + edge, has_edge);
+#pragma unroll
+      for (int u = 0; u < V; u++) {
+        const uint32_t v = u * NT + tid;
+#pragma unroll
+        for (int e = 0; e < W; e++) offer(x[u][e], e0 + head + v * W + e, v < nvec);
+      }
+    }
+    __syncthreads();
+    const uint32_t nc = ncand, want = min(k, cnt);
+    if (tid < k && tid >= want) best[tid] = 0;
+    if (nc <= CAP && nc >= want) {
+      for (uint32_t i = tid; i < nc; i += NT) {
+        const u64 mine = cand[i];
+        uint32_t over = 0;
+        for (uint32_t o = 0; o < nc; o++) over += cand[o] > mine ? 1u : 0u;
+        if (over < k) best[over] = mine;
+      }
+    } else {
+      u64 last = ~0ull;
+      for (uint32_t i = 0; i < want; i++) {
+        u64 t = 0;
+        auto see = [&](float v, uint32_t at, bool in) {
+          const u64 q = key_of(v, at);
+          if (in && q < last && q > t) t = q;
+        };
+        see(xe, e0 + edge, has_edge);
+#pragma unroll
+        for (int u = 0; u < V; u++) {
+          const uint32_t v = u * NT + tid;
+#pragma unroll
+          for (int e = 0; e < W; e++) see(x[u][e], e0 + head + v * W + e, v < nvec);
+        }
+        t = wave_max64(t);
+        __syncthreads();
+        if (lane == 0) wred[wv] = t;
+        __syncthreads();
+        t = wred[0];
+#pragma unroll
+        for (int o = 1; o < NW; o++) t = wred[o] > t ? wred[o] : t;
+        if (tid == 0) best[i] = t;
+        last = t;
+      }
+    }
+    __syncthreads();
+  }
+  // the piece's sums, in the waves' order
+  RowSums rs{m, 0.0f, 0.0f, 0.0f, false};
+  uint32_t rk = 0;
+#pragma unroll
+  for (int i = 0; i < NW; i++) {
+    rs.l += red[i][0];
+    rs.w += red[i][1];
+    rs.c += red[i][2];
+    rk += redu[i][0];
+    rs.bad |= redu[i][1] != 0;
+  }
+  if (S > 1) {
+    uint32_t* out = a.part + (uint64_t)blockIdx.x * (kHead + 2 * k);
+    if (tid == 0) {
+      out[0] = __builtin_bit_cast(uint32_t, rs.m);
+      out[1] = __builtin_bit_cast(uint32_t, rs.c);
+      out[2] = __builtin_bit_cast(uint32_t, rs.l);
+      out[3] = __builtin_bit_cast(uint32_t, rs.w);
+      out[4] = rk;
+      out[5] = rs.bad;
+    }
+    if (tid < k) {
+      out[kHead + 2 * tid] = (uint32_t)best[tid];
+      out[kHead + 2 * tid + 1] = (uint32_t)(best[tid] >> 32);
+    }
+    return;
+  }
+  const float ls = rs.log_sum();
+  if (tid == 0) {
+    a.ent[r] = rs.entropy(ls);
+    if (a.tok) {
+      a.lp[r] = given ? rs.lp(xt, ls) : __builtin_nanf("");
+      a.rank[r] = given ? rk : 0xFFFFFFFFu;
+    }
+  }
+  if (tid < k) {
+    a.top_tok[(uint64_t)r * k + tid] = 0xFFFFFFFFu - (uint32_t)best[tid];
+    a.top_lp[(uint64_t)r * k + tid] = rs.lp(value_of((uint32_t)(best[tid] >> 32)), ls);
+  }
+}
+
+// A row's pieces, a wave a row and a lane a piece: the sums brought to the
+// row's maximum, and k rounds of a maximum over the pieces' next keys.
+template <typename T>
+__global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S) {
+  const uint32_t r = blockIdx.x, lane = threadIdx.x, k = a.top;
+  const uint32_t* p = a.part + ((uint64_t)r * S + lane) * (kHead + 2 * k);
+  const bool in = lane < S;
+  RowSums q{-INFINITY, 0.0f, 0.0f, 0.0f, false};
+  uint32_t rk = 0;
+  if (in) {
+    q.m = __builtin_bit_cast(float, p[0]);
+    q.c = __builtin_bit_cast(float, p[1]);
+    q.l = __builtin_bit_cast(float, p[2]);
+    q.w = __builtin_bit_cast(float, p[3]);
+    rk = p[4];
+    q.bad = p[5] != 0;
+  }
+  const uint32_t tk = a.tok ? a.tok[r] : 0xFFFFFFFFu;
+  const bool given = tk < a.vocab;
+  const float xt = given ? (float)((const T*)a.logits + (uint64_t)r * a.ld)[tk] : 0.0f;
+  RowSums t{wmax(q.m), 0.0f, 0.0f, 0.0f, (bool)__any(q.bad)};
+  // e^(x - M) = f e^(x - m), (x - M) = (x - m) + d; a piece below the
+  // maximum has no entry at it
+  const float d = fmaxf(q.m - t.m, -200.0f);
+  const bool at = q.m == t.m, none = q.m == -INFINITY;
+  const float f = none ? 0.0f : __expf(d);
+  float s[3];
+  s[0] = at ? q.c : 0.0f;
+  s[1] = at ? q.l : f * (q.c + q.l);
+  s[2] = at ? q.w : f * (q.w + d * (q.c + q.l));
+  wsum_n(s);
+  t.c = s[0];
+  t.l = s[1];
+  t.w = s[2];
+#pragma unroll
+  for (int mk = 32; mk >= 1; mk >>= 1) rk += __shfl_xor(rk, mk, 64);
+  const float ls = t.log_sum();
+  if (lane == 0) {
+    a.ent[r] = t.entropy(ls);
+    if (a.tok) {
+      a.lp[r] = given ? t.lp(xt, ls) : __builtin_nanf("");
+      a.rank[r] = given ? rk : 0xFFFFFFFFu;
+    }
+  }
+  uint32_t at_i = 0;
+  auto next = [&]() -> u64 {
+    return in && at_i < k ? (u64)p[kHead + 2 * at_i + 1] << 32 | p[kHead + 2 * at_i] : 0ull;
+  };
+  u64 mine = k ? next() : 0;
+  for (uint32_t i = 0; i < k; i++) {
+    const u64 b = wave_max64(mine);
+    if (mine == b) {
+      a.top_tok[(uint64_t)r * k + i] = 0xFFFFFFFFu - (uint32_t)b;
+      a.top_lp[(uint64_t)r * k + i] = t.lp(value_of((uint32_t)(b >> 32)), ls);
+      at_i++;
+      mine = next();
+    }
+  }
+}
+
+// The pieces of a row: whole rows of up to 32768 logits where the rows alone
+// fill the chip, else pieces of 8192, or of 2048 where those are few.
+struct Plan {
+  uint32_t C, S;
+  bool wide;
+};
+Plan plan_of(uint32_t n, uint32_t vocab) {
+  Plan p;
+  p.wide = n >= 256 || vocab > 64 * 8192;
+  const uint32_t cap = p.wide ? 32768u : (uint64_t)n * vocab >= 256ull * 8192 ? 8192u : 2048u;
+  p.S = (vocab + cap - 1) / cap;
+  if (p.S > 64) p.S = 64;
+  p.C = ((vocab + p.S - 1) / p.S + 7) & ~7u;
+  p.S = (vocab + p.C - 1) / p.C;
+  return p;
+}
+
+}  // namespace
+
+uint64_t logprobs_part_words(uint32_t n, uint32_t vocab, uint32_t top) {
+  const Plan p = plan_of(n, vocab);
+  return p.S > 1 ? (uint64_t)n * p.S * (kHead + 2 * top) : 0;
+}
+
+hipError_t launch_logprobs(const LogprobArgs& a, int type, hipStream_t st) {
+  if (!a.logits || a.vocab == 0 || a.vocab > kLpMaxVocab || a.top > kLpMaxTop || a.top > a.vocab || a.ld < a.vocab || !a.ent)
+    return hipErrorInvalidValue;
+  if (a.n == 0) return hipSuccess;
+  const Plan p = plan_of(a.n, a.vocab);
+  if ((p.S > 1 && !a.part) || (uint64_t)a.n * p.S > 0x7FFFFFFFull) return hipErrorInvalidValue;
+  auto go = [&](auto t) -> hipError_t {
+    using T = decltype(t);
+    constexpr int W = 16 / sizeof(T);
+    const dim3 g(a.n * p.S);
+    if (p.wide)
+      hipLaunchKernelGGL((k_logprobs<T, 1024, 32 / W>), g, dim3(1024), 0, st, a, p.C, p.S);
+    else
+      hipLaunchKernelGGL((k_logprobs<T, 256, 32 / W>), g, dim3(256), 0, st, a, p.C, p.S);
+    if (p.S > 1) hipLaunchKernelGGL((k_logprobs_join<T>), dim3(a.n), dim3(64), 0, st, a, p.S);
+    return hipGetLastError();
+  };
+  switch (type) {
+    case ET_F32: return go(float{});
+    case ET_BF16: return go(__bf16{});
+    case ET_F16: return go(_Float16{});
+    default: return hipErrorInvalidValue;
+  }
+}
+
+}  // namespace ana

@@ -1,0 +1,184 @@
+"""libana's operators on device memory, over torch tensors (include/ana.h,
+"operators on device memory"): keys and values in 4 bits, attention over
+them, and the log probabilities of rows of logits.
+
+A ctypes mirror, as ana_amd itself is: every value is computed by libana.so.
+torch holds the tensors, allocates outputs and workspaces, and names the
+stream: the work is queued on the tensors' device's current stream, can be
+captured there, and is not waited for. Tensors of other streams are the
+caller's to order, as for any torch operation.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import ANA_OK, AnaError, lib
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _Kv4(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("device", C.c_int), ("seqs", C.c_uint32), ("slots", C.c_uint32),
+                ("heads", C.c_uint32), ("hd", C.c_uint32)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("n", C.c_uint32), ("rows", C.c_uint32), ("seq", C.c_void_p), ("pos", C.c_void_p),
+                ("off", C.c_void_p)]
+
+
+class _Mat(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("row", C.c_uint64), ("head", C.c_uint64)]
+
+
+def _check(r: int) -> None:
+    if r != ANA_OK:
+        raise AnaError(r, lib().ana_error(None).decode())
+
+
+def _device(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise ValueError(f"{name} is not on a GPU")
+    return t.device.index
+
+
+def _stream(device: int) -> int:
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _ints(t, n: int, device: int, name: str):
+    """A device array of whole numbers: int32, consecutive, n of them."""
+    if t is None:
+        return None
+    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: a consecutive int32 tensor of {n}, not {tuple(t.shape)} {t.dtype}")
+    if t.device.index != device or not t.is_cuda:
+        raise ValueError(f"{name} is on {t.device}, not on GPU {device}")
+    return t.data_ptr()
+
+
+def _mat(t: torch.Tensor, rows: int, heads: int, hd: int, dtype, device: int, name: str) -> _Mat:
+    if t.dim() != 3 or tuple(t.shape) != (rows, heads, hd) or t.dtype != dtype:
+        raise ValueError(f"{name}: {(rows, heads, hd)} {dtype}, not {tuple(t.shape)} {t.dtype}")
+    if not t.is_cuda or t.device.index != device:
+        raise ValueError(f"{name} is on {t.device}, not on GPU {device}")
+    a, b, c = t.stride()
+    if c != 1 and hd > 1:
+        raise ValueError(f"{name}: the last axis is not consecutive")
+    return _Mat(t.data_ptr(), a, b)
+
+
+class KV4:
+    """A cache of keys and values in 4 bits (MXFP4) for `seqs` sequences:
+    rings of `slots` positions, data uint8 [seqs, heads, ceil(slots / 32),
+    34 hd] in ana.h's layout. Takes the tensor it is given, as a cache that
+    was moved or saved, or (KV4.empty) a new one of zeros."""
+
+    def __init__(self, data: torch.Tensor, slots: int):
+        if data.dtype != torch.uint8 or data.dim() != 4 or not data.is_contiguous():
+            raise ValueError("KV4: a consecutive uint8 tensor of four axes")
+        s, h, t, r = data.shape
+        if slots < 1 or t != (slots + 31) // 32 or r % 34 or lib().ana_kv4_bytes(s, slots, h, r // 34) != data.numel():
+            raise ValueError(f"KV4: {tuple(data.shape)} is not a cache of {slots} slots")
+        self.data, self.slots = data, slots
+        self.seqs, self.heads, self.hd = s, h, r // 34
+        self.device = _device(data, "KV4")
+        self._c = _Kv4(data.data_ptr(), self.device, s, slots, h, r // 34)
+
+    @classmethod
+    def empty(cls, seqs: int, slots: int, heads: int, hd: int, device="cuda") -> "KV4":
+        if lib().ana_kv4_bytes(seqs, slots, heads, hd) == 0:
+            raise ValueError(f"KV4: no cache of {seqs} sequences, {slots} slots, {heads} heads of {hd}")
+        return cls(torch.zeros((seqs, heads, (slots + 31) // 32, 34 * hd), dtype=torch.uint8, device=device), slots)
+
+
+def _rows(cache: KV4, rows: int, pos, seq, off) -> _Rows:
+    n = pos.numel()
+    return _Rows(n, rows, _ints(seq, n, cache.device, "seq"), _ints(pos, n, cache.device, "pos"),
+                 _ints(off, n + 1, cache.device, "off"))
+
+
+def kv4_write(cache: KV4, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, seq=None, off=None) -> None:
+    """Keys and values [rows, heads, hd] into the cache: sequence i (its
+    place seq[i], or i) at positions pos[i] and on, its rows off[i] ..
+    off[i + 1] - 1 (or row i alone). ana_kv4_write."""
+    rows = k.shape[0]
+    r = _rows(cache, rows, pos, seq, off)
+    km = _mat(k, rows, cache.heads, cache.hd, k.dtype, cache.device, "k")
+    vm = _mat(v, rows, cache.heads, cache.hd, k.dtype, cache.device, "v")
+    _check(lib().ana_kv4_write(C.byref(cache._c), C.byref(r), _TYPES.get(k.dtype, -1), C.byref(km), C.byref(vm),
+                               _stream(cache.device)))
+
+
+def kv4_read(cache: KV4, pos: torch.Tensor, rows: int, seq=None, off=None, dtype=torch.float32):
+    """The values that the cache holds at the rows' positions: k and v
+    [rows, heads, hd]. Rows that no sequence has are left unset.
+    ana_kv4_read."""
+    r = _rows(cache, rows, pos, seq, off)
+    k = torch.empty((rows, cache.heads, cache.hd), dtype=dtype, device=cache.data.device)
+    v = torch.empty_like(k)
+    km = _mat(k, rows, cache.heads, cache.hd, dtype, cache.device, "k")
+    vm = _mat(v, rows, cache.heads, cache.hd, dtype, cache.device, "v")
+    _check(lib().ana_kv4_read(C.byref(cache._c), C.byref(r), _TYPES.get(dtype, -1), C.byref(km), C.byref(vm),
+                              _stream(cache.device)))
+    return k, v
+
+
+def kv4_attend(q: torch.Tensor, cache: KV4, pos: torch.Tensor, seq=None, off=None, sink=None, scale=None, live: int = 0,
+               out=None) -> torch.Tensor:
+    """Softmax attention of query rows [rows, hq, hd] over the cache, whose
+    own keys and values have been written; each row sees the positions up to
+    its own that its ring holds. sink: float32 [hq]; scale: hd ** -0.5 unless
+    given; live: the most positions a sequence holds, where the program knows
+    it to be fewer than the ring's (only the split of the work depends on
+    it); out: where the outputs go (rows that no sequence has stay as they
+    are there). ana_kv4_attend."""
+    rows, hq = q.shape[0], q.shape[1]
+    r = _rows(cache, rows, pos, seq, off)
+    qm = _mat(q, rows, hq, cache.hd, q.dtype, cache.device, "q")
+    if out is None:
+        out = torch.empty((rows, hq, cache.hd), dtype=q.dtype, device=q.device)
+    om = _mat(out, rows, hq, cache.hd, q.dtype, cache.device, "out")
+    if sink is not None and (sink.dtype != torch.float32 or sink.shape != (hq,) or not sink.is_contiguous()
+                             or not sink.is_cuda or sink.device.index != cache.device):
+        raise ValueError(f"sink: a consecutive float32 tensor of {hq} on GPU {cache.device}")
+    L = lib()
+    nb = L.ana_kv4_attend_ws(C.byref(cache._c), C.byref(r), hq, live)
+    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
+    _check(L.ana_kv4_attend(C.byref(cache._c), C.byref(r), _TYPES.get(q.dtype, -1), C.byref(qm), hq,
+                            cache.hd ** -0.5 if scale is None else scale,
+                            None if sink is None else sink.data_ptr(), C.byref(om), live,
+                            None if ws is None else ws.data_ptr(), nb, _stream(cache.device)))
+    return out
+
+
+def logprobs(logits: torch.Tensor, tokens=None, top: int = 0):
+    """Of each row of logits [n, vocab]: the log probability and the rank of
+    the given token (tokens int32 [n]; None for neither), the entropy, and
+    the `top` likeliest tokens with their log probabilities, ties to the
+    lower index: (logprob [n], entropy [n], rank [n], top [n, top],
+    top_logprob [n, top]), float32 and int32. Rank counts the tokens before
+    it, -1 for a token outside the vocabulary. ana_row_logprobs."""
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logprobs: rows of logits, each consecutive")
+    device = _device(logits, "logits")
+    n, vocab = logits.shape
+    ids = _ints(tokens, n, device, "tokens")
+    new = dict(device=logits.device)
+    ent = torch.empty(n, dtype=torch.float32, **new)
+    lp = rank = None
+    if tokens is not None:
+        lp = torch.empty(n, dtype=torch.float32, **new)
+        rank = torch.empty(n, dtype=torch.int32, **new)
+    ids_top = torch.empty((n, top), dtype=torch.int32, **new)
+    lp_top = torch.empty((n, top), dtype=torch.float32, **new)
+    L = lib()
+    nb = L.ana_row_logprobs_ws(n, vocab, top)
+    ws = torch.empty(nb, dtype=torch.uint8, **new) if nb else None
+    _check(L.ana_row_logprobs(device, _TYPES.get(logits.dtype, -1), logits.data_ptr(), logits.stride(0), n, vocab, ids,
+                              top, None if lp is None else lp.data_ptr(), ent.data_ptr(),
+                              None if rank is None else rank.data_ptr(), ids_top.data_ptr(), lp_top.data_ptr(),
+                              None if ws is None else ws.data_ptr(), nb, _stream(device)))
+    return lp, ent, rank, ids_top, lp_top

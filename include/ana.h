@@ -278,6 +278,110 @@ typedef struct ana_manifest {
  * unreadable file, a wrong magic or a short header. */
 int ana_manifest_read(const char* path, ana_manifest* out);
 
+/* ---- operators on device memory ----
+ * The kernels of a context's ANA_KV4 rings and of its log probabilities, for
+ * programs that hold their own tensors on the device (no counterpart in the
+ * reference). Unlike the calls on a context they take device pointers and
+ * queue their work on `stream` (a hipStream_t; NULL the device's default
+ * stream) without waiting for it: the memory stays the caller's, and stays
+ * valid until the stream has passed the call. They allocate nothing,
+ * synchronise nothing and can be captured into a graph. A call that needs a
+ * workspace takes it from the caller; two calls that may run at the same
+ * time need two. `device` is the pointers' device; the calling thread's
+ * current device is left as it was. Any thread may call them; after a
+ * nonzero answer ana_error(NULL) holds the calling thread's message.
+ *
+ * Tensors are [rows][heads][hd] with any strides between rows and between
+ * heads, counted in elements, the last axis consecutive. Addresses and
+ * strides on 16 bytes are read and written fastest. */
+#define ANA_T_F32 0
+#define ANA_T_BF16 1
+#define ANA_T_F16 2
+
+/* Keys and values of `seqs` sequences in 4 bits: rings of `slots` positions
+ * (position p in slot p mod slots), `heads` key heads of hd = 32, 64 or 128
+ * values. MXFP4: a value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4 or 6 and a
+ * sign), and 32 values next to each other along a head share a scale byte b,
+ * 2^(b - 127). A block with largest magnitude a takes the least scale from
+ * 2^-125 on with a <= 7 scale, a value the nearest code, ties to the even
+ * one; a block with an infinity or a NaN in it becomes NaN (b = 255).
+ * data holds ana_kv4_bytes bytes on a 16-byte border, for each sequence and
+ * head ceil(slots / 32) records of 32 slots and 34 hd bytes:
+ *   keys    [4 j][16 m][2 h][hd / 8]  slot 16 h + m, dims j hd / 4 ..
+ *   values  [4 j][16 m][8 e][hd / 32] slot 16 (e / 4) + 4 j + e % 4, dims m hd / 16 ..
+ *   key scales   [hd / 32][16 m][2 h]
+ *   value scales [hd / 32][4 j][8 e]
+ * two codes a byte, the even dimension's in the low half. */
+typedef struct {
+  void* data;
+  int device;
+  uint32_t seqs, slots, heads, hd;
+} ana_kv4;
+
+/* The rows of a call, in device memory: sequence i of n has its place
+ * seq[i] in the cache (seq NULL: i; a place outside 0 .. seqs - 1 is none:
+ * nothing is stored for it, and its outputs are zeros) and rows off[i] ..
+ * off[i + 1] - 1 of the tensors, at positions pos[i] and on (off NULL: row i
+ * alone, rows == n). off does not go down, and ends at `rows` at most; rows
+ * before off[0] and from off[n] on are not read, and their outputs are left
+ * as they were. */
+typedef struct {
+  uint32_t n, rows;
+  const uint32_t *seq, *pos, *off;
+} ana_kv4_rows;
+
+/* a tensor: its address, and the elements from row to row and head to head */
+typedef struct {
+  void* p;
+  uint64_t row, head;
+} ana_mat;
+
+/* the bytes of a cache; 0 where its shape is refused */
+uint64_t ana_kv4_bytes(uint32_t seqs, uint32_t slots, uint32_t heads, uint32_t hd);
+
+/* Keys k and values v (of ANA_T_ type `type`) into the cache. Of a
+ * sequence with more rows than slots only the last `slots` are stored; a
+ * sequence that the call lists again (with rows) is stored the first time. */
+int ana_kv4_write(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_mat* k, const ana_mat* v,
+                  void* stream);
+
+/* The values that the cache holds at the rows' positions, to k and v. */
+int ana_kv4_read(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_mat* k, const ana_mat* v,
+                 void* stream);
+
+/* Softmax attention of query rows [rows][hq][hd] over the cache; query head
+ * a reads key head a / (hq / heads). The call's own keys and values have
+ * been written. A row at position p, of a sequence whose last row is at P,
+ * sees the positions up to p that the ring still holds (those above P -
+ * slots): o = sum_j e^(scale q.k_j) v_j over (sum_j e^(scale q.k_j) +
+ * e^sink[a]), sink (hq floats) NULL for none; 0 where it sees nothing.
+ * What a row does not see, NaN included, does not change it. In f32 the
+ * products are exact up to their f32 sums; 16-bit outputs take
+ * probabilities to 2^-17. `live`, where not 0, is the most positions a
+ * sequence holds after the call, as far as the caller knows: it only
+ * chooses how the work is split. ws: ana_kv4_attend_ws bytes of workspace
+ * for the same arguments, on a 16-byte border. */
+int ana_kv4_attend(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_mat* q, uint32_t hq, float scale,
+                   const float* sink, const ana_mat* o, uint64_t live, void* ws, uint64_t ws_bytes, void* stream);
+uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq, uint64_t live);
+
+/* Of n rows of `vocab` logits (of ANA_T_ type `type`, ld elements from row
+ * to row), in one read of them: lp[i], the log probability of the given
+ * token tok[i] (NaN for a token outside the vocabulary), and rank[i], the
+ * tokens before it in the order of value, then of lower index (0: it is the
+ * greedy pick; 2^32 - 1 outside the vocabulary); tok NULL: neither is
+ * written. ent[i], the entropy in nats; top_tok and top_lp [n][top], the
+ * first `top` (0 .. 64, at most vocab) tokens in that order and their log
+ * probabilities. A logit of -inf has probability 0; in a row with nothing
+ * else every log probability is -inf and the entropy 0. NaN comes after
+ * every number in the order; a NaN or +inf in a row makes its log
+ * probabilities and entropy NaN. Sums are f32. vocab up to 2^21. ws:
+ * ana_row_logprobs_ws bytes, on a 4-byte border. */
+int ana_row_logprobs(int device, int type, const void* logits, uint64_t ld, uint32_t n, uint32_t vocab,
+                     const uint32_t* tok, uint32_t top, float* lp, float* ent, uint32_t* rank, uint32_t* top_tok,
+                     float* top_lp, void* ws, uint64_t ws_bytes, void* stream);
+uint64_t ana_row_logprobs_ws(uint32_t n, uint32_t vocab, uint32_t top);
+
 /* ---- the fast BPE tokenizer (bend/Tokenizer.bend), host side ----
  * Tokens: 0 = BOS, 1 = EOS, 2..257 the bytes, then one per merge in id
  * order. The GPU path sees ids only; these serve the prompts and the
