@@ -47,6 +47,8 @@ hipError_t launch_kv4_write(const Kv4& c, const Kv4Rows& r, int type, const Kv4M
 hipError_t launch_kv4_read(const Kv4& c, const Kv4Rows& r, int type, const Kv4Mat& k, const Kv4Mat& v,
                            hipStream_t st);
 
+constexpr uint32_t kKv4PartHead = 4;   // a partial result's words before its outputs
+
 struct Kv4Attend {
   Kv4 c;
   Kv4Rows r;
@@ -54,7 +56,7 @@ struct Kv4Attend {
   uint32_t hq;
   float scale;
   const float* sink;   // [hq] or nullptr
-  float* part;         // partials [rows][hq][nsplit][hd + 2], when nsplit > 1
+  float* part;         // partials [rows][hq][nsplit][kKv4PartHead + hd], when nsplit > 1
   uint32_t nsplit, tps;  // pieces of the slots, tiles each but the last
 };
 // how a call's slots are split (live: the most positions a sequence holds
@@ -63,7 +65,7 @@ struct Kv4Attend {
 void kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live, uint32_t* nsplit,
                uint32_t* tps);
 inline uint64_t kv4_part_floats(uint32_t rows, uint32_t hq, uint32_t hd, uint32_t nsplit) {
-  return nsplit > 1 ? (uint64_t)rows * hq * nsplit * (hd + 2) : 0;
+  return nsplit > 1 ? (uint64_t)rows * hq * nsplit * (kKv4PartHead + hd) : 0;
 }
 hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st);
 

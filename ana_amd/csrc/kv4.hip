@@ -280,6 +280,33 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8_t (&o)[N]) {
     }
 }
 
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+// split8 for probabilities (never next to the largest float): a part of two
+// in one conversion, and what it leaves of each, x - part, in one dot product
+// of two with (-1, 0) or (0, -1), exact as every term is
+template <int N>
+__device__ __forceinline__ void split8_p(const float (&x)[8], bf16x8_t (&o)[N]) {
+  // (kept from the compiler, which writes the first as the inline constant
+  // -1.0, and that one is the second)
+  uint32_t c0 = 0x0000BF80u, c1 = 0xBF800000u;
+  asm("" : "+v"(c0), "+v"(c1));
+  const bf16x2_t m0 = __builtin_bit_cast(bf16x2_t, c0), m1 = __builtin_bit_cast(bf16x2_t, c1);
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    f32x2_t r = {x[e], x[e + 1]};
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const bf16x2_t h = __builtin_convertvector(r, bf16x2_t);
+      o[n][e] = h[0];
+      o[n][e + 1] = h[1];
+      if (n + 1 < N) {
+        r[0] = __builtin_amdgcn_fdot2_f32_bf16(h, m0, r[0], false);
+        r[1] = __builtin_amdgcn_fdot2_f32_bf16(h, m1, r[1], false);
+      }
+    }
+  }
+}
+
 // a record as a lane reads it
 template <int D>
 struct Raw {
@@ -333,11 +360,11 @@ __device__ __forceinline__ bf16x8_t key_op(const Raw<D>& r, int h, int s, float 
 }
 // the value operands of dims m D / 16 + 2 u and + 1 over the lane's eight slots
 template <int D, int U>
-__device__ __forceinline__ void val_ops(const Raw<D>& r, const float (&sc)[8], bf16x8_t& a, bf16x8_t& b) {
+__device__ __forceinline__ void val_ops(const uint32_t (&w)[D / 16], const float (&sc)[8], bf16x8_t& a, bf16x8_t& b) {
   uint32_t x[8];
   static_for<8>([&](auto e_) {
     constexpr int e = decltype(e_)::value, byte = e * (D / 32) + U;
-    x[e] = two_of<byte % 4>(r.v[byte / 4], sc[e]);
+    x[e] = two_of<byte % 4>(w[byte / 4], sc[e]);
   });
   u32x4_t lo, hi;
 #pragma unroll
@@ -366,83 +393,61 @@ __device__ __forceinline__ uint32_t pair_or(uint32_t x) {
   return x | __shfl_xor(x, 32, 64);
 }
 
-// What a workgroup's pairs see: slot s holds a position of the ring's last
-// turn (up to slot cur) or of the one before.
+// What a workgroup's pairs see. Slot s holds the position back(s) before the
+// sequence's last one, last; a pair `ago` positions before the last sees the
+// slots that are live and as far back or farther.
 struct View {
-  uint32_t cur, live;   // the last position's slot; live slots
-  int64_t turn;         // position of slot 0 in the last turn
-  uint32_t slots;
+  uint32_t slots, cur, live;   // the ring's; the last position's; live ones
   __device__ __forceinline__ View(uint32_t last, uint32_t slots_) : slots(slots_) {
     cur = last % slots;
-    turn = (int64_t)last - cur;
     live = last < slots ? last + 1 : slots;
   }
-  __device__ __forceinline__ bool sees(uint32_t s, uint32_t p) const {
-    const int64_t at = s <= cur ? turn + s : turn - slots + s;
-    return s < live && at <= (int64_t)p;
-  }
-  // whether every slot of tile t is live and holds a position up to p (the
-  // positions above p are those of slots after p's up to cur)
-  __device__ __forceinline__ bool whole(uint32_t t, uint32_t last, uint32_t p) const {
+  __device__ __forceinline__ uint32_t back(uint32_t s) const { return s <= cur ? cur - s : cur + slots - s; }
+  __device__ __forceinline__ bool sees(uint32_t s, uint32_t ago) const { return s < live && back(s) >= ago; }
+  // whether every slot of tile t is live and `ago` back or more (those that
+  // are not are the `ago` slots up to cur, round the ring)
+  __device__ __forceinline__ bool whole(uint32_t t, uint32_t ago) const {
     const uint32_t s0 = t * 32, s1 = s0 + 31;
     if (s1 >= live) return false;
-    if (last == p) return true;
-    if (last - p >= slots) return false;
-    const uint32_t a = (p + 1) % slots;
-    return a <= cur ? (s1 < a || s0 > cur) : (s1 < a && s0 > cur);
+    if (ago == 0) return true;
+    if (ago >= slots) return false;
+    return ago <= cur + 1 ? (s1 + ago < cur + 1 || s0 > cur) : (s1 + ago < cur + 1 + slots && s0 > cur);
   }
 };
 
-// Pairs of a sequence: c = row * G + query head within the key head's group.
-// One tile's scores for 16 pairs, its probabilities and their product with
-// the values, with the pairs' running maxima and sums; K and V operands come
-// from key(h, s) and val(t).
-template <int D, int NPP>
-struct Acc {
-  f32x4_t o[D / 16];
-  float m, l;
-  uint32_t nan;   // blocks of dims that a seen value which is not finite makes so
-  __device__ __forceinline__ void clear() {
-#pragma unroll
-    for (int t = 0; t < D / 16; t++) o[t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    m = -INFINITY;
-    l = 0.0f;
-    nan = 0;
-  }
-  // scores (already scaled to base 2, masked) of the pair's eight slots of a
-  // tile: the probabilities in parts
-  __device__ __forceinline__ void soften(float (&x)[8], bf16x8_t (&p)[NPP]) {
-    float t = x[0];
-#pragma unroll
-    for (int e = 1; e < 8; e++) t = fmaxf(t, x[e]);
-    t = pair_max(t);
-    if (__any(t > m)) {
-      const float n = fmaxf(m, t);
-      const float f = n == m ? 1.0f : __builtin_amdgcn_exp2f(m - n);
-      m = n;
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < D / 16; i++) o[i] *= f;
-    }
-    const float b = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      x[e] = __builtin_amdgcn_exp2f(x[e] - b);
-      l += x[e];
-    }
-    split8(x, p);
-  }
-};
+constexpr float kLog2e = 1.4426950408889634f;
+// a piece's partial result: its maximum and sum, then (on 16 bytes) its D outputs
+constexpr uint32_t kPartHead = kKv4PartHead;
+// pairs of a sequence up to which the few-row kernel takes it
+constexpr uint32_t kFewPairs = 16;
+// A running maximum is only raised once a score passes it by this much (in
+// base 2): probabilities then reach 2^kSlack, which costs f32 and bf16 no
+// digit, and most tiles rescale nothing.
+constexpr float kSlack = 10.0f;
 
+// The queries' scale: f32 queries carry it (times log2 e) into their parts,
+// 16-bit ones enter as they are and only take its sign.
+template <typename T>
+__device__ __forceinline__ float query_factor(float sc) {
+  if constexpr (sizeof(T) == 4) return sc;
+  return sc < 0.0f ? -1.0f : 1.0f;
+}
+template <typename T>
+__device__ __forceinline__ float score_factor(float sc) {
+  if constexpr (sizeof(T) == 4) return 1.0f;
+  return fabsf(sc);
+}
 // the query operand of a pair: dims j D / 4 + 8 s + e of its row, in parts
 template <typename T, int D, int NP>
 __device__ __forceinline__ void query_ops(const Kv4Mat& q, uint32_t row, uint32_t head, uint32_t j, bool on, bool vec,
-                                          bf16x8_t (&o)[NP][D / 32]) {
+                                          float f, bf16x8_t (&o)[NP][D / 32]) {
   const T* p = (const T*)q.p + (uint64_t)row * q.row + (uint64_t)head * q.head + j * (D / 4);
 #pragma unroll
   for (int s = 0; s < D / 32; s++) {
     float x[8] = {};
     if (on) load8(p + 8 * s, vec, x);
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] *= f;
     bf16x8_t t[NP];
     split8(x, t);
 #pragma unroll
@@ -450,42 +455,84 @@ __device__ __forceinline__ void query_ops(const Kv4Mat& q, uint32_t row, uint32_
   }
 }
 
-constexpr float kLog2e = 1.4426950408889634f;
-// pairs of a sequence up to which the few-row kernel takes it
-constexpr uint32_t kFewPairs = 16;
-
-// a pair's finished output dims j D / 4 .. (n = D / 4 of them in a lane):
-// with a sink, then normalised
-template <typename T>
+// the weight of what was summed with maximum m, and the denominator, with the
+// head's sink
 __device__ __forceinline__ float finish_sum(float m, float l, const float* sink, uint32_t head, float* f) {
-  // the weight of what was summed with maximum m, and the denominator
-  float den = l;
   *f = 1.0f;
-  if (sink) {
-    const float s = sink[head] * kLog2e;
-    const float n = fmaxf(m, s);
-    if (n != -INFINITY) {
-      *f = __builtin_amdgcn_exp2f(m - n);
-      den = l * *f + __builtin_amdgcn_exp2f(s - n);
-    }
-    if (s != s) den = s;
-  }
-  return den;
+  if (!sink) return l;
+  const float s = sink[head] * kLog2e;
+  const float n = fmaxf(m, s);
+  if (s != s) return s;
+  if (n == -INFINITY) return l;
+  *f = __builtin_amdgcn_exp2f(m - n);
+  return l * *f + __builtin_amdgcn_exp2f(s - n);
 }
+
+// blocks of values that are not finite among those a pair sees, a bit a block
+// of dims (read again: the rare path)
+template <int D>
+__device__ __forceinline__ uint32_t nan_blocks(const uint8_t* rec, uint32_t tile, const View& view, uint32_t ago, uint32_t j) {
+  uint32_t n = 0;
+  const uint8_t* vs = rec + 33 * D + j * 8;
+#pragma unroll 1
+  for (uint32_t e = 0; e < 8; e++) {
+    if (!view.sees(tile * 32 + 16 * (e / 4) + 4 * j + e % 4, ago)) continue;
+#pragma unroll
+    for (uint32_t b = 0; b < D / 32; b++) n |= vs[b * 32 + e] == 255 ? 1u << b : 0u;
+  }
+  return n;
+}
+// the value scales of slots that are not live, and of blocks that are not
+// finite, as 2^-127
+__device__ __forceinline__ void quiet_values(uint32_t (&vs)[2], uint32_t tile, uint32_t live, uint32_t j) {
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const uint32_t mask = 0xFFu << (8 * (e % 4));
+    if (tile * 32 + 16 * (e / 4) + 4 * j + e % 4 >= live || (vs[e / 4] & mask) == mask) vs[e / 4] &= ~mask;
+  }
+}
+template <int D>
+__device__ __forceinline__ bool not_finite(const Raw<D>& r) {
+  return has255(r.ks) | has255(r.vs[0]) | has255(r.vs[1]);
+}
+__device__ __forceinline__ bf16x8_t nan_op() {
+  const u32x4_t n = {0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
+  return __builtin_bit_cast(bf16x8_t, n);
+}
+
+// u's DPP move within its quad of lanes
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad(uint32_t u) {
+  return (uint32_t)__builtin_amdgcn_mov_dpp((int)u, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t quad(float f) { return quad<CTRL>(__builtin_bit_cast(uint32_t, f)); }
 
 // Few rows (up to 16 pairs of one sequence and key head): one workgroup per
 // (sequence, key head, piece of the slots), its four waves taking every
 // fourth tile with the next one's loads in flight, each with a running
-// softmax of its own; they meet in LDS. Bound by the records' bytes.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint32_t nt16) {
-  constexpr int NP = Parts<T>::q, NPP = Parts<T>::p;
+// softmax of its own; they meet in LDS.
+//
+// Pairs are few against the 16 columns of an MFMA, so with NC = 2 or 4 a pair
+// takes NC neighbouring columns, one for each part: of the query in the first
+// product (whose columns' sum is the score) and of the probability in the
+// second, one MFMA each where NC = 1 takes one a part. A lane of the NC then
+// has exponentials to take for only 8 / NC of its slots, which its neighbours
+// get by DPP moves. (256 sequences of 2048 slots, 12 heads of 64, f32: a tile
+// costs 320 vector instructions and 24 MFMAs with NC = 1, where the vector
+// units were busy 87% of 128 us.)
+template <typename T, int D, int NC>
+__global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint32_t ncol) {
+  constexpr int NP = Parts<T>::q, QP = NC == 1 ? NP : 1, NPP = NC == 1 ? Parts<T>::p : 1;
+  constexpr int PC = 16 / NC;          // pairs a workgroup
+  constexpr int OWN = NC == 1 ? 4 : 4 / NC;  // slots of four that a lane takes exponentials of
   __shared__ float om[4][16][D + 4];
   __shared__ float mm[4][16], ll[4][16];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, m = lane & 15, j = lane >> 4;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, j = lane >> 4;
+  const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t w = blockIdx.x;
-  const uint32_t sub = w % nt16;
-  w /= nt16;
+  const uint32_t sub = w % ncol;
+  w /= ncol;
   const uint32_t head = w % a.c.heads, i = w / a.c.heads, z = blockIdx.y;
   const uint32_t G = a.hq / a.c.heads;
   uint32_t row0 = i, len = 1;
@@ -494,178 +541,270 @@ __global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint
     if (o1 <= o0 || o1 > a.r.rows) return;
     row0 = o0;
     len = o1 - o0;
-    if ((uint64_t)len * G > kFewPairs) return;
+    if (len > kFewPairs || len * G > kFewPairs) return;
   }
   const uint32_t q = a.r.seq ? a.r.seq[i] : i;
-  const uint32_t pos = a.r.pos[i], last = pos + len - 1;
-  const uint32_t np = min(len * G - sub * 16, 16u);   // pairs here
-  const uint32_t c0 = sub * 16;
+  const uint32_t last = a.r.pos[i] + len - 1;
+  const uint32_t c0 = sub * PC, np = min(len * G - c0, (uint32_t)PC);   // the pairs here
   const bool ok = q < a.c.seqs;
   const View view(last, a.c.slots);
   const uint32_t tiles = ok ? (view.live + 31) / 32 : 0u;
   const uint32_t t0 = z * a.tps, t1 = z + 1 == a.nsplit ? tiles : min(tiles, t0 + a.tps);
   if (a.nsplit > 1 && t0 >= t1) return;
-  const uint32_t pr = c0 + m, t = pr / G, g = pr % G;
-  const bool on = m < np;
-  bf16x8_t qo[NP][D / 32];
-  query_ops<T, D, NP>(a.q, row0 + t, head * G + g, j, on, vec, qo);
-  const uint32_t p = pos + t;
+  const uint32_t pm = m / NC, part = m % NC;
+  const uint32_t t = (c0 + pm) / G, g = (c0 + pm) % G;
   const float sc = a.scale * kLog2e;
-  Acc<D, NPP> acc;
-  acc.clear();
-  const uint8_t* base = record_of(a.c, ok ? q : 0, head, 0);
-  Raw<D> cur, nxt;
-  uint32_t tile = t0 + wv;
-  if (tile < t1) {
-    load_k(cur, base + (uint64_t)tile * (34 * D), lane);
-    load_v(cur, base + (uint64_t)tile * (34 * D), lane);
-  }
-  for (; tile < t1; tile += 4) {
-    if (tile + 4 < t1) {
-      load_k(nxt, base + (uint64_t)(tile + 4) * (34 * D), lane);
-      load_v(nxt, base + (uint64_t)(tile + 4) * (34 * D), lane);
-    }
-    const bool whole = view.whole(tile, last, pos);
-    if (!whole) {
-      // the values of slots that hold nothing are not to count
+  bf16x8_t qo[QP][D / 32];
+  {
+    bf16x8_t all[NP][D / 32];
+    query_ops<T, D, NP>(a.q, row0 + t, head * G + g, j, pm < np, vec, query_factor<T>(sc), all);
+    if constexpr (NC == 1) {
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (tile * 32 + 16 * (e / 4) + 4 * j + e % 4 >= view.live) cur.vs[e / 4] &= ~(0xFFu << (8 * (e % 4)));
+      for (int n = 0; n < NP; n++)
+#pragma unroll
+        for (int d = 0; d < D / 32; d++) qo[n][d] = all[n][d];
+    } else {
+#pragma unroll
+      for (int d = 0; d < D / 32; d++) {
+        u32x4_t o = __builtin_bit_cast(u32x4_t, all[0][d]);
+        if constexpr (NP > 1) {
+          const u32x4_t o1 = __builtin_bit_cast(u32x4_t, all[1][d]), o2 = __builtin_bit_cast(u32x4_t, all[NP - 1][d]);
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e] = part == 0 ? o[e] : part == 1 ? o1[e] : part < NP ? o2[e] : 0u;
+        }
+        qo[0][d] = __builtin_bit_cast(bf16x8_t, o);
+      }
     }
-    const bool bad = __any(has255(cur.ks) | has255(cur.vs[0]) | has255(cur.vs[1]));
+  }
+  const float sf = score_factor<T>(sc);
+  const uint32_t ago = len - 1 - t;   // positions from the pair's to the last
+  // a probability's part of this column, p & pm1 less p & pm0: eight bits each
+  const uint32_t pm1 = part == 0 ? 0xFFFF0000u : part == 1 ? 0xFFFFFF00u : 0xFFFFFFFFu;
+  const uint32_t pm0 = part == 0 ? 0u : part == 1 ? 0xFFFF0000u : part == 2 ? 0xFFFFFF00u : 0xFFFFFFFFu;
+  f32x4_t o[D / 16];
+#pragma unroll
+  for (int d = 0; d < D / 16; d++) o[d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float mx = -INFINITY, l = 0.0f;
+  uint32_t nan = 0;
+  const uint8_t* base = record_of(a.c, ok ? q : 0, head, 0);
+
+  auto load = [&](Raw<D>& r, uint32_t tile) {
+    const uint8_t* rec = base + (uint64_t)min(tile, t1 - 1) * (34 * D);
+    load_k(r, rec, lane);
+    load_v(r, rec, lane);
+  };
+  auto tile_of = [&](Raw<D>& r, uint32_t tile) {
+    const bool whole = view.whole(tile, len - 1);
+    const bool bad = __any(not_finite(r));
     f32x4_t s[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       s[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-      const float ksc = scale_of(cur.ks, h);
+      const float ksc = scale_of(r.ks, h);
 #pragma unroll
       for (int d = 0; d < D / 32; d++) {
-        bf16x8_t ko = key_op<D>(cur, h, d, ksc);
-        if (bad && ((cur.ks >> (8 * h)) & 0xFF) == 255) {
-          const u32x4_t nn = {0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
-          ko = __builtin_bit_cast(bf16x8_t, nn);
+        bf16x8_t ko = key_op<D>(r, h, d, ksc);
+        if (bad && ((r.ks >> (8 * h)) & 0xFF) == 255) ko = nan_op();
+#pragma unroll
+        for (int n = 0; n < QP; n++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ko, qo[n][d], s[h], 0, 0, 0);
+      }
+    }
+    // the scores that this lane goes on with: all, or (NC > 1) of slots 4 j +
+    // i those with i mod NC its column's, over the NC columns' sum
+    float x[2 * OWN];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      if constexpr (NC == 1) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[4 * h + e] = s[h][e];
+      } else {
+        float u[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          u[e] = part & 1 ? s[h][2 * e + 1] : s[h][2 * e];
+          if constexpr (NP > 1)
+            u[e] += __builtin_bit_cast(float, quad<0xB1>(part & 1 ? s[h][2 * e] : s[h][2 * e + 1]));
         }
-#pragma unroll
-        for (int n = 0; n < NP; n++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ko, qo[n][d], s[h], 0, 0, 0);
+        if constexpr (NC == 2) {
+          x[2 * h] = u[0];
+          x[2 * h + 1] = u[1];
+        } else {
+          x[h] = (part & 2 ? u[1] : u[0]) + __builtin_bit_cast(float, quad<0x4E>(part & 2 ? u[0] : u[1]));
+        }
       }
     }
-    float x[8];
+    if (!whole || bad) {
 #pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = s[e / 4][e % 4] * sc;
-    if (!whole) {
-#pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (!view.sees(tile * 32 + 16 * (e / 4) + 4 * j + e % 4, p)) x[e] = -INFINITY;
-    }
-    if (bad) {
-      // a value block that is not finite counts for the pairs that see it
-      // alone: out of the product, and into their dims at the end
-      const uint8_t* vs = base + (uint64_t)tile * (34 * D) + 33 * D + j * 8;
-      for (int e = 0; e < 8; e++) {
-        const uint32_t slot = tile * 32 + 16 * (e / 4) + 4 * j + e % 4;
-        if (!view.sees(slot, p)) continue;
-        for (int b = 0; b < D / 32; b++)
-          if (vs[b * 32 + e] == 255) acc.nan |= 1u << b;
+      for (int e = 0; e < 2 * OWN; e++) {
+        const uint32_t in4 = NC == 1 ? e % 4 : NC == 2 ? 2 * (e % 2) + part : part;
+        if (!view.sees(tile * 32 + 16 * (e / OWN) + 4 * j + in4, ago)) x[e] = -INFINITY;
       }
+      if (bad) nan |= nan_blocks<D>(base + (uint64_t)tile * (34 * D), tile, view, ago, j);
+      quiet_values(r.vs, tile, view.live, j);
+    }
+    float top = x[0];
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (((cur.vs[e / 4] >> (8 * (e % 4))) & 0xFF) == 255) cur.vs[e / 4] &= ~(0xFFu << (8 * (e % 4)));
+    for (int e = 1; e < 2 * OWN; e++) top = fmaxf(top, x[e]);
+    if (__any(top * sf > mx + kSlack)) {
+      if constexpr (NC >= 2) top = fmaxf(top, __builtin_bit_cast(float, quad<0xB1>(top)));
+      if constexpr (NC >= 4) top = fmaxf(top, __builtin_bit_cast(float, quad<0x4E>(top)));
+      const float n = fmaxf(mx, pair_max(top) * sf);
+      const float f = n == mx ? 1.0f : __builtin_amdgcn_exp2f(mx - n);
+      mx = n;
+      l *= f;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) o[d] *= f;
+    }
+    const float b = mx == -INFINITY ? 0.0f : mx;
+#pragma unroll
+    for (int e = 0; e < 2 * OWN; e++) {
+      x[e] = __builtin_amdgcn_exp2f(sizeof(T) == 4 ? x[e] - b : fmaf(x[e], sf, -b));
+      l += x[e];
     }
     bf16x8_t po[NPP];
-    acc.soften(x, po);
+    if constexpr (NC == 1) {
+      split8_p(x, po);
+    } else {
+      u32x4_t pk;
+      static_for<4>([&](auto e_) {
+        constexpr int e = decltype(e_)::value;   // slots 2 e and 2 e + 1 of the eight
+        uint32_t v[2];
+        static_for<2>([&](auto i_) {
+          constexpr int i = decltype(i_)::value, in4 = (2 * e + i) % 4, h = e / 2;
+          uint32_t u;
+          if constexpr (NC == 4) u = quad<in4 * 0x55>(x[h]);
+          else u = quad<in4 % 2 ? 0xF5 : 0xA0>(x[2 * h + in4 / 2]);
+          v[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, u & pm1) - __builtin_bit_cast(float, u & pm0));
+        });
+        pk[e] = __builtin_amdgcn_perm(v[1], v[0], 0x07060302u);
+      });
+      po[0] = __builtin_bit_cast(bf16x8_t, pk);
+    }
     float vsc[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) vsc[e] = scale_of(cur.vs[e / 4], e % 4);
+    for (int e = 0; e < 8; e++) vsc[e] = scale_of(r.vs[e / 4], e % 4);
     static_for<D / 32>([&](auto u_) {
       constexpr int u = decltype(u_)::value;
       bf16x8_t v0, v1;
-      val_ops<D, u>(cur, vsc, v0, v1);
+      val_ops<D, u>(r.v, vsc, v0, v1);
 #pragma unroll
       for (int n = 0; n < NPP; n++) {
-        acc.o[2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, po[n], acc.o[2 * u], 0, 0, 0);
-        acc.o[2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, po[n], acc.o[2 * u + 1], 0, 0, 0);
+        o[2 * u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v0, po[n], o[2 * u], 0, 0, 0);
+        o[2 * u + 1] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v1, po[n], o[2 * u + 1], 0, 0, 0);
       }
     });
-    cur = nxt;
+  };
+  {
+    Raw<D> ra, rb;
+    uint32_t tile = t0 + wv;
+    if (tile < t1) {
+      load(ra, tile);
+#pragma unroll 1
+      for (;;) {
+        load(rb, tile + 4);
+        tile_of(ra, tile);
+        tile += 4;
+        if (tile >= t1) break;
+        load(ra, tile + 4);
+        tile_of(rb, tile);
+        tile += 4;
+        if (tile >= t1) break;
+      }
+    }
   }
   // the four waves meet
-  const float l = pair_sum(acc.l);
-  const uint32_t nan = pair_or(acc.nan);
-  if (j == 0) {
-    mm[wv][m] = acc.m;
-    ll[wv][m] = l;
+  l = pair_sum(l);
+  nan = pair_or(nan);
+  if constexpr (NC >= 2) l += __builtin_bit_cast(float, quad<0xB1>(l));
+  if constexpr (NC >= 4) l += __builtin_bit_cast(float, quad<0x4E>(l));
+  if (j == 0 && part == 0) {
+    mm[wv][pm] = mx;
+    ll[wv][pm] = l;
   }
 #pragma unroll
   for (int i4 = 0; i4 < 4; i4++)
 #pragma unroll
     for (int t16 = 0; t16 < D / 16; t16++) {
       const uint32_t d = j * (D / 4) + i4 * (D / 16) + t16;
-      om[wv][m][d] = (nan >> (d / 32)) & 1 ? __builtin_nanf("") : acc.o[t16][i4];
+      om[wv][m][d] = (nan >> (d / 32)) & 1 ? __builtin_nanf("") : o[t16][i4];
     }
   __syncthreads();
   for (uint32_t k = tid; k < np * D; k += 256) {
     const uint32_t pp = k / D, d = k % D;
     const float M = fmaxf(fmaxf(mm[0][pp], mm[1][pp]), fmaxf(mm[2][pp], mm[3][pp]));
-    float lsum = 0.0f, o = 0.0f;
+    float lsum = 0.0f, y = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
       // (a wave without a seen slot has nothing, but a score that is not a number stays one)
       const float f = mm[u][pp] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm[u][pp] - M);
       lsum += ll[u][pp] * f;
-      o += om[u][pp][d] * f;
+      float v = om[u][pp * NC][d];
+#pragma unroll
+      for (int n = 1; n < NC; n++) v += om[u][pp * NC + n][d];
+      y += v * f;
     }
     const uint32_t row = row0 + (c0 + pp) / G, hd = head * G + (c0 + pp) % G;
     if (a.nsplit > 1) {
-      float* part = a.part + (((uint64_t)row * a.hq + hd) * a.nsplit + z) * (D + 2);
-      part[2 + d] = o;
+      float* out = a.part + (((uint64_t)row * a.hq + hd) * a.nsplit + z) * (D + kPartHead);
+      out[kPartHead + d] = y;
       if (d == 0) {
-        part[0] = M;
-        part[1] = lsum;
+        out[0] = M;
+        out[1] = lsum;
       }
     } else {
       float f;
-      const float den = finish_sum<T>(M, lsum, a.sink, hd, &f);
-      const float y = ok && (den != 0.0f) ? o * f / den : 0.0f;
-      ((T*)a.o.p)[(uint64_t)row * a.o.row + (uint64_t)hd * a.o.head + d] = (T)y;
+      const float den = finish_sum(M, lsum, a.sink, hd, &f);
+      ((T*)a.o.p)[(uint64_t)row * a.o.row + (uint64_t)hd * a.o.head + d] = (T)(ok && den != 0.0f ? y * f / den : 0.0f);
     }
   }
 }
 
 // Many rows (more than 16 pairs of one sequence and key head): a workgroup
-// takes 64 NQ pairs, 16 NQ a wave, over the slots they see, 64 at a time.
-// Each wave turns one of the step's four halves (two tiles' keys, two tiles'
-// values) into operands in LDS, lane by lane as the MFMAs want them, so
-// every read and write there is a lane's own 16 bytes; the step's records
-// were loaded a step ahead, and two sets of operands leave one barrier a
-// step.
+// takes 64 NQ pairs, 16 NQ a wave, over the tiles they see, one at a time.
+// Its waves turn the tile into operands in LDS (a wave the keys of 16 slots,
+// or half of the values' dims), lane by lane as the MFMAs want them, so every
+// read and write there is a lane's own 16 bytes; the next tile's record is
+// loaded a tile ahead, and two sets of operands leave one barrier a tile. The
+// vector units (softmax and parts) and the matrix cores bind about equally,
+// so what counts is that a SIMD holds three such waves of different
+// workgroups to overlap them. bf16 outputs take a probability rounded once to
+// bf16, and the denominator the sum of the rounded ones (a second part was 8
+// of 24 MFMAs a tile and 16 pairs at hd 128).
 template <typename T, int D>
 struct Many {
   // pairs a wave: the queries' parts and the outputs share its registers
   static constexpr int NQ = D == 128 && Parts<T>::q > 1 ? 1 : 2;
+  static constexpr int NPP = Parts<T>::q == 1 ? 1 : Parts<T>::p;
   static constexpr uint32_t pairs = 64 * NQ;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 2) void k_kv4_many(Kv4Attend a, uint32_t vec) {
-  constexpr int NP = Parts<T>::q, NPP = Parts<T>::p, NQ = Many<T, D>::NQ;
+__global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) {
+  constexpr int NP = Parts<T>::q, NPP = Many<T, D>::NPP, NQ = Many<T, D>::NQ;
   constexpr uint32_t PW = Many<T, D>::pairs;
-  constexpr int KOPS = 2 * (D / 32), VOPS = D / 16;     // operands a tile
-  __shared__ bf16x8_t kop[2][2][KOPS][64], vop[2][2][VOPS][64];
+  constexpr int KS = D / 32, OPS = D / 16;     // steps of a key operand, operands of a tile's keys (values)
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr uint32_t OR = D + 4;               // a row of outputs in LDS
+  constexpr size_t LDS = std::max<size_t>(2 * 2 * OPS * 64 * 16, 4 * 16 * OR * 4);
+  __shared__ __align__(16) char lds[LDS];
   __shared__ uint32_t flag[2][4];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6, m = lane & 15, j = lane >> 4;
+  bf16x8_t(*ops)[2][OPS][64] = reinterpret_cast<bf16x8_t(*)[2][OPS][64]>(lds);   // [buffer][keys, values]
+  const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, j = lane >> 4;
+  const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t head = blockIdx.y, z = blockIdx.z, G = a.hq / a.c.heads;
   // the workgroup's sequence and its part of that sequence's pairs
   uint32_t i = 0, part_i = 0, before = 0;
   bool found = false;
+#pragma unroll 1
   for (uint32_t b = 0; b < a.r.n && !found; b += 64) {
     uint32_t nt = 0;
     if (b + lane < a.r.n) {
       const uint32_t o0 = a.r.off[b + lane], o1 = a.r.off[b + lane + 1];
-      const uint64_t pairs = o1 > o0 && o1 <= a.r.rows ? (uint64_t)(o1 - o0) * G : 0;
-      nt = pairs > kFewPairs ? (uint32_t)((pairs + PW - 1) / PW) : 0;
+      const uint32_t pairs = o1 > o0 && o1 <= a.r.rows ? (o1 - o0) * G : 0;
+      nt = pairs > kFewPairs ? (pairs + PW - 1) / PW : 0;
     }
     uint32_t sum = nt;
-#pragma unroll
+#pragma unroll 1
     for (int k = 1; k < 64; k <<= 1) {
       const uint32_t o = __shfl_up(sum, k, 64);
       if (lane >= (uint32_t)k) sum += o;
@@ -674,205 +813,267 @@ __global__ __launch_bounds__(256, 2) void k_kv4_many(Kv4Attend a, uint32_t vec) 
     if (hit) {
       const int f = __ffsll((long long)hit) - 1;
       i = b + f;
-      part_i = blockIdx.x - before - (__shfl(sum, f, 64) - __shfl(nt, f, 64));
+      // (a sequence's last rows see the most: they start first)
+      part_i = before + __shfl(sum, f, 64) - 1 - blockIdx.x;
       found = true;
     } else {
       before += __shfl(sum, 63, 64);
     }
   }
   if (!found) return;
+  i = __builtin_amdgcn_readfirstlane(i);
+  part_i = __builtin_amdgcn_readfirstlane(part_i);
   const uint32_t row0 = a.r.off[i], len = a.r.off[i + 1] - row0;
   const uint32_t q = a.r.seq ? a.r.seq[i] : i;
   const bool ok = q < a.c.seqs;
   const uint32_t pos = a.r.pos[i], last = pos + len - 1;
-  const uint64_t all = (uint64_t)len * G;
-  const uint64_t c0 = (uint64_t)part_i * PW;
+  const uint32_t all = len * G, c0 = part_i * PW;   // (rows x query heads < 2^31)
   const View view(last, a.c.slots);
-  const uint32_t p_lo = pos + (uint32_t)(c0 / G), p_hi = pos + (uint32_t)((min(all, c0 + PW) - 1) / G);
+  const uint32_t t_lo = c0 / G, t_hi = (min(all, c0 + PW) - 1) / G;
   // before the ring wraps, slots past the last row's position hold nothing
   // that any of the pairs sees
-  const uint32_t seen = last < a.c.slots ? p_hi + 1 : view.live;
+  const bool flat = last < a.c.slots;
+  const uint32_t seen = flat ? pos + t_hi + 1 : view.live;
   const uint32_t tiles = ok ? (seen + 31) / 32 : 0u;
   const uint32_t t0 = z * a.tps, t1 = z + 1 == a.nsplit ? tiles : min(tiles, t0 + a.tps);
 
-  bf16x8_t qo[NQ][NP][D / 32];
-  uint32_t p[NQ], wave_hi = 0;
-  uint64_t c[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; n++) {
-    c[n] = c0 + (wv * NQ + n) * 16 + m;
-    const bool on = c[n] < all;
-    const uint32_t t = on ? (uint32_t)(c[n] / G) : 0, g = on ? (uint32_t)(c[n] % G) : 0;
-    p[n] = pos + t;
-    query_ops<T, D, NP>(a.q, row0 + t, head * G + g, j, on, vec, qo[n]);
-  }
-  {
-    const uint64_t w0 = c0 + wv * NQ * 16;
-    wave_hi = w0 < all ? pos + (uint32_t)((min(all, w0 + NQ * 16) - 1) / G) : 0;
-    if (w0 >= all) wave_hi = pos;   // (its columns count for nothing)
-  }
-  const float sc = a.scale * kLog2e;
-  Acc<D, NPP> acc[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; n++) acc[n].clear();
   const uint8_t* base = record_of(a.c, ok ? q : 0, head, 0);
-  Raw<D> raw;
-  const uint32_t half = wv & 1;   // 0: keys, 1: values
-  auto load = [&](uint32_t step) {
-    const uint32_t tile = min(step + (wv >> 1), tiles - 1);
-    if (half == 0) load_k(raw, base + (uint64_t)tile * (34 * D), lane);
-    else load_v(raw, base + (uint64_t)tile * (34 * D), lane);
+  // a wave's part of a record: the key codes of slots m and 16 + m, or the
+  // value codes, and eight bytes with their scales; the same loads for both,
+  // so that they stay in flight through a tile
+  uint32_t rw[OPS], rs[2];
+  const uint32_t half = wv & 1;
+  const bool keys = wv < 2;
+  const uint32_t krow = j * D / 128 * 16 + m;   // this lane's key scales, two bytes each
+  const uint32_t w_at = (keys ? 0 : 16 * D) + lane * (D / 4);
+  const uint32_t s_at = keys ? 32 * D + (krow * 2 & ~7u) : 33 * D + (m * D / 512 * 4 + j) * 8;
+  auto load = [&](uint32_t tile) {
+    const uint8_t* rec = base + (uint64_t)tile * (34 * D);
+    load_words<D>(rw, rec + w_at);
+    const uint2 t = *reinterpret_cast<const uint2*>(rec + s_at);
+    rs[0] = t.x;
+    rs[1] = t.y;
   };
-  auto stage = [&](uint32_t step, uint32_t buf) {
-    const uint32_t rt = wv >> 1, tile = step + rt;
-    uint32_t bad;
-    if (half == 0) {
-      bad = has255(raw.ks);
+  auto stage = [&](uint32_t tile, uint32_t buf) {
+    bool bad;
+    if (keys) {
+      const uint32_t s0 = rs[0], s1 = rs[1], b8 = ((krow & 2 ? s1 : s0) >> ((krow & 1) * 16 + half * 8)) & 0xFF;
+      const float ksc = __builtin_bit_cast(float, b8 << 23);
+      bad = __any(b8 == 255);
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
-        const float ksc = scale_of(raw.ks, h);
-        const bool nan = ((raw.ks >> (8 * h)) & 0xFF) == 255;
-#pragma unroll
-        for (int d = 0; d < D / 32; d++) {
-          u32x4_t o = __builtin_bit_cast(u32x4_t, key_op<D>(raw, h, d, ksc));
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[e] = nan ? 0x7FC07FC0u : o[e];
-          kop[buf][rt][h * (D / 32) + d][lane] = __builtin_bit_cast(bf16x8_t, o);
-        }
+      for (int d = 0; d < KS; d++) {
+        const uint32_t w0 = rw[d], w1 = rw[KS + d], w = half ? w1 : w0;
+        const u32x4_t o = {two_of<0>(w, ksc), two_of<1>(w, ksc), two_of<2>(w, ksc), two_of<3>(w, ksc)};
+        bf16x8_t ko = __builtin_bit_cast(bf16x8_t, o);
+        if (bad && b8 == 255) ko = nan_op();
+        ops[buf][0][half * KS + d][lane] = ko;
       }
     } else {
-      bad = has255(raw.vs[0]) | has255(raw.vs[1]);
+      bad = __any(has255(rs[0]) | has255(rs[1]));
+      if (bad || tile * 32 + 32 > view.live) quiet_values(rs, tile, view.live, j);
       float vsc[8];
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const uint32_t slot = tile * 32 + 16 * (e / 4) + 4 * j + e % 4;
-        const uint32_t b = (raw.vs[e / 4] >> (8 * (e % 4))) & 0xFF;
-        vsc[e] = slot >= view.live || b == 255 ? 0.0f : __builtin_bit_cast(float, b << 23);
-      }
-      static_for<D / 32>([&](auto u_) {
+      for (int e = 0; e < 8; e++) vsc[e] = scale_of(rs[e / 4], e % 4);
+      static_for<KS>([&](auto u_) {
         constexpr int u = decltype(u_)::value;
-        val_ops<D, u>(raw, vsc, vop[buf][rt][2 * u][lane], vop[buf][rt][2 * u + 1][lane]);
+        if (half == (KS > 1 ? u / (KS / 2) : 0))
+          val_ops<D, u>(rw, vsc, ops[buf][1][2 * u][lane], ops[buf][1][2 * u + 1][lane]);
       });
     }
-    const bool any = __any(bad);
-    if (lane == 0) flag[buf][wv] = any;
+    if (lane == 0) flag[buf][wv] = bad;
   };
-  uint32_t buf = 0;
-  if (t0 < t1) {
-    load(t0);
-    stage(t0, 0);
-  }
-  __syncthreads();
-  for (uint32_t step = t0; step < t1; step += 2) {
-    const bool more = step + 2 < t1;
-    if (more) load(step + 2);
+  if (t0 < t1) load(t0);   // (in flight while the queries are read)
+
+  const float sc = a.scale * kLog2e;
+  bf16x8_t qo[NQ][NP][KS];
+  uint32_t ago[NQ];
 #pragma unroll
-    for (int rt = 0; rt < 2; rt++) {
-      const uint32_t tile = step + rt;
-      if (tile >= t1) break;
-      // a tile past every position of the wave's pairs (no wrap)
-      if (last < a.c.slots && tile * 32 > wave_hi) continue;
-      const bool whole = view.whole(tile, last, p_lo);
-      const bool bad = flag[buf][2 * rt + 1];
+  for (int n = 0; n < NQ; n++) {
+    const uint32_t c = c0 + (wv * NQ + n) * 16 + m;
+    const bool on = c < all;
+    const uint32_t t = on ? c / G : t_lo, g = on ? c % G : 0;
+    ago[n] = len - 1 - t;
+    query_ops<T, D, NP>(a.q, row0 + t, head * G + g, j, on, vec, query_factor<T>(sc), qo[n]);
+  }
+  // the last slot that a pair of this wave sees, where the ring has not wrapped
+  const uint32_t w0 = c0 + wv * NQ * 16;
+  const uint32_t wave_hi = w0 < all ? pos + (min(all, w0 + NQ * 16) - 1) / G : 0;
+  const float sf = score_factor<T>(sc);
+  f32x4_t o[NQ][OPS], less[NQ];
+  float mx[NQ], l[NQ];
+  uint32_t nan[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; n++) {
+    less[n] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int d = 0; d < OPS; d++) o[n][d] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    mx[n] = -INFINITY;
+    l[n] = 0.0f;
+    nan[n] = 0;
+  }
+  uint32_t buf = 0;
+  if (t0 < t1) stage(t0, 0);
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t tile = t0; tile < t1; tile++) {
+    const bool more = tile + 1 < t1;
+    if (more) load(tile + 1);
+    // (past every position of the wave's pairs: nothing to do)
+    if (!flat || tile * 32 <= wave_hi) {
+      const bool whole = view.whole(tile, len - 1 - t_lo);
+      const bool bad = flag[buf][2] | flag[buf][3];
+      // (f32 scores come out less their pair's maximum: the products start from it)
       f32x4_t s[NQ][2];
 #pragma unroll
-      for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = less[n];
 #pragma unroll
-      for (int d = 0; d < D / 32; d++)
+      for (int d = 0; d < KS; d++)
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const bf16x8_t ko = kop[buf][rt][h * (D / 32) + d][lane];
+          const bf16x8_t ko = ops[buf][0][h * KS + d][lane];
 #pragma unroll
-          for (int n = 0; n < NQ; n++)
+          for (int u = 0; u < NP; u++)
 #pragma unroll
-            for (int u = 0; u < NP; u++)
+            for (int n = 0; n < NQ; n++)
               s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ko, qo[n][u][d], s[n][h], 0, 0, 0);
         }
       bf16x8_t po[NQ][NPP];
+      float x[NQ][8];
+      bool raise = false;
+      float top[NQ];
+#pragma unroll
+      for (int n = 0; n < NQ; n++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[n][e] = s[n][e / 4][e % 4];
+      if (!whole) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const uint32_t slot = tile * 32 + 16 * (e / 4) + 4 * j + e % 4, back = view.back(slot);
+          const bool live = slot < view.live;
+#pragma unroll
+          for (int n = 0; n < NQ; n++) x[n][e] = live && back >= ago[n] ? x[n][e] : -INFINITY;
+        }
+      }
+      if (bad) {
+#pragma unroll 1
+        for (int n = 0; n < NQ; n++) {
+          const uint32_t t = nan_blocks<D>(base + (uint64_t)tile * (34 * D), tile, view, n ? ago[NQ - 1] : ago[0], j);
+          if (n == 0) nan[0] |= t;
+          else nan[NQ - 1] |= t;
+        }
+      }
 #pragma unroll
       for (int n = 0; n < NQ; n++) {
-        float x[8];
+        top[n] = x[n][0];
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = s[n][e / 4][e % 4] * sc;
-        if (!whole) {
+        for (int e = 1; e < 8; e++) top[n] = fmaxf(top[n], x[n][e]);
+        if constexpr (F32) raise |= top[n] > (mx[n] == -INFINITY ? mx[n] : kSlack);
+        else raise |= top[n] * sf > mx[n] + kSlack;
+      }
+      if (__any(raise)) {
 #pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (!view.sees(tile * 32 + 16 * (e / 4) + 4 * j + e % 4, p[n])) x[e] = -INFINITY;
-        }
-        if (bad) {
-          const uint8_t* vs = base + (uint64_t)tile * (34 * D) + 33 * D + j * 8;
-          for (int e = 0; e < 8; e++) {
-            if (!view.sees(tile * 32 + 16 * (e / 4) + 4 * j + e % 4, p[n])) continue;
-            for (int b = 0; b < D / 32; b++)
-              if (vs[b * 32 + e] == 255) acc[n].nan |= 1u << b;
+        for (int n = 0; n < NQ; n++) {
+          const float was = mx[n] == -INFINITY ? 0.0f : mx[n];
+          const float v = fmaxf(mx[n], F32 ? pair_max(top[n]) + was : pair_max(top[n]) * sf);
+          const float f = v == mx[n] ? 1.0f : __builtin_amdgcn_exp2f(mx[n] - v);
+          mx[n] = v;
+          if constexpr (F32) {
+            const float b = v == -INFINITY ? 0.0f : v;
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[n][e] -= b - was;
+            less[n] = f32x4_t{-b, -b, -b, -b};
           }
+          l[n] *= f;
+#pragma unroll
+          for (int d = 0; d < OPS; d++) o[n][d] *= f;
         }
-        acc[n].soften(x, po[n]);
       }
 #pragma unroll
-      for (int t = 0; t < D / 16; t++) {
-        const bf16x8_t vo = vop[buf][rt][t][lane];
+      for (int n = 0; n < NQ; n++) {
+        const float b = mx[n] == -INFINITY ? 0.0f : mx[n];
 #pragma unroll
-        for (int n = 0; n < NQ; n++)
+        for (int e = 0; e < 8; e++) x[n][e] = __builtin_amdgcn_exp2f(F32 ? x[n][e] : fmaf(x[n][e], sf, -b));
+        split8_p(x[n], po[n]);
+        if constexpr (NPP == 1) {
+          const bf16x2_t one = {(__bf16)1.0f, (__bf16)1.0f};
 #pragma unroll
-          for (int u = 0; u < NPP; u++)
-            acc[n].o[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, po[n][u], acc[n].o[t], 0, 0, 0);
+          for (int e = 0; e < 8; e += 2)
+            l[n] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{po[n][0][e], po[n][0][e + 1]}, one, l[n], false);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; e++) l[n] += x[n][e];
+        }
+      }
+#pragma unroll
+      for (int t = 0; t < OPS; t++) {
+        const bf16x8_t vo = ops[buf][1][t][lane];
+#pragma unroll
+        for (int u = 0; u < NPP; u++)
+#pragma unroll
+          for (int n = 0; n < NQ; n++)
+            o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, po[n][u], o[n][t], 0, 0, 0);
       }
     }
-    if (more) stage(step + 2, buf ^ 1);
+    if (more) stage(tile + 1, buf ^ 1);
     __syncthreads();
     buf ^= 1;
   }
+  // the outputs, 16 pairs at a time through the wave's part of LDS, so that a
+  // store's lanes write whole rows
+  float(*rows)[OR] = reinterpret_cast<float(*)[OR]>(lds + wv * (16 * OR * 4));
+  const bool split = a.nsplit > 1;
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
-    const float l = pair_sum(acc[n].l);
-    const uint32_t nan = pair_or(acc[n].nan);
-    if (c[n] >= all) continue;
-    const uint32_t row = row0 + (uint32_t)(c[n] / G), hd = head * G + (uint32_t)(c[n] % G);
-    if (a.nsplit > 1) {
-      float* part = a.part + (((uint64_t)row * a.hq + hd) * a.nsplit + z) * (D + 2);
+    const float ls = pair_sum(l[n]);
+    const uint32_t nn = pair_or(nan[n]);
+    float f = 1.0f, inv = 1.0f;
+    const uint32_t c = c0 + (wv * NQ + n) * 16 + m;
+    const bool on = c < all;
+    const uint32_t row = on ? row0 + c / G : row0, hq = on ? head * G + c % G : 0;
+    float* part = a.part + (((uint64_t)row * a.hq + hq) * a.nsplit + z) * (D + kPartHead);
+    if (!split) {
+      const float den = finish_sum(mx[n], ls, a.sink, hq, &f);
+      inv = ok && den != 0.0f ? f / den : 0.0f;
+    } else if (on && j == 0) {
+      part[0] = mx[n];
+      part[1] = ls;
+    }
 #pragma unroll
-      for (int i4 = 0; i4 < 4; i4++)
+    for (int i4 = 0; i4 < 4; i4++)
 #pragma unroll
-        for (int t = 0; t < D / 16; t++) {
-          const uint32_t d = j * (D / 4) + i4 * (D / 16) + t;
-          part[2 + d] = (nan >> (d / 32)) & 1 ? __builtin_nanf("") : acc[n].o[t][i4];
-        }
-      if (j == 0) {
-        part[0] = acc[n].m;
-        part[1] = l;
+      for (int t = 0; t < OPS; t += 2) {
+        const uint32_t d = j * (D / 4) + i4 * OPS + t;
+        const bool bad = (nn >> (d / 32)) & 1;
+        *reinterpret_cast<float2*>(&rows[m][d]) =
+            make_float2(bad ? __builtin_nanf("") : o[n][t][i4] * inv, bad ? __builtin_nanf("") : o[n][t + 1][i4] * inv);
       }
-    } else {
-      float f;
-      const float den = finish_sum<T>(acc[n].m, l, a.sink, hd, &f);
-      const float inv = ok && den != 0.0f ? f / den : 0.0f;
-      T* o = (T*)a.o.p + (uint64_t)row * a.o.row + (uint64_t)hd * a.o.head + j * (D / 4);
-      float y[D / 4];
+    __builtin_amdgcn_wave_barrier();
+    // where each pair's row goes, in elements (of the partials, or the outputs)
+    const uint64_t to = split ? (uint64_t)(part - a.part) + kPartHead : (uint64_t)row * a.o.row + (uint64_t)hq * a.o.head;
+    constexpr uint32_t LR = D / 8;   // lanes a row, eight outputs each
 #pragma unroll
-      for (int i4 = 0; i4 < 4; i4++)
-#pragma unroll
-        for (int t = 0; t < D / 16; t++) {
-          const uint32_t d = j * (D / 4) + i4 * (D / 16) + t;
-          const float v = acc[n].o[t][i4] * inv;
-          y[i4 * (D / 16) + t] = (nan >> (d / 32)) & 1 ? __builtin_nanf("") : v;
-        }
-#pragma unroll
-      for (int k = 0; k < D / 32; k++) {
-        float t8[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) t8[e] = y[8 * k + e];
-        store8(o + 8 * k, vec, t8);
+    for (uint32_t r = 0; r < 16; r += 64 / LR) {
+      const uint32_t pp = r + lane / LR, d = lane % LR * 8;
+      const uint64_t at = (uint64_t)(uint32_t)__shfl((uint32_t)(to >> 32), pp, 64) << 32 | (uint32_t)__shfl((uint32_t)to, pp, 64);
+      const bool mine = __shfl((int)on, pp, 64);
+      const f32x4_t y0 = *reinterpret_cast<const f32x4_t*>(&rows[pp][d]), y1 = *reinterpret_cast<const f32x4_t*>(&rows[pp][d + 4]);
+      const float y[8] = {y0[0], y0[1], y0[2], y0[3], y1[0], y1[1], y1[2], y1[3]};
+      if (mine) {
+        if (split) store8(a.part + at + d, true, y);
+        else store8((T*)a.o.p + at + d, vec, y);
       }
     }
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
 // The pieces of a (row, query head), a wave each: weights 2^(m_z - M), then
-// the sink, then the division. The few-row kernel writes no piece past its
+// the sink, then the division. D / 4 lanes take a piece's outputs, so several
+// pieces are in flight at once. The few-row kernel writes no piece past its
 // sequence's last slot; the other one writes all of them.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a) {
-  constexpr uint32_t R = D / 32;
+  constexpr uint32_t L = D / 4, GR = 64 / L;   // lanes a piece, pieces at once
   const uint32_t lane = threadIdx.x & 63;
   const uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const uint32_t row = (uint32_t)(w / a.hq), hd = (uint32_t)(w % a.hq);
@@ -890,27 +1091,36 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a) {
   const View view(a.r.pos[i] + len - 1, a.c.slots);
   uint32_t nz = min(a.nsplit, ((view.live + 31) / 32 + a.tps - 1) / a.tps);
   if (q >= a.c.seqs) nz = 0;
-  const float* part = a.part + ((uint64_t)row * a.hq + hd) * a.nsplit * (D + 2);
+  const float* part = a.part + ((uint64_t)row * a.hq + hd) * a.nsplit * (D + kPartHead);
   float M = -INFINITY;
-  for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, part[(uint64_t)z * (D + 2)]);
+  for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, part[z * (D + kPartHead)]);
   M = wmax(M);
-  float l = 0.0f, o[(R + 1) / 2] = {};
-  for (uint32_t z = 0; z < nz; z++) {
-    const float* p = part + (uint64_t)z * (D + 2);
+  const uint32_t g = lane / L, d = lane % L * 4;
+  float l = 0.0f;
+  f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t z = g; z < nz; z += GR) {
+    const float* p = part + z * (D + kPartHead);
+    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p + kPartHead + d);
     const float m = p[0];
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
     l += p[1] * f;
+    o += y * f;
+  }
 #pragma unroll
-    for (uint32_t u = 0; u < (R + 1) / 2; u++)
-      if (lane + 64 * u < D) o[u] += p[2 + lane + 64 * u] * f;
+  for (uint32_t mk = L; mk < 64; mk <<= 1) {
+    l += __shfl_xor(l, mk, 64);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], mk, 64);
   }
   float f;
-  const float den = finish_sum<T>(M, l, a.sink, hd, &f);
+  const float den = finish_sum(M, l, a.sink, hd, &f);
+  const float inv = nz && den != 0.0f ? f / den : 0.0f;
+  T* out = (T*)a.o.p + (uint64_t)row * a.o.row + (uint64_t)hd * a.o.head + d;
+  if (g == 0) {
 #pragma unroll
-  for (uint32_t u = 0; u < (R + 1) / 2; u++)
-    if (lane + 64 * u < D)
-      ((T*)a.o.p)[(uint64_t)row * a.o.row + (uint64_t)hd * a.o.head + lane + 64 * u] =
-          (T)(nz && den != 0.0f ? o[u] * f / den : 0.0f);
+    for (int e = 0; e < 4; e++) out[e] = (T)(nz ? o[e] * inv : 0.0f);
+  }
 }
 
 template <typename T>
@@ -994,8 +1204,13 @@ hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {
     constexpr int D = decltype(d)::value;
     const uint32_t vec = on16<T>(a.q) && on16<T>(a.o);
     const uint32_t G = a.hq / a.c.heads;
-    const uint32_t nt16 = a.r.off ? 1 : (G + 15) / 16;
-    hipLaunchKernelGGL((k_kv4_few<T, D>), dim3(a.r.n * a.c.heads * nt16, a.nsplit), dim3(256), 0, st, a, vec, nt16);
+    // a pair's columns: one a part, where single rows leave the room
+    constexpr int NC = sizeof(T) == 4 ? 4 : 2;
+    const bool wide = !a.r.off && G * NC <= 16;
+    const uint32_t ncol = a.r.off ? 1 : (G + 15) / 16;
+    const dim3 grid(a.r.n * a.c.heads * ncol, a.nsplit);
+    if (wide) hipLaunchKernelGGL((k_kv4_few<T, D, NC>), grid, dim3(256), 0, st, a, vec, 1u);
+    else hipLaunchKernelGGL((k_kv4_few<T, D, 1>), grid, dim3(256), 0, st, a, vec, ncol);
     if (a.r.off) {
       constexpr uint32_t PW = Many<T, D>::pairs;
       const uint32_t gx = (uint32_t)(((uint64_t)a.r.rows * G + PW - 1) / PW) + a.r.n;

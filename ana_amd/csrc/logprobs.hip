@@ -30,7 +30,7 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr uint32_t kHead = 8;   // a piece's words before its keys: m, c, l, w, rank, bad
+constexpr uint32_t kHead = 8;   // a piece's words before its keys: m, c, l, w, rank
 
 // a logit's order as a whole number: larger for larger ones, -0 as +0, 0 for NaN
 __device__ __forceinline__ uint32_t order_of(float x) {
@@ -53,27 +53,23 @@ __device__ __forceinline__ u64 wave_max64(u64 v) {
   return v;
 }
 
-template <typename T, int W>
-__device__ __forceinline__ void load_vec(const T* p, float* x) {
-  typedef T vecw __attribute__((ext_vector_type(W)));
-  const vecw v = *reinterpret_cast<const vecw*>(p);
-#pragma unroll
-  for (int e = 0; e < W; e++) x[e] = (float)v[e];
-}
+// the larger of two, NaN if either is
+__device__ __forceinline__ float max_or_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// a row's results from its sums (bad: a NaN or +inf among the logits)
+// a row's results from its sums: entries at the maximum m are c, the others'
+// sums l and w
 struct RowSums {
   float m, c, l, w;
-  bool bad;
-  // log of the sum over e^m, and of a logit
+  // a NaN among the logits makes l one
+  __device__ __forceinline__ bool bad() const { return m == INFINITY || l != l; }
   __device__ __forceinline__ float log_sum() const { return log1pf((c - 1.0f) + l); }
   __device__ __forceinline__ float lp(float x, float ls) const {
-    if (bad || x != x) return __builtin_nanf("");
+    if (bad() || x != x) return __builtin_nanf("");
     if (x == -INFINITY) return x;
     return (x - m) - ls;
   }
   __device__ __forceinline__ float entropy(float ls) const {
-    if (bad) return __builtin_nanf("");
+    if (bad()) return __builtin_nanf("");
     return m == -INFINITY ? 0.0f : ls - w / (c + l);
   }
 };
@@ -81,14 +77,18 @@ struct RowSums {
 // Piece z of row r, elements z C .. (C a multiple of 16 bytes of elements, at
 // most NT V W). The row may start anywhere: whole 16-byte vectors from its
 // first border on, the elements before and after them one each for the first
-// threads. Alone (one piece) it writes the row's results, else its sums and
-// keys.
+// threads. Places that no logit fills hold -inf, which changes no sum and
+// nothing that is compared with a finite bound; the paths without one look at
+// the places. Alone (one piece) it writes the row's results, else its sums
+// and keys.
 template <typename T, int NT, int V>
-__global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint32_t S) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_logprobs(LogprobArgs a, uint32_t C, uint32_t S) {
   constexpr int W = 16 / sizeof(T), NW = NT / 64, CAP = 512;
+  typedef T vec_t __attribute__((ext_vector_type(W)));
   __shared__ float tmax[NW][64];
+  __shared__ __align__(16) float gmax[64];
   __shared__ float red[NW][3];
-  __shared__ uint32_t redu[NW][2];
+  __shared__ uint32_t redu[NW];
   __shared__ float bound_s;
   __shared__ uint32_t ncand;
   __shared__ u64 cand[CAP], best[kLpMaxTop], wred[NW];
@@ -100,15 +100,15 @@ __global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint
   const uint32_t head = min((uint32_t)((16 - (uintptr_t)p % 16) % 16 / sizeof(T)), cnt);
   const uint32_t nvec = (cnt - head) / W, tail0 = head + nvec * W;
   const uint32_t k = a.top;
-  float x[V][W];
+  vec_t x[V];
 #pragma unroll
   for (int u = 0; u < V; u++) {
     const uint32_t v = u * NT + tid;
     if (v < nvec) {
-      load_vec<T, W>(p + head + v * W, x[u]);
+      x[u] = *reinterpret_cast<const vec_t*>(p + head + v * W);
     } else {
 #pragma unroll
-      for (int e = 0; e < W; e++) x[u][e] = -INFINITY;
+      for (int e = 0; e < W; e++) x[u][e] = (T)-INFINITY;
     }
   }
   // this thread's element before or after the vectors
@@ -120,14 +120,19 @@ __global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint
   const float xt = given ? (float)row[tk] : 0.0f;
   if (tid == 0) ncand = 0;
 
-  float m = xe == xe ? xe : -INFINITY;
-  bool bad = !(xe < INFINITY);
+  // f(value, index) over the thread's share of the piece, read again: the
+  // rare paths, which would take the common ones' registers
+  auto each = [&](auto&& f) {
+#pragma unroll 1
+    for (uint32_t i = tid; i < cnt; i += NT) f((float)p[i], e0 + i);
+  };
+
+  float m = fmaxf(xe, -INFINITY);
 #pragma unroll
   for (int u = 0; u < V; u++)
+    if (u * NT < nvec) {
 #pragma unroll
-    for (int e = 0; e < W; e++) {
-      bad |= !(x[u][e] < INFINITY);
-      m = fmaxf(m, x[u][e]);
+      for (int e = 0; e < W; e++) m = fmaxf(m, (float)x[u][e]);
     }
   const float tm = m;
   tmax[wv][lane] = tm;
@@ -137,95 +142,106 @@ __global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint
 #pragma unroll
   for (int i = 1; i < NW; i++) gm = fmaxf(gm, tmax[i][lane]);
   m = wmax(gm);
-  if (wv == 0 && k) {
-    // the group maximum that k of them reach
+  if (wv == NW - 1 && k) {
+    // the k-th largest group maximum: the least that fewer than k are above
+    gmax[lane] = gm;
+    __builtin_amdgcn_wave_barrier();
     uint32_t above = 0;
-    for (int i = 0; i < 64; i++) {
-      const float o = lane_f(gm, i);
-      above += o > gm || (o == gm && i < (int)lane);
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+      const f32x4_t o = reinterpret_cast<const f32x4_t*>(gmax)[i];
+      above += (o[0] > gm) + (o[1] > gm) + (o[2] > gm) + (o[3] > gm);
     }
-    if (above == k - 1) bound_s = gm;
+    const float b = -wmax(above < k ? -gm : -INFINITY);
+    if (lane == 0) bound_s = b;
   }
   // (+inf: the row's results are NaN whatever the sums)
   const float ms = m == -INFINITY || m == INFINITY ? 0.0f : m;
-  float l = 0.0f, w = 0.0f, c = 0.0f;
-  uint32_t above = 0;
   constexpr float log2e = 1.4426950408889634f;
-  // an entry's terms; far below the maximum (and for -inf) both are 0
-  auto term = [&](float v, bool skip_top) {
-    const float d = fmaxf(v - ms, -200.0f);
-    const float t = __builtin_amdgcn_exp2f(d * log2e);
-    l += skip_top && v == m ? 0.0f : t;
-    w = fmaf(t, d, w);
-  };
-  if (__any(tm == m)) {
-    term(xe, true);
-    c += xe == m && has_edge ? 1.0f : 0.0f;
-#pragma unroll
-    for (int u = 0; u < V; u++) {
-      const bool in = (uint32_t)u * NT + tid < nvec;
-#pragma unroll
-      for (int e = 0; e < W; e++) {
-        term(x[u][e], true);
-        c += x[u][e] == m && in ? 1.0f : 0.0f;
+  float l = 0.0f, w = 0.0f, c = 0.0f;
+  auto sums = [&](auto top) {
+    // (far below the maximum, and at -inf, both terms are 0)
+    auto term = [&](float v) {
+      const float d = max_or_nan(v - ms, -200.0f);
+      float t = __builtin_amdgcn_exp2f(d * log2e);
+      if constexpr (decltype(top)::value) {
+        t = v == m ? 0.0f : t;
+        c += v == m ? 1.0f : 0.0f;
       }
-    }
-  } else {
-    term(xe, false);
+      l += t;
+      w = fmaf(t, d, w);
+    };
+    term(xe);
 #pragma unroll
     for (int u = 0; u < V; u++)
+      if (u * NT < nvec) {
 #pragma unroll
-      for (int e = 0; e < W; e++) term(x[u][e], false);
-  }
-  if (given) {
-    const uint32_t ot = order_of(xt);
-    auto over = [&](float v, uint32_t i, bool in) {
-      // (a NaN is above nothing; every number is above a NaN)
-      const bool gt = v > xt || (ot == 0 && v == v);
-      const bool eq = v == xt || (ot == 0 && v != v);
-      above += in && (gt || (eq && i < tk)) ? 1u : 0u;
-    };
-    over(xe, e0 + edge, has_edge);
+        for (int e = 0; e < W; e++) term((float)x[u][e]);
+      }
+  };
+  if (__any(tm == m)) sums(std::true_type{});
+  else sums(std::false_type{});
+  uint32_t above = 0;
+  if (given && xt > -INFINITY) {
+    // above x_t, or before the token and not below it: above the next float down
+    const uint32_t ut = __builtin_bit_cast(uint32_t, xt);
+    const float xp = xt == 0.0f ? -1.401298464e-45f : __builtin_bit_cast(float, xt > 0.0f ? ut - 1 : ut + 1);
+    above += has_edge && xe > (e0 + edge < tk ? xp : xt);
 #pragma unroll
-    for (int u = 0; u < V; u++) {
-      const uint32_t v = u * NT + tid;
+    for (int u = 0; u < V; u++)
+      if (u * NT < nvec) {
+        const uint32_t i = e0 + head + (u * NT + tid) * W;
+        const float t = i + W <= tk ? xp : xt;
 #pragma unroll
-      for (int e = 0; e < W; e++) over(x[u][e], e0 + head + v * W + e, v < nvec);
-    }
+        for (int e = 0; e < W; e++) above += (float)x[u][e] > t;
+        if (__any(i <= tk && tk < i + W)) {
+#pragma unroll
+          for (int e = 0; e < W; e++) above += i + W > tk && i + e < tk && (float)x[u][e] == xt;
+        }
+      }
+  } else if (given) {
+    const u64 kt = key_of(xt, tk);
+    each([&](float v, uint32_t i) { above += key_of(v, i) > kt; });
   }
   float s3[3] = {l, w, c};
   wsum_n(s3);
-  uint32_t ab = above;
 #pragma unroll
-  for (int mk = 32; mk >= 1; mk >>= 1) ab += __shfl_xor(ab, mk, 64);
-  const uint32_t anybad = __any(bad);
+  for (int mk = 32; mk >= 1; mk >>= 1) above += __shfl_xor(above, mk, 64);
   if (lane == 0) {
     red[wv][0] = s3[0];
     red[wv][1] = s3[1];
     red[wv][2] = s3[2];
-    redu[wv][0] = ab;
-    redu[wv][1] = anybad;
+    redu[wv] = above;
   }
   __syncthreads();
   if (k) {
     const float bound = bound_s;
-    auto offer = [&](float v, uint32_t i, bool in) {
-      if (in && v >= bound) {
-        const uint32_t at = atomicAdd(&ncand, 1u);
-        if (at < CAP) cand[at] = key_of(v, i);
-      }
-    };
-    if (__any(tm >= bound)) {
-      offer(xe, e0 + edge, has_edge);
+    const uint32_t want = min(k, cnt);
+    uint32_t nc = 0;
+    if (bound > -INFINITY) {
+      if (__any(tm >= bound)) {
+        auto offer = [&](float v, uint32_t i) {
+          if (v >= bound) {
+            const uint32_t at = atomicAdd(&ncand, 1u);
+            if (at < CAP) cand[at] = key_of(v, i);
+          }
+        };
+        offer(xe, e0 + edge);
 #pragma unroll
-      for (int u = 0; u < V; u++) {
-        const uint32_t v = u * NT + tid;
+        for (int u = 0; u < V; u++)
+          if (u * NT < nvec) {
+            float t = (float)x[u][0];
 #pragma unroll
-        for (int e = 0; e < W; e++) offer(x[u][e], e0 + head + v * W + e, v < nvec);
+            for (int e = 1; e < W; e++) t = fmaxf(t, (float)x[u][e]);
+            if (__any(t >= bound)) {
+#pragma unroll
+              for (int e = 0; e < W; e++) offer((float)x[u][e], e0 + head + (u * NT + tid) * W + e);
+            }
+          }
       }
+      __syncthreads();
+      nc = ncand;
     }
-    __syncthreads();
-    const uint32_t nc = ncand, want = min(k, cnt);
     if (tid < k && tid >= want) best[tid] = 0;
     if (nc <= CAP && nc >= want) {
       for (uint32_t i = tid; i < nc; i += NT) {
@@ -238,17 +254,10 @@ __global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint
       u64 last = ~0ull;
       for (uint32_t i = 0; i < want; i++) {
         u64 t = 0;
-        auto see = [&](float v, uint32_t at, bool in) {
+        each([&](float v, uint32_t at) {
           const u64 q = key_of(v, at);
-          if (in && q < last && q > t) t = q;
-        };
-        see(xe, e0 + edge, has_edge);
-#pragma unroll
-        for (int u = 0; u < V; u++) {
-          const uint32_t v = u * NT + tid;
-#pragma unroll
-          for (int e = 0; e < W; e++) see(x[u][e], e0 + head + v * W + e, v < nvec);
-        }
+          if (q < last && q > t) t = q;
+        });
         t = wave_max64(t);
         __syncthreads();
         if (lane == 0) wred[wv] = t;
@@ -263,15 +272,14 @@ __global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint
     __syncthreads();
   }
   // the piece's sums, in the waves' order
-  RowSums rs{m, 0.0f, 0.0f, 0.0f, false};
+  RowSums rs{m, 0.0f, 0.0f, 0.0f};
   uint32_t rk = 0;
 #pragma unroll
   for (int i = 0; i < NW; i++) {
     rs.l += red[i][0];
     rs.w += red[i][1];
     rs.c += red[i][2];
-    rk += redu[i][0];
-    rs.bad |= redu[i][1] != 0;
+    rk += redu[i];
   }
   if (S > 1) {
     uint32_t* out = a.part + (uint64_t)blockIdx.x * (kHead + 2 * k);
@@ -281,7 +289,6 @@ __global__ __launch_bounds__(NT) void k_logprobs(LogprobArgs a, uint32_t C, uint
       out[2] = __builtin_bit_cast(uint32_t, rs.l);
       out[3] = __builtin_bit_cast(uint32_t, rs.w);
       out[4] = rk;
-      out[5] = rs.bad;
     }
     if (tid < k) {
       out[kHead + 2 * tid] = (uint32_t)best[tid];
@@ -310,7 +317,7 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
   const uint32_t r = blockIdx.x, lane = threadIdx.x, k = a.top;
   const uint32_t* p = a.part + ((uint64_t)r * S + lane) * (kHead + 2 * k);
   const bool in = lane < S;
-  RowSums q{-INFINITY, 0.0f, 0.0f, 0.0f, false};
+  RowSums q{-INFINITY, 0.0f, 0.0f, 0.0f};
   uint32_t rk = 0;
   if (in) {
     q.m = __builtin_bit_cast(float, p[0]);
@@ -318,17 +325,16 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
     q.l = __builtin_bit_cast(float, p[2]);
     q.w = __builtin_bit_cast(float, p[3]);
     rk = p[4];
-    q.bad = p[5] != 0;
   }
   const uint32_t tk = a.tok ? a.tok[r] : 0xFFFFFFFFu;
   const bool given = tk < a.vocab;
   const float xt = given ? (float)((const T*)a.logits + (uint64_t)r * a.ld)[tk] : 0.0f;
-  RowSums t{wmax(q.m), 0.0f, 0.0f, 0.0f, (bool)__any(q.bad)};
+  RowSums t{wmax(q.m), 0.0f, 0.0f, 0.0f};
   // e^(x - M) = f e^(x - m), (x - M) = (x - m) + d; a piece below the
   // maximum has no entry at it
   const float d = fmaxf(q.m - t.m, -200.0f);
   const bool at = q.m == t.m, none = q.m == -INFINITY;
-  const float f = none ? 0.0f : __expf(d);
+  const float f = none ? 0.0f : __expf(d);   // (a NaN in l stays one)
   float s[3];
   s[0] = at ? q.c : 0.0f;
   s[1] = at ? q.l : f * (q.c + q.l);
@@ -363,18 +369,21 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
   }
 }
 
-// The pieces of a row: whole rows of up to 32768 logits where the rows alone
-// fill the chip, else pieces of 8192, or of 2048 where those are few.
+// How a row is cut: whole rows of up to 32768 logits (one launch; 512 rows
+// of 32768 f32 logits take 20 us whole and 30 in pieces of 8192 with the
+// join, one row 8 and 10), longer ones in pieces of 8192, of which a CU holds
+// eight (3000 rows of 50021 bf16 logits: 110 us, and 126 in two pieces of
+// 1024 threads), or of 32768 where those would be too many for one wave to
+// join.
 struct Plan {
   uint32_t C, S;
-  bool wide;
+  bool wide;   // 1024 threads and up to 32768 logits a workgroup, else 256 and 8192
 };
-Plan plan_of(uint32_t n, uint32_t vocab) {
+Plan plan_of(uint32_t vocab) {
   Plan p;
-  p.wide = n >= 256 || vocab > 64 * 8192;
-  const uint32_t cap = p.wide ? 32768u : (uint64_t)n * vocab >= 256ull * 8192 ? 8192u : 2048u;
+  p.wide = (vocab > 8192 && vocab <= 32768) || vocab > 64 * 8192;
+  const uint32_t cap = p.wide ? 32768u : 8192u;
   p.S = (vocab + cap - 1) / cap;
-  if (p.S > 64) p.S = 64;
   p.C = ((vocab + p.S - 1) / p.S + 7) & ~7u;
   p.S = (vocab + p.C - 1) / p.C;
   return p;
@@ -383,7 +392,7 @@ Plan plan_of(uint32_t n, uint32_t vocab) {
 }  // namespace
 
 uint64_t logprobs_part_words(uint32_t n, uint32_t vocab, uint32_t top) {
-  const Plan p = plan_of(n, vocab);
+  const Plan p = plan_of(vocab);
   return p.S > 1 ? (uint64_t)n * p.S * (kHead + 2 * top) : 0;
 }
 
@@ -391,7 +400,7 @@ hipError_t launch_logprobs(const LogprobArgs& a, int type, hipStream_t st) {
   if (!a.logits || a.vocab == 0 || a.vocab > kLpMaxVocab || a.top > kLpMaxTop || a.top > a.vocab || a.ld < a.vocab || !a.ent)
     return hipErrorInvalidValue;
   if (a.n == 0) return hipSuccess;
-  const Plan p = plan_of(a.n, a.vocab);
+  const Plan p = plan_of(a.vocab);
   if ((p.S > 1 && !a.part) || (uint64_t)a.n * p.S > 0x7FFFFFFFull) return hipErrorInvalidValue;
   auto go = [&](auto t) -> hipError_t {
     using T = decltype(t);

@@ -357,7 +357,8 @@ int ana_kv4_read(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_ma
  * e^sink[a]), sink (hq floats) NULL for none; 0 where it sees nothing.
  * What a row does not see, NaN included, does not change it. In f32 the
  * products are exact up to their f32 sums; 16-bit outputs take
- * probabilities to 2^-17. `live`, where not 0, is the most positions a
+ * probabilities to 2^-16, bf16 ones of a sequence with more than 16 query
+ * rows a key head rounded to bf16. `live`, where not 0, is the most positions a
  * sequence holds after the call, as far as the caller knows: it only
  * chooses how the work is split. ws: ana_kv4_attend_ws bytes of workspace
  * for the same arguments, on a 16-byte border. */

@@ -109,20 +109,22 @@ def attend(q, data, slots, pos, seq, off, sink, scale):
     return o, pv, big, cnt
 
 
-def attend_tolerance(typ, o, pv, big, cnt, hd):
+def attend_tolerance(typ, o, pv, big, cnt, hd, rounded=False):
     """What rounding allows. A score is a sum of at most 3 hd exact products in
     f32, then two multiplications: off by (3 hd + 2) 2^-24 of the sum of its
     terms' sizes. An exponential's relative error is that of its argument
     (in base e) and of exp2 (2 steps) and the subtraction of the maximum
     (2^-24 of a number that the scores' sizes bound). Sums of cnt
     probabilities and of cnt products lose at most cnt 2^-24 each, the pieces'
-    joins a few more. A 16-bit output's probabilities are taken to 2^-17. All
+    joins a few more. A 16-bit output's probabilities are taken to 2^-16 (cut
+    to 16 bits), or (rounded: bf16, more than 16 query rows of a key head)
+    each rounded once to bf16, by at most half a step, 2^-8. All
     count against sum p |v|, at most twice (in the sum and in the
     denominator); then the output's own rounding."""
     e = EPS["f32"]
     rel = 2 * ((3 * hd + 2) * e * big + 2 * e * big + 4 * e) + (2 * cnt + 32) * e
     if typ != "f32":
-        rel = rel + 2.0 ** -17
+        rel = rel + 2 * (2.0 ** -8 if rounded else 2.0 ** -16)
     return rel * pv + EPS[typ] * np.abs(o) + (2.0 ** -25 if typ == "f16" else 1e-37)
 
 

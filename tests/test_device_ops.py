@@ -90,7 +90,7 @@ def test_refuses_heads_and_workspaces():
     assert rc == ana_amd.ANA_EINVAL and "2^31" in msg
     long = cache(slots=1 << 20)
     need = ana_amd.lib().ana_kv4_attend_ws(C.byref(long), C.byref(rows()), 4, 0)
-    assert need > 0 and need % (4 * 66 * 2 * 4) == 0
+    assert need > 0 and need % (2 * 4 * 16) == 0
     for ws, n in ((None, need), (A, need - 1), (A + 4, need)):
         rc, msg = attend(long, rows(), mat(row=256), mat(row=256), ws=ws, nws=n)
         assert rc == ana_amd.ANA_EINVAL and "workspace" in msg
@@ -124,8 +124,8 @@ def logprobs(**kw):
     (dict(top=65), "alternatives"), (dict(vocab=5, top=6), "alternatives"), (dict(ld=99), "overlap"),
     (dict(logits=None), "null"), (dict(ent=None), "null"), (dict(lp=None), "null"), (dict(rank=None), "null"),
     (dict(top_tok=None), "null"), (dict(top_lp=None), "null"), (dict(logits=A + 2), "border"),
-    (dict(n=1 << 26), "2^25"), (dict(vocab=32768, ld=32768, ws=None), "workspace"),
-    (dict(vocab=32768, ld=32768, nws=8), "workspace")])
+    (dict(n=1 << 26), "2^25"), (dict(vocab=40000, ld=40000, ws=None), "workspace"),
+    (dict(vocab=40000, ld=40000, nws=8), "workspace")])
 def test_refuses_logprobs(kw, why):
     rc, msg = logprobs(**kw)
     assert rc == ana_amd.ANA_EINVAL and why in msg
