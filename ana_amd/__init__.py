@@ -23,6 +23,7 @@ ANA_OK, ANA_EINVAL, ANA_ECKPT, ANA_EDEVICE, ANA_ENOMEM, ANA_EUNSUP, ANA_ETOK, AN
 EXACT_FP32 = 0
 FAST_FP32 = 1
 BF16 = 2
+KV4 = 0x100  # with FAST_FP32 or BF16: the softmax rings in 4 bits
 EOS = 1  # bend/Tokenizer.bend: BOS 0, EOS 1
 
 
@@ -74,6 +75,9 @@ SIGNATURES = {
     "ana_logits": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, _f32p]),
     "ana_top": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, _u32p]),
     "ana_stats": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, _u32p, _f32p, _u32p, _f32p]),
+    "ana_logprobs": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, _u32p, C.c_uint32, _f32p, _f32p, _u32p, _u32p, _f32p]),
+    "ana_score_logprobs_n": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, _u32p, _u32p, _u32p, C.c_uint32, _f32p, _f32p,
+                                       _u32p, _u32p, _f32p]),
     "ana_pick": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, C.POINTER(_Sampling), _u64p, _u32p]),
     "ana_rng_seeded": (None, [C.c_uint64, _u64p]),
     "ana_generate": (C.c_int, [C.c_void_p, C.c_uint32, _u32p, _u32p, _u32p, C.c_uint32,
@@ -188,6 +192,35 @@ def rng_of(sample_seed: str) -> np.ndarray:
     """dc.rng.of: SAMPLE_SEED parsed as U64, else seed 0."""
     v = u64_read(sample_seed)
     return rng_seeded(0 if v is None else v)
+
+
+@dataclass
+class Logprobs:
+    """Rows of log probabilities: the given tokens' (logprob, rank: the tokens
+    before it; None where none were given), the entropies in nats, and the
+    likeliest tokens [rows, top] with theirs."""
+
+    logprob: np.ndarray | None
+    entropy: np.ndarray
+    rank: np.ndarray | None
+    top: np.ndarray
+    top_logprob: np.ndarray
+
+    @classmethod
+    def empty(cls, n: int, top: int, given: bool) -> "Logprobs":
+        f, u = np.float32, np.uint32
+        return cls(np.empty(n, f) if given else None, np.empty(n, f), np.empty(n, u) if given else None,
+                   np.empty((n, top), u), np.empty((n, top), f))
+
+    def _out(self):
+        """ana_logprobs' output arguments."""
+        def p(a, t):
+            return None if a is None else _p(a, t)
+        return (p(self.logprob, C.c_float), p(self.entropy, C.c_float), p(self.rank, C.c_uint32),
+                p(self.top, C.c_uint32), p(self.top_logprob, C.c_float))
+
+    def _rows(self, a: int, b: int) -> "Logprobs":
+        return Logprobs(self.logprob[a:b], self.entropy[a:b], self.rank[a:b], self.top[a:b], self.top_logprob[a:b])
 
 
 class Decoder:
@@ -321,6 +354,35 @@ class Decoder:
         self._check(lib().ana_stats(self.h, s.size, _p(s, C.c_uint32), _p(t, C.c_uint32), _p(p, C.c_float),
                                     _p(a, C.c_uint32), _p(pa, C.c_float)))
         return p, a, pa
+
+    def logprobs(self, seqs, toks=None, top: int = 0) -> "Logprobs":
+        """After each sequence's last fed token: the log probability and rank
+        of toks[i] (None for neither), the entropy, and the `top` likeliest
+        tokens. ana_logprobs."""
+        s = _u32(seqs)
+        t = None if toks is None else _u32(toks)
+        if t is not None and t.size != s.size:
+            raise ValueError("logprobs: one token per sequence")
+        r = Logprobs.empty(s.size, top, t is not None)
+        self._check(lib().ana_logprobs(self.h, s.size, _p(s, C.c_uint32), None if t is None else _p(t, C.c_uint32),
+                                       top, *r._out()))
+        return r
+
+    def score_logprobs_n(self, seqs, pos, toks, top: int = 0) -> list:
+        """score_n's windows: one Logprobs a sequence, row t of it token
+        t + 1's after token t. ana_score_logprobs_n."""
+        s, p = _u32(seqs), _u32(pos)
+        ts = [_u32(t) for t in toks]
+        if not (p.size == s.size == len(ts)):
+            raise ValueError(f"score_logprobs_n: {s.size} sequences, {p.size} positions, {len(ts)} windows")
+        ln = np.array([t.size for t in ts], dtype=np.uint32)
+        flat = np.ascontiguousarray(np.concatenate(ts + [np.zeros(1, np.uint32)]), dtype=np.uint32)
+        rows = [max(int(k) - 1, 0) for k in ln]
+        r = Logprobs.empty(sum(rows), top, True)
+        self._check(lib().ana_score_logprobs_n(self.h, s.size, _p(s, C.c_uint32), _p(p, C.c_uint32),
+                                               _p(ln, C.c_uint32), _p(flat, C.c_uint32), top, *r._out()))
+        ends = np.cumsum([0] + rows)
+        return [r._rows(int(a), int(b)) for a, b in zip(ends, ends[1:])]
 
     def pick(self, seqs, st: Settings, rng: np.ndarray | None = None) -> np.ndarray:
         """S.pick on the device; rng (n x 4 uint64) advances in place."""

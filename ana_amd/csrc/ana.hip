@@ -18,6 +18,8 @@
 #include <vector>
 
 #include "ana_internal.h"
+#include "kv4.h"
+#include "logprobs.h"
 
 using namespace ana;
 
@@ -32,6 +34,10 @@ struct ana_ctx {
   uint32_t max_seqs = 1, chunk = 64, wb = 1;
   uint32_t rows = 1;                 // capacity of the row workspaces (a prefill batch)
   int mode = ANA_EXACT_FP32;         // numerics
+  bool kv4 = false;                  // the softmax rings in 4 bits (ANA_KV4)
+  float* d_kpart = nullptr;          // their attention's partials
+  uint32_t* d_kseg = nullptr;        // a prefill step's chunks for it: places, positions, row offsets
+  std::vector<uint32_t> h_kseg;
   float* W = nullptr;                // parameters [P]
   uint16_t* Wh = nullptr;            // ANA_BF16: the parameters as bfloat16 [P]
   uint16_t* Wp = nullptr;            // ANA_BF16: the persistent kernel's bf16 matrices that start off 16 bytes in Wh, on 16 bytes
@@ -59,6 +65,11 @@ struct ana_ctx {
   uint32_t* d_tgt = nullptr;         // scoring: each row's target token
   float* d_stat = nullptr;           // ana_stats: each row's p and rival p, then the rivals
   float* d_ce = nullptr;             // scoring: each row's G.lse - logit[target]
+  // ana_logprobs, ana_score_logprobs_n: each row's results (lp_rows rows),
+  // and the pieces' workspace
+  uint32_t* d_lp = nullptr;
+  uint32_t* d_lpw = nullptr;
+  uint32_t lp_rows = 1;
   __bf16* d_sah = nullptr;   // ANA_BF16 prefill: a product's activations in bf16
   __bf16* d_hh = nullptr;    // ANA_BF16 prefill: gate|up's outputs in bf16, down's input
   bool hh_bf = false;        // d_hh holds the last gate|up's outputs
@@ -280,7 +291,7 @@ static void release(ana_ctx* c) {
   void* ps[] = {c->d_play, c->feed_save, c->d_ctl, c->d_trace, c->W, c->Wh, c->Wp, c->d_part, c->d_gla, c->state, c->xs, c->X, c->XA, c->XN, c->QKV, c->Z, c->O, c->HH, c->LG,
                 c->d_seq, c->d_pos, c->d_tok, c->d_pick, c->d_out, c->d_step, c->d_rng, c->d_amax,
                 c->d_ss, c->d_pm, c->d_gtab, c->d_grun, c->d_atab, c->d_rseq, c->d_rpos, c->SC, c->d_tgt, c->d_ce, c->d_stat, c->d_rcp,
-                c->d_sah, c->d_hh, c->d_rsc, c->PK, c->W3, c->d_a3, c->d_h3, c->d_hpc, c->d_hpctl, c->d_oh, c->d_nxh, c->d_ssp};
+                c->d_sah, c->d_hh, c->d_rsc, c->PK, c->W3, c->d_a3, c->d_h3, c->d_hpc, c->d_hpctl, c->d_oh, c->d_nxh, c->d_ssp, c->d_kpart, c->d_kseg, c->d_lp, c->d_lpw};
   for (void* p : ps)
     if (p) (void)hipFree(p);
   for (hipEvent_t e : c->ev) (void)hipEventDestroy(e);
@@ -289,6 +300,12 @@ static void release(ana_ctx* c) {
 
 static StateRef sref(const ana_ctx* c, uint32_t l) {
   return StateRef{c->state, c->seq_stride, c->layer_off[l]};
+}
+// a softmax layer's rings in 4 bits
+static Kv4 kv4_of(const ana_ctx* c, uint32_t l) {
+  const ana_config& cf = c->cfg;
+  return Kv4{reinterpret_cast<uint8_t*>(c->state + c->layer_off[l]), 4 * c->seq_stride, c->max_seqs, cf.ctx,
+             (cf.ctx + 31) / 32, cf.heads, cf.d / cf.heads};
 }
 
 // what the kernels require of a configuration
@@ -325,17 +342,24 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
   ana_opts o{};
   o.max_seqs = 1;
   if (opts) o = *opts;
+  const bool kv4 = o.numerics >= 0 && (o.numerics & ANA_KV4);
+  if (kv4) o.numerics &= ~ANA_KV4;
   if (o.numerics != ANA_EXACT_FP32 && o.numerics != ANA_FAST_FP32 && o.numerics != ANA_BF16)
     return fail(nullptr, ANA_EUNSUP, "ana_open: unknown numerics mode %d", o.numerics);
+  if (kv4 && o.numerics == ANA_EXACT_FP32)
+    return fail(nullptr, ANA_EUNSUP, "ana_open: the exact mode keeps its rings in fp32 (ANA_KV4 goes with the fast modes)");
   if (o.max_seqs == 0) o.max_seqs = 1;
   if (o.prefill_chunk == 0) o.prefill_chunk = 64;
   Ftc2 ck;
   std::string why = read_ftc2(path, &ck);
   if (!why.empty()) return fail(nullptr, ANA_ECKPT, "%s", why.c_str());
   if (const char* u = unsupported(ck.cfg)) return fail(nullptr, ANA_EUNSUP, "ana_open: %s", u);
+  if (kv4 && !kv4_fits(ck.cfg.d / ck.cfg.heads))
+    return fail(nullptr, ANA_EUNSUP, "ana_open: rings in 4 bits take head dimensions of 32 and 64");
   ana_ctx* c = new ana_ctx();
   c->device = o.device;
   c->mode = o.numerics;
+  c->kv4 = kv4;
   c->cfg = ck.cfg;
   c->step = ck.step;
   c->P = params_of(ck.cfg);
@@ -368,7 +392,8 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
   uint64_t off = 0;
   for (uint32_t l = 0; l < cf.layers; l++) {
     c->layer_off.push_back(off);
-    off += c->blk[l].gla ? (uint64_t)cf.heads * hd * hd : 2ull * cf.ctx * d;
+    off += c->blk[l].gla ? (uint64_t)cf.heads * hd * hd
+                         : kv4 ? kv4_seq_bytes(cf.ctx, cf.heads, hd) / 4 : 2ull * cf.ctx * d;
   }
   c->seq_stride = off;
   auto bad = [&](hipError_t e) {
@@ -409,6 +434,10 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
       (e = dalloc(&c->d_tgt, c->rows)) != hipSuccess || (e = dalloc(&c->d_ce, c->rows)) != hipSuccess ||
       (e = dalloc(&c->d_stat, 3 * (uint64_t)c->max_seqs)) != hipSuccess)
     return bad(e);
+  c->lp_rows = std::max(c->max_seqs, c->rows);
+  if ((e = dalloc(&c->d_lp, (uint64_t)c->lp_rows * (3 + 2 * kLpMaxTop))) != hipSuccess ||
+      (e = dalloc(&c->d_lpw, logprobs_part_words(std::max(c->max_seqs, c->sc_rows), cf.vocab, kLpMaxTop))) != hipSuccess)
+    return bad(e);
   // a prefill step's residual-row pairs, chunks, and rows' sequences and
   // positions (every mode)
   if ((e = dalloc(&c->d_rcp, 2 * (uint64_t)c->rows)) != hipSuccess ||
@@ -424,6 +453,21 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
         (e = dalloc(&c->d_gtab, c->gsub_cap)) != hipSuccess || (e = dalloc(&c->d_atab, c->atab_cap)) != hipSuccess)
       return bad(e);
     c->gla = gla_scan_carve(c->d_gla, c->rows, c->gsub_cap, c->seg_cap, d, cf.heads);
+  }
+  if (kv4) {
+    // the partials of the largest call, of single rows or of a prefill step's
+    uint64_t most = 0;
+    const Kv4 kc = kv4_of(c, 0);
+    for (uint32_t r = 1; r <= c->rows; r++) {
+      uint32_t ns, tps;
+      kv4_split(kc, r, r, true, cf.heads, 0, &ns, &tps);
+      most = std::max(most, kv4_part_floats(r, cf.heads, hd, ns));
+      if (r > c->wb) continue;
+      kv4_split(kc, r, r, false, cf.heads, 0, &ns, &tps);
+      most = std::max(most, kv4_part_floats(r, cf.heads, hd, ns));
+    }
+    if ((e = dalloc(&c->d_kpart, most)) != hipSuccess || (e = dalloc(&c->d_kseg, 3 * (uint64_t)c->seg_cap + 1)) != hipSuccess)
+      return bad(e);
   }
   if (c->mode == ANA_BF16) {
     const uint64_t kmax = std::max(d, cf.f);
@@ -700,7 +744,7 @@ static hipError_t persist_setup(ana_ctx* c) {
   if ((e = hipDeviceGetAttribute(&coop, hipDeviceAttributeCooperativeLaunch, c->device)) != hipSuccess) return e;
   const uint32_t G = (uint32_t)std::min(pr.multiProcessorCount, 256);
   const bool exact = c->mode == ANA_EXACT_FP32;
-  if (!coop || !decode1_fits(cf, G, exact)) return hipSuccess;
+  if (!coop || c->kv4 || !decode1_fits(cf, G, exact)) return hipSuccess;   // (its attention reads fp32 rings)
   int rate_khz = 0;   // the constant-rate clock the kernel's waits are timed by
   if ((e = hipDeviceGetAttribute(&rate_khz, hipDeviceAttributeWallClockRate, c->device)) != hipSuccess) return e;
   if (rate_khz <= 0) return hipSuccess;
@@ -903,6 +947,49 @@ struct Seg {
   uint32_t seq, pos0, row0, T;
 };
 
+// A softmax layer's mix over rings in 4 bits, QKV to O: the rows' keys and
+// values (qk-normed with their queries) into the rings, then their attention.
+// A prefill step's chunks go together where none reaches past the ring's
+// wrap; one that does goes a token at a time, each row seeing the whole window
+// before its own (dd.sm.toks).
+static int kv4_mix(ana_ctx* c, uint32_t l, uint32_t B, const uint32_t* seq, const uint32_t* pos,
+                   const std::vector<Seg>* segs, bool fresh_all) {
+  const ana_config& cf = c->cfg;
+  const Blk& b = c->blk[l];
+  const uint32_t d = cf.d, hd = d / cf.heads;
+  const Kv4 kc = kv4_of(c, l);
+  auto rows = [&](const Kv4Rows& r, uint32_t row0) -> int {
+    float* x = c->QKV + (size_t)row0 * 3 * d;
+    const Kv4Mat q{x, 3ull * d, hd}, k{x + d, 3ull * d, hd}, v{x + 2 * d, 3ull * d, hd};
+    HIPCHK(c, launch_kv4_write(kc, r, ET_F32, k, v, cf.qk ? c->W + b.gk : nullptr, cf.qk ? c->W + b.gq : nullptr,
+                               cf.qk ? &q : nullptr, cf.heads, c->st));
+    Kv4Attend a{};
+    a.c = kc;
+    a.r = r;
+    a.q = q;
+    a.o = Kv4Mat{c->O + (size_t)row0 * d, d, hd};
+    a.hq = cf.heads;
+    a.scale = 1.0f / sqrtf((float)hd);
+    a.sink = cf.sinks ? c->W + b.sink : nullptr;
+    a.part = c->d_kpart;
+    // (the whole ring: one split for every position, so a row's result does
+    // not depend on what is decoded beside it or on the call's length)
+    kv4_split(kc, r.n, r.rows, r.off != nullptr, cf.heads, 0, &a.nsplit, &a.tps);
+    HIPCHK(c, launch_kv4_attend(a, ET_F32, c->st));
+    return ANA_OK;
+  };
+  if (!segs) return rows(Kv4Rows{seq, pos, nullptr, B, B}, 0);
+  const uint32_t n = (uint32_t)segs->size();
+  if (int r = rows(Kv4Rows{c->d_kseg, c->d_kseg + n, c->d_kseg + 2 * n, n, B}, 0)) return r;
+  if (fresh_all) return ANA_OK;
+  for (const Seg& sg : *segs) {
+    if ((uint64_t)sg.pos0 + sg.T <= cf.ctx) continue;
+    for (uint32_t t = sg.row0; t < sg.row0 + sg.T; t++)
+      if (int r = rows(Kv4Rows{c->d_rseq + t, c->d_rpos + t, nullptr, 1, 1}, t)) return r;
+  }
+  return ANA_OK;
+}
+
 // every layer for B rows of X (embedded already). Decode (segs == nullptr):
 // row b is sequence seq[b] at position pos[b] (device arrays). Prefill:
 // the rows are chunks of several sequences (segs); the products run over all
@@ -961,6 +1048,20 @@ static int run_layers(ana_ctx* c, uint32_t B, const uint32_t* seq, const uint32_
       HIPCHK(c, hipMemcpyAsync(c->d_gtab, c->h_gtab.data(), sizeof(GlaSub) * nsub, hipMemcpyHostToDevice, c->st));
     HIPCHK(c, hipMemcpyAsync(c->d_rseq, c->h_rseq.data(), 4 * (size_t)B, hipMemcpyHostToDevice, c->st));
     HIPCHK(c, hipMemcpyAsync(c->d_rpos, c->h_rpos.data(), 4 * (size_t)B, hipMemcpyHostToDevice, c->st));
+    if (c->kv4) {
+      // the chunks for the rings' operators; one that reaches past the wrap
+      // has no place there, and goes token by token
+      const uint32_t n = (uint32_t)segs->size();
+      c->h_kseg.resize(3 * n + 1);
+      for (uint32_t i = 0; i < n; i++) {
+        const Seg& sg = (*segs)[i];
+        c->h_kseg[i] = (uint64_t)sg.pos0 + sg.T <= cf.ctx ? sg.seq : 0xFFFFFFFFu;
+        c->h_kseg[n + i] = sg.pos0;
+        c->h_kseg[2 * n + i] = sg.row0;
+      }
+      c->h_kseg[3 * n] = B;
+      HIPCHK(c, hipMemcpyAsync(c->d_kseg, c->h_kseg.data(), 4 * c->h_kseg.size(), hipMemcpyHostToDevice, c->st));
+    }
   }
   for (uint32_t l = 0; l < cf.layers; l++) {
     const Blk& b = c->blk[l];
@@ -995,6 +1096,16 @@ static int run_layers(ana_ctx* c, uint32_t B, const uint32_t* seq, const uint32_
     } else if (b.gla) {
       HIPCHK(c, launch_gla_serial(c->QKV, c->Z, cf.rglru ? W + b.lam : nullptr, sref(c, l), c->O, c->d_grun,
                                   (uint32_t)c->h_grun.size(), d, cf.heads, cf.rglru, c->st));
+    } else if (c->kv4) {
+      int r;
+      if (chunk) {
+        r = kv4_mix(c, l, B, seq, pos, segs, fresh_all);
+      } else {
+        ProfScope ps(c, ANA_K_ATTN, c->attn_bytes);
+        r = kv4_mix(c, l, B, seq, pos, nullptr, true);
+      }
+      if (r) return r;
+      c->oh_ok = false;   // (the outputs are in fp32)
     } else {
       AttnArgs a{};
       a.gq = cf.qk ? W + b.gq : nullptr;
@@ -1106,7 +1217,8 @@ static double attn_bytes_of(const ana_ctx* c, const uint32_t* pos, uint32_t n, u
   for (uint32_t i = 0; i < n; i++) {
     const uint64_t p = (uint64_t)pos[i] + plus;
     const uint64_t live = std::min<uint64_t>(p, cf.ctx - 1) + 1;
-    b += 4.0 * cf.d * (2.0 * live + 2.0 + 3.0 + 1.0);
+    if (c->kv4) b += cf.d * (34.0 / 32.0 * (live + 1.0) + 4.0 * (3.0 + 1.0));
+    else b += 4.0 * cf.d * (2.0 * live + 2.0 + 3.0 + 1.0);
   }
   return b;
 }
@@ -1264,10 +1376,26 @@ static int score_head(ana_ctx* c, uint32_t r0, uint32_t g) {
 // With ce (scoring, Evaluate.bend's window.go): sequence i feeds its first
 // len[i] - 1 tokens, and after each fed token t the head's G.lse minus the
 // logit of token t + 1 goes to ce (len[i] - 1 values a sequence, in order).
+// With lp, the same rows' log probabilities in place of ce.
+struct LpOut {
+  uint32_t top;
+  float *lp, *ent;
+  uint32_t *rank, *top_tok;
+  float* top_lp;
+};
+// the device's results of rows rows (at lp_rows a kind), from row r0 on
+static LogprobArgs lp_args(const ana_ctx* c, const float* logits, uint32_t n, const uint32_t* tok, uint32_t top, uint32_t r0) {
+  uint32_t* p = c->d_lp;
+  const size_t R = c->lp_rows;
+  return LogprobArgs{logits, c->cfg.vocab, n, c->cfg.vocab, top, tok, reinterpret_cast<float*>(p) + r0,
+                     reinterpret_cast<float*>(p + R) + r0, p + 2 * R + r0, p + 3 * R + (size_t)r0 * top,
+                     reinterpret_cast<float*>(p + 3 * R + R * top) + (size_t)r0 * top, c->d_lpw};
+}
 static int feeds_n(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq, const uint32_t* pos,
-                   const uint32_t* len, const uint32_t* toks, float* ce = nullptr) {
+                   const uint32_t* len, const uint32_t* toks, float* ce = nullptr, const LpOut* lo = nullptr) {
   if (n == 0) return ANA_OK;
   if (!seq || !pos || !len || !toks) return fail(c, ANA_EINVAL, "%s: null argument", fn);
+  const bool score = ce || lo;
   std::vector<uint8_t> seen(c->max_seqs, 0);
   std::vector<uint64_t> off(n), coff(n);
   std::vector<uint32_t> flen(n);
@@ -1277,9 +1405,9 @@ static int feeds_n(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq, 
     if (seen[seq[i]]++) return fail(c, ANA_EINVAL, "%s: sequence %u listed twice", fn, seq[i]);
     off[i] = total;
     total += len[i];
-    flen[i] = ce ? (len[i] ? len[i] - 1 : 0) : len[i];
+    flen[i] = score ? (len[i] ? len[i] - 1 : 0) : len[i];
     coff[i] = ctot;
-    ctot += ce ? flen[i] : 0;
+    ctot += score ? flen[i] : 0;
   }
   for (uint64_t i = 0; i < total; i++)
     if (toks[i] >= c->cfg.vocab) return fail(c, ANA_EINVAL, "%s: token %u outside the vocabulary", fn, toks[i]);
@@ -1289,6 +1417,7 @@ static int feeds_n(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq, 
   std::vector<uint32_t> rows, tg, rcp;
   std::vector<uint64_t> cix;
   std::vector<float> hce;
+  std::vector<uint32_t> hlp;
   auto flush = [&]() -> int {
     if (segs.empty()) return ANA_OK;
     const uint32_t M = (uint32_t)rows.size();
@@ -1306,20 +1435,40 @@ static int feeds_n(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq, 
     HIPCHK(c, launch_embed(c->W, c->d_tok, d, M, c->X, nullptr, c->st));
     if (int r = run_layers(c, M, nullptr, nullptr, &segs)) return r;
     HIPCHK(c, launch_copy_rows(c->X, c->d_rcp, (uint32_t)segs.size(), d, c->xs, c->st));
-    if (ce) {
+    if (score) {
       HIPCHK(c, hipMemcpyAsync(c->d_tgt, tg.data(), 4 * (size_t)M, hipMemcpyHostToDevice, c->st));
       for (uint32_t r0 = 0; r0 < M; r0 += c->sc_rows) {
         const uint32_t g = std::min(c->sc_rows, M - r0);
         if (int r = score_head(c, r0, g)) return r;
-        HIPCHK(c, launch_ce(c->SC, c->cfg.vocab, g, c->d_tgt + r0, c->d_ce + r0, c->st));
+        if (lo) HIPCHK(c, launch_logprobs(lp_args(c, c->SC, g, c->d_tgt + r0, lo->top, r0), ET_F32, c->st));
+        else HIPCHK(c, launch_ce(c->SC, c->cfg.vocab, g, c->d_tgt + r0, c->d_ce + r0, c->st));
       }
-      hce.resize(M);
-      HIPCHK(c, hipMemcpyAsync(hce.data(), c->d_ce, 4 * (size_t)M, hipMemcpyDeviceToHost, c->st));
+      if (lo) {
+        const size_t R = c->lp_rows, w = 3 + 2 * (size_t)lo->top;
+        hlp.resize(M * w);
+        const size_t at[5] = {0, R, 2 * R, 3 * R, 3 * R + R * lo->top}, per[5] = {1, 1, 1, lo->top, lo->top};
+        for (size_t k = 0, o = 0; k < 5; o += M * per[k], k++)
+          if (per[k])
+            HIPCHK(c, hipMemcpyAsync(hlp.data() + o, c->d_lp + at[k], 4 * M * per[k], hipMemcpyDeviceToHost, c->st));
+      } else {
+        hce.resize(M);
+        HIPCHK(c, hipMemcpyAsync(hce.data(), c->d_ce, 4 * (size_t)M, hipMemcpyDeviceToHost, c->st));
+      }
     }
     // the host rows are read by the copies above before they change
     HIPCHK(c, hipStreamSynchronize(c->st));
-    if (ce)
-      for (uint32_t r = 0; r < M; r++) ce[cix[r]] = hce[r];
+    for (uint32_t r = 0; ce && r < M; r++) ce[cix[r]] = hce[r];
+    for (uint32_t r = 0; lo && r < M; r++) {
+      const size_t k = lo->top;
+      const uint32_t* h = hlp.data();
+      memcpy(lo->lp + cix[r], h + r, 4);
+      memcpy(lo->ent + cix[r], h + M + r, 4);
+      lo->rank[cix[r]] = h[2 * (size_t)M + r];
+      if (k) {
+        memcpy(lo->top_tok + cix[r] * k, h + 3 * (size_t)M + r * k, 4 * k);
+        memcpy(lo->top_lp + cix[r] * k, h + 3 * (size_t)M + M * k + r * k, 4 * k);
+      }
+    }
     segs.clear();
     rows.clear();
     tg.clear();
@@ -1348,7 +1497,7 @@ static int feeds_n(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq, 
         if (int r = flush()) return r;
       segs.push_back(Seg{seq[i], pos[i] + t0, (uint32_t)rows.size(), T});
       rows.insert(rows.end(), toks + off[i] + t0, toks + off[i] + t0 + T);
-      if (ce)
+      if (score)
         for (uint32_t t = t0; t < t0 + T; t++) {
           tg.push_back(toks[off[i] + t + 1]);
           cix.push_back(coff[i] + t);
@@ -1380,6 +1529,24 @@ extern "C" int ana_score_n(ana_ctx* c, uint32_t n, const uint32_t* seq, const ui
   if (!c) return ANA_EINVAL;
   if (!ce && n) return fail(c, ANA_EINVAL, "ana_score_n: null output");
   return feeds_n(c, "ana_score_n", n, seq, pos, len, toks, ce);
+}
+
+// the outputs of the log probabilities' calls
+static int check_lp(ana_ctx* c, const char* fn, const LpOut& o, bool given) {
+  if (o.top > kLpMaxTop || o.top > c->cfg.vocab)
+    return fail(c, ANA_EINVAL, "%s: %u alternatives (at most %u)", fn, o.top, std::min(kLpMaxTop, c->cfg.vocab));
+  if (!o.ent || (given && (!o.lp || !o.rank)) || (o.top && (!o.top_tok || !o.top_lp)))
+    return fail(c, ANA_EINVAL, "%s: null output", fn);
+  return ANA_OK;
+}
+
+extern "C" int ana_score_logprobs_n(ana_ctx* c, uint32_t n, const uint32_t* seq, const uint32_t* pos,
+                                    const uint32_t* len, const uint32_t* toks, uint32_t top, float* lp, float* ent,
+                                    uint32_t* rank, uint32_t* top_tok, float* top_lp) {
+  if (!c) return ANA_EINVAL;
+  const LpOut o{top, lp, ent, rank, top_tok, top_lp};
+  if (int r = check_lp(c, "ana_score_logprobs_n", o, true)) return r;
+  return feeds_n(c, "ana_score_logprobs_n", n, seq, pos, len, toks, nullptr, &o);
 }
 
 // the listed sequences' residual rows, gathered (one sequence's in place)
@@ -1424,6 +1591,33 @@ extern "C" int ana_stats(ana_ctx* c, uint32_t n, const uint32_t* seq, const uint
   HIPCHK(c, hipMemcpyAsync(prob, dp, 4 * n, hipMemcpyDeviceToHost, c->st));
   HIPCHK(c, hipMemcpyAsync(alt, dalt, 4 * n, hipMemcpyDeviceToHost, c->st));
   HIPCHK(c, hipMemcpyAsync(alt_prob, dpa, 4 * n, hipMemcpyDeviceToHost, c->st));
+  HIPCHK(c, hipStreamSynchronize(c->st));
+  return ANA_OK;
+}
+
+extern "C" int ana_logprobs(ana_ctx* c, uint32_t n, const uint32_t* seq, const uint32_t* tok, uint32_t top, float* lp,
+                            float* ent, uint32_t* rank, uint32_t* top_tok, float* top_lp) {
+  if (!c) return ANA_EINVAL;
+  const char* fn = "ana_logprobs";
+  const LpOut o{top, lp, ent, rank, top_tok, top_lp};
+  if (int r = check_lp(c, fn, o, tok != nullptr)) return r;
+  const float* x;
+  if (int r = head_of(c, fn, n, seq, &x)) return r;
+  for (uint32_t i = 0; tok && i < n; i++)
+    if (tok[i] >= c->cfg.vocab) return fail(c, ANA_EINVAL, "%s: token %u outside the vocabulary", fn, tok[i]);
+  if (int r = run_head(c, x, n, false)) return r;
+  if (tok) HIPCHK(c, hipMemcpyAsync(c->d_tgt, tok, 4 * n, hipMemcpyHostToDevice, c->st));
+  const LogprobArgs a = lp_args(c, c->LG, n, tok ? c->d_tgt : nullptr, top, 0);
+  HIPCHK(c, launch_logprobs(a, ET_F32, c->st));
+  if (tok) {
+    HIPCHK(c, hipMemcpyAsync(lp, a.lp, 4 * n, hipMemcpyDeviceToHost, c->st));
+    HIPCHK(c, hipMemcpyAsync(rank, a.rank, 4 * n, hipMemcpyDeviceToHost, c->st));
+  }
+  HIPCHK(c, hipMemcpyAsync(ent, a.ent, 4 * n, hipMemcpyDeviceToHost, c->st));
+  if (top) {
+    HIPCHK(c, hipMemcpyAsync(top_tok, a.top_tok, 4 * (size_t)n * top, hipMemcpyDeviceToHost, c->st));
+    HIPCHK(c, hipMemcpyAsync(top_lp, a.top_lp, 4 * (size_t)n * top, hipMemcpyDeviceToHost, c->st));
+  }
   HIPCHK(c, hipStreamSynchronize(c->st));
   return ANA_OK;
 }
@@ -1925,8 +2119,27 @@ extern "C" int ana_state(ana_ctx* c, uint32_t seq, uint32_t layer, float* out, s
     const uint64_t end = layer + 1 < c->cfg.layers ? c->layer_off[layer + 1] : c->seq_stride;
     cnt = end - c->layer_off[layer];
   }
+  const bool ring4 = c->kv4 && layer < c->cfg.layers && !c->blk[layer].gla;
+  if (ring4) cnt = 2ull * c->cfg.ctx * c->cfg.d;
   if (n != cnt) return fail(c, ANA_EINVAL, "ana_state: layer %u holds %zu floats, not %zu", layer, cnt, n);
   HIPCHK(c, hipSetDevice(c->device));
+  if (ring4) {
+    // the rings as values, as many slots at a time as the step's rows hold
+    const ana_config& cf = c->cfg;
+    const uint32_t d = cf.d, step = std::min(c->rows, cf.ctx);
+    for (uint32_t s = 0; s < cf.ctx; s += step) {
+      const uint32_t m = std::min(step, cf.ctx - s);
+      const uint32_t rows[4] = {seq, s, 0, m};
+      HIPCHK(c, hipMemcpyAsync(c->d_kseg, rows, sizeof rows, hipMemcpyHostToDevice, c->st));
+      float* v = c->QKV + (size_t)m * d;
+      HIPCHK(c, launch_kv4_read(kv4_of(c, layer), Kv4Rows{c->d_kseg, c->d_kseg + 1, c->d_kseg + 2, 1, m}, ET_F32,
+                                Kv4Mat{c->QKV, d, d / cf.heads}, Kv4Mat{v, d, d / cf.heads}, c->st));
+      HIPCHK(c, hipMemcpyAsync(out + (size_t)s * d, c->QKV, 4 * (size_t)m * d, hipMemcpyDeviceToHost, c->st));
+      HIPCHK(c, hipMemcpyAsync(out + ((size_t)cf.ctx + s) * d, v, 4 * (size_t)m * d, hipMemcpyDeviceToHost, c->st));
+      HIPCHK(c, hipStreamSynchronize(c->st));
+    }
+    return ANA_OK;
+  }
   HIPCHK(c, hipMemcpyAsync(out, src, 4 * cnt, hipMemcpyDeviceToHost, c->st));
   HIPCHK(c, hipStreamSynchronize(c->st));
   return ANA_OK;

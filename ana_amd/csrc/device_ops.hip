@@ -42,7 +42,8 @@ int check_cache(const char* fn, const ana_kv4* c, Kv4* o) {
   if (!c || !c->data) return fail_call(ANA_EINVAL, "%s: null cache", fn);
   if (const char* why = shape_problem(c->seqs, c->slots, c->heads, c->hd)) return fail_call(ANA_EINVAL, "%s: %s", fn, why);
   if ((uintptr_t)c->data % 16) return fail_call(ANA_EINVAL, "%s: the cache is not on a 16-byte border", fn);
-  *o = Kv4{(uint8_t*)c->data, c->seqs, c->slots, (c->slots + 31) / 32, c->heads, c->hd};
+  *o = Kv4{(uint8_t*)c->data, kv4_seq_bytes(c->slots, c->heads, c->hd), c->seqs, c->slots, (c->slots + 31) / 32, c->heads,
+           c->hd};
   return ANA_OK;
 }
 
@@ -82,7 +83,7 @@ int launched(const char* fn, hipError_t e) {
 
 extern "C" uint64_t ana_kv4_bytes(uint32_t seqs, uint32_t slots, uint32_t heads, uint32_t hd) {
   if (shape_problem(seqs, slots, heads, hd)) return 0;
-  return (uint64_t)seqs * heads * ((slots + 31) / 32) * kv4_record(hd);
+  return seqs * kv4_seq_bytes(slots, heads, hd);
 }
 
 extern "C" int ana_kv4_write(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_mat* k, const ana_mat* v,
@@ -129,7 +130,7 @@ static int check_heads(const char* fn, const ana_kv4* c, const ana_kv4_rows* r, 
 
 extern "C" uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq, uint64_t live) {
   if (!c || !r || hq == 0 || shape_problem(c->seqs, c->slots, c->heads, c->hd) || hq % c->heads) return 0;
-  const Kv4 kc{nullptr, c->seqs, c->slots, (c->slots + 31) / 32, c->heads, c->hd};
+  const Kv4 kc{nullptr, 0, c->seqs, c->slots, (c->slots + 31) / 32, c->heads, c->hd};
   uint32_t ns, tps;
   kv4_split(kc, r->n, r->rows, r->off != nullptr, hq, live, &ns, &tps);
   return 4 * kv4_part_floats(r->rows, hq, c->hd, ns);

@@ -18,9 +18,13 @@ namespace ana {
 // are written at once never share a byte.
 struct Kv4 {
   uint8_t* data;
+  uint64_t seq_bytes;   // from a sequence's records to the next one's (a multiple of 16)
   uint32_t seqs, slots, tiles, heads, hd;
 };
 __host__ __device__ inline uint32_t kv4_record(uint32_t hd) { return 34 * hd; }
+inline uint64_t kv4_seq_bytes(uint32_t slots, uint32_t heads, uint32_t hd) {
+  return (uint64_t)heads * (((uint64_t)slots + 31) / 32) * kv4_record(hd);
+}
 
 // The rows of a call: sequence i (cache place seq[i], or i) has rows off[i]
 // .. off[i + 1] - 1 (or row i alone) at positions from pos[i].
@@ -40,7 +44,8 @@ enum ElemType : int { ET_F32 = 0, ET_BF16 = 1, ET_F16 = 2 };
 inline bool kv4_fits(uint32_t hd) { return hd == 32 || hd == 64 || hd == 128; }
 
 // k and v into the cache. With gk, k is qk-normed first, and with q (f32) the
-// query rows are normed in place with gq (one launch for a decoder layer).
+// query rows of sequences with a place are normed in place with gq (one launch
+// for a decoder layer).
 hipError_t launch_kv4_write(const Kv4& c, const Kv4Rows& r, int type, const Kv4Mat& k, const Kv4Mat& v,
                             const float* gk, const float* gq, const Kv4Mat* q, uint32_t qheads, hipStream_t st);
 // the values that the cache holds for the rows

@@ -103,7 +103,7 @@ __device__ __forceinline__ RowAt row_at(const Kv4& c, const Kv4Rows& r, uint32_t
 }
 
 __device__ __forceinline__ uint8_t* record_of(const Kv4& c, uint32_t q, uint32_t head, uint32_t tile) {
-  return c.data + (((uint64_t)q * c.heads + head) * c.tiles + tile) * kv4_record(c.hd);
+  return c.data + q * c.seq_bytes + ((uint64_t)head * c.tiles + tile) * kv4_record(c.hd);
 }
 
 // |x| 2^(127 - b) as an E2M1 code, to the nearest, ties to the even code.
@@ -151,7 +151,7 @@ __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k,
     for (int e = 0; e < 8; e++) x[e] = (x[e] * n) * (1.0f + g[sub * 8 + e]);
   }
   if (z == 2) {
-    if (a.on) store8(p, vec, x);
+    if (a.ok) store8(p, vec, x);
     return;
   }
   bool put = a.ok && a.last - a.p < c.slots;

@@ -58,6 +58,15 @@ extern "C" {
 #define ANA_BF16 2       /* matrices read as bfloat16 (rounded once at load); fp32
                             activations, accumulation and state: logits within 2e-2 */
 
+/* ANA_FAST_FP32 | ANA_KV4 or ANA_BF16 | ANA_KV4: the softmax layers' K and V rings
+ * in 4 bits, 7.5 times smaller than in fp32 (the cache of ana_kv4 below: at d 768 and ctx
+ * 2048, 12.6 MB a layer and sequence become 1.7 MB). Every row attends
+ * to keys and values as the rings hold them, its own too; all else is the mode's. The
+ * rounding is the checkpoint's to bear: the modes' tolerances do not cover it. Head
+ * dimensions of 32 and 64; the one-sequence loops take the step graphs. ANA_EUNSUP with
+ * ANA_EXACT_FP32 */
+#define ANA_KV4 0x100
+
 /* bend/Config.bend:7-10 */
 typedef struct {
   uint32_t vocab, ctx, d, f, layers, heads;
@@ -66,7 +75,8 @@ typedef struct {
 
 typedef struct {
   int device;              /* HIP device ordinal */
-  int numerics;            /* ANA_EXACT_FP32, ANA_FAST_FP32 or ANA_BF16 */
+  int numerics;            /* ANA_EXACT_FP32, ANA_FAST_FP32 or ANA_BF16, the last two
+                              also with ANA_KV4 */
   uint32_t max_seqs;       /* sequences the context keeps state for (>= 1) */
   uint32_t prefill_chunk;  /* tokens of each sequence a prefill step takes; 0 = 64, as
                               ANA_PREFILL_CHUNK. In ANA_BF16, and past the ring's wrap, exactly
@@ -150,6 +160,23 @@ int ana_logits(struct ana_ctx* ctx, uint32_t n, const uint32_t* seq, float* out)
 int ana_stats(struct ana_ctx* ctx, uint32_t n, const uint32_t* seq, const uint32_t* tok, float* prob,
               uint32_t* alt, float* alt_prob);
 
+/* After each listed sequence's last fed token, what ana_row_logprobs gives of
+ * the head's logits: the log probability and rank of tok[i] (tok NULL:
+ * neither is written), the entropy, and the `top` (0 .. 64) likeliest tokens
+ * with their log probabilities ([n][top]), ties to the lower index. No
+ * counterpart in the reference (ana_stats gives its one rival); the sums are
+ * f32 in every mode. */
+int ana_logprobs(struct ana_ctx* ctx, uint32_t n, const uint32_t* seq, const uint32_t* tok, uint32_t top,
+                 float* lp, float* ent, uint32_t* rank, uint32_t* top_tok, float* top_lp);
+
+/* ana_score_n's windows with the same results in place of its summands:
+ * after each fed token t, token t + 1's log probability and rank, the
+ * entropy and the alternatives; len[i] - 1 of each a sequence, one sequence
+ * after another. */
+int ana_score_logprobs_n(struct ana_ctx* ctx, uint32_t n, const uint32_t* seq, const uint32_t* pos,
+                         const uint32_t* len, const uint32_t* toks, uint32_t top, float* lp, float* ent,
+                         uint32_t* rank, uint32_t* top_tok, float* top_lp);
+
 /* Greedy's pick on the device: dd.top (bend/Dense/Decode.bend:475-484,
  * 648-660), the least index reaching the maximum logit; vocab when no logit
  * does (a NaN maximum), where the caller falls back to ana_pick. */
@@ -199,7 +226,8 @@ int ana_generate_noalloc(struct ana_ctx* ctx, uint32_t n, const uint32_t* seq, c
                          uint32_t* out);
 
 /* Copy one sequence's state out (for parity checks): layer l's GLA S
- * (heads x hd x hd floats) or K ring then V ring (2 x ctx x d floats); l ==
+ * (heads x hd x hd floats) or K ring then V ring (2 x ctx x d floats; with
+ * ANA_KV4 the values that the codes stand for); l ==
  * layers gives the residual row (d floats). n is the float count of out. */
 int ana_state(struct ana_ctx* ctx, uint32_t seq, uint32_t layer, float* out, size_t n);
 
