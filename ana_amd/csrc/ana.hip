@@ -459,12 +459,8 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
     uint64_t most = 0;
     const Kv4 kc = kv4_of(c, 0);
     for (uint32_t r = 1; r <= c->rows; r++) {
-      uint32_t ns, tps;
-      kv4_split(kc, r, r, true, cf.heads, 0, &ns, &tps);
-      most = std::max(most, kv4_part_floats(r, cf.heads, hd, ns));
-      if (r > c->wb) continue;
-      kv4_split(kc, r, r, false, cf.heads, 0, &ns, &tps);
-      most = std::max(most, kv4_part_floats(r, cf.heads, hd, ns));
+      most = std::max(most, kv4_part_floats(r, cf.heads, hd, kv4_split(kc, r, r, true, cf.heads, 0)));
+      if (r <= c->wb) most = std::max(most, kv4_part_floats(r, cf.heads, hd, kv4_split(kc, r, r, false, cf.heads, 0)));
     }
     if ((e = dalloc(&c->d_kpart, most)) != hipSuccess || (e = dalloc(&c->d_kseg, 3 * (uint64_t)c->seg_cap + 1)) != hipSuccess)
       return bad(e);
@@ -972,9 +968,8 @@ static int kv4_mix(ana_ctx* c, uint32_t l, uint32_t B, const uint32_t* seq, cons
     a.scale = 1.0f / sqrtf((float)hd);
     a.sink = cf.sinks ? c->W + b.sink : nullptr;
     a.part = c->d_kpart;
-    // (the whole ring: one split for every position, so a row's result does
-    // not depend on what is decoded beside it or on the call's length)
-    kv4_split(kc, r.n, r.rows, r.off != nullptr, cf.heads, 0, &a.nsplit, &a.tps);
+    // (for the whole ring: the captured steps serve every position)
+    a.nsplit = kv4_split(kc, r.n, r.rows, r.off != nullptr, cf.heads, 0);
     HIPCHK(c, launch_kv4_attend(a, ET_F32, c->st));
     return ANA_OK;
   };

@@ -131,8 +131,7 @@ static int check_heads(const char* fn, const ana_kv4* c, const ana_kv4_rows* r, 
 extern "C" uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq, uint64_t live) {
   if (!c || !r || hq == 0 || shape_problem(c->seqs, c->slots, c->heads, c->hd) || hq % c->heads) return 0;
   const Kv4 kc{nullptr, 0, c->seqs, c->slots, (c->slots + 31) / 32, c->heads, c->hd};
-  uint32_t ns, tps;
-  kv4_split(kc, r->n, r->rows, r->off != nullptr, hq, live, &ns, &tps);
+  const uint32_t ns = kv4_split(kc, r->n, r->rows, r->off != nullptr, hq, live);
   return 4 * kv4_part_floats(r->rows, hq, c->hd, ns);
 }
 
@@ -148,7 +147,7 @@ extern "C" int ana_kv4_attend(const ana_kv4* c, const ana_kv4_rows* r, int type,
   if (int e = check_mat(fn, "q", q, type, r, hq, c->hd, &a.q)) return e;
   if (int e = check_mat(fn, "o", o, type, r, hq, c->hd, &a.o)) return e;
   if (r->n == 0 || r->rows == 0) return ANA_OK;
-  kv4_split(a.c, r->n, r->rows, r->off != nullptr, hq, live, &a.nsplit, &a.tps);
+  a.nsplit = kv4_split(a.c, r->n, r->rows, r->off != nullptr, hq, live);
   const uint64_t need = 4 * kv4_part_floats(r->rows, hq, c->hd, a.nsplit);
   if (need && (!ws || ws_bytes < need))
     return fail_call(ANA_EINVAL, "%s: a workspace of %llu bytes, not %llu", fn, (unsigned long long)need,

@@ -62,13 +62,12 @@ struct Kv4Attend {
   float scale;
   const float* sink;   // [hq] or nullptr
   float* part;         // partials [rows][hq][nsplit][kKv4PartHead + hd], when nsplit > 1
-  uint32_t nsplit, tps;  // pieces of the slots, tiles each but the last
+  uint32_t nsplit;     // pieces that a sequence's slots are cut into at most
 };
-// how a call's slots are split (live: the most positions a sequence holds
-// after the call, as far as the caller knows; 0: the ring's slots), and the
-// floats of partials that takes
-void kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live, uint32_t* nsplit,
-               uint32_t* tps);
+// the pieces of a call (live: the most positions a sequence holds after it,
+// as far as the caller knows; 0: the ring's slots), and the floats of
+// partials they take
+uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live);
 inline uint64_t kv4_part_floats(uint32_t rows, uint32_t hq, uint32_t hd, uint32_t nsplit) {
   return nsplit > 1 ? (uint64_t)rows * hq * nsplit * (kKv4PartHead + hd) : 0;
 }

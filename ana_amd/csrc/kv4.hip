@@ -106,16 +106,6 @@ __device__ __forceinline__ uint8_t* record_of(const Kv4& c, uint32_t q, uint32_t
   return c.data + q * c.seq_bytes + ((uint64_t)head * c.tiles + tile) * kv4_record(c.hd);
 }
 
-// |x| 2^(127 - b) as an E2M1 code, to the nearest, ties to the even code.
-// From 1 up a code is the float's exponent and first mantissa bit; below, the
-// halves.
-__device__ __forceinline__ uint32_t e2m1(float y) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, y);
-  const uint32_t hi = ((u + 0x1FFFFFu + ((u >> 22) & 1)) >> 22) - 252;
-  const uint32_t lo = (uint32_t)(int)rintf(y + y);
-  return min(y < 1.0f ? lo : hi, 7u);
-}
-
 // A call's keys and values into the cache: a workgroup takes 32 rows of one
 // head, eight dims a thread (a slot's codes of one lane of the attention are
 // hd / 4 dims of a key and hd / 16 of a value). z = 0 the keys, 1 the
@@ -172,10 +162,14 @@ __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k,
   const int e8 = (int)(top >> 23) - 2 + ((top & 0x7FFFFFu) > 0x600000u ? 1 : 0);
   const uint32_t b = bad ? 255u : (uint32_t)min(max(e8, 2), 252);
   const float f = __builtin_bit_cast(float, (254u - min(b, 252u)) << 23);
+  // (to the nearest code, ties to the even one, past the largest to it; the
+  // same in integer steps took 14 instructions a value where this takes 1.5,
+  // and 32 us where it takes 24 for 16384 rows of 8 heads of 128 in bf16)
   uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 8; e++)
-    w |= (e2m1(fabsf(x[e]) * f) | (__builtin_bit_cast(uint32_t, x[e]) >> 31 << 3)) << (4 * e);
+  static_for<4>([&](auto u) {
+    constexpr int e = 2 * decltype(u)::value;
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(w, x[e] * f, x[e + 1] * f, 1.0f, decltype(u)::value);
+  });
   if (bad) w = 0;
   if (!put) return;
   const uint32_t slot = a.p % c.slots, s = slot % 32, h = s / 16, m = s % 16, dim = sub * 8;
@@ -201,45 +195,63 @@ __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k,
 }
 
 // k_kv4_write the other way: the values that the cache holds for the rows
-// (zeros for a sequence without a place in the cache)
+// (zeros for a sequence without a place in the cache). A thread takes 16
+// bytes of the outputs, so that a store's lanes write whole lines (with eight
+// f32 a thread, in two stores of every other 16 bytes, 8384 rows of 12 heads
+// of 64 took 37 us).
 template <typename T, int D>
-__global__ __launch_bounds__(4 * D) void k_kv4_read(Kv4 c, Kv4Rows r, Kv4Mat k, Kv4Mat v, uint32_t vec) {
-  constexpr uint32_t TPR = D / 8;
+__global__ __launch_bounds__(32 * D * sizeof(T) / 16) void k_kv4_read(Kv4 c, Kv4Rows r, Kv4Mat k, Kv4Mat v, uint32_t vec) {
+  constexpr uint32_t E = 16 / sizeof(T), TPR = D / E;   // outputs a thread, threads a row
   const uint32_t tid = threadIdx.x, sub = tid % TPR, row = blockIdx.x * 32 + tid / TPR, head = blockIdx.y;
   const uint32_t i0 = r.off ? find_seq(r.off, r.n, blockIdx.x * 32) : 0;
   const RowAt a = row_at(c, r, row, i0);
   if (!a.on) return;
   uint32_t w = 0, b = 2;
   if (a.ok) {
-    const uint32_t slot = a.p % c.slots, s = slot % 32, h = s / 16, m = s % 16, dim = sub * 8;
+    const uint32_t slot = a.p % c.slots, s = slot % 32, h = s / 16, m = s % 16, dim = sub * E;
     const uint8_t* rec = record_of(c, a.q, head, slot / 32);
+    auto codes = [&](const uint8_t* at) -> uint32_t {
+      if constexpr (E == 8) return *reinterpret_cast<const uint32_t*>(at);
+      else return *reinterpret_cast<const uint16_t*>(at);
+    };
     if (blockIdx.z == 0) {
       const uint32_t j = dim / (D / 4);
-      w = *reinterpret_cast<const uint32_t*>(rec + (j * 16 + m) * (D / 4) + h * (D / 8) + dim % (D / 4) / 2);
+      w = codes(rec + (j * 16 + m) * (D / 4) + h * (D / 8) + dim % (D / 4) / 2);
       b = rec[32 * D + (dim / 32 * 16 + m) * 2 + h];
     } else {
       const uint32_t j = m / 4, e = h * 4 + m % 4;
-      const uint8_t* at = rec + 16 * D + (j * 16 + dim / (D / 16)) * (D / 4) + e * (D / 32);
-      if constexpr (D == 128) {
-        w = *reinterpret_cast<const uint32_t*>(at);
+      // (a lane of the attention has D / 16 dims of a slot, its neighbours' are D / 4 bytes on)
+      const uint8_t* at = rec + 16 * D + (j * 16 + dim / (D / 16)) * (D / 4) + e * (D / 32) + dim % (D / 16) / 2;
+      if constexpr (E <= D / 16) {
+        w = codes(at);
       } else if constexpr (D == 64) {
         w = *reinterpret_cast<const uint16_t*>(at) | (uint32_t)*reinterpret_cast<const uint16_t*>(at + D / 4) << 16;
       } else {
 #pragma unroll
-        for (int u = 0; u < 4; u++) w |= (uint32_t)at[u * (D / 4)] << (8 * u);
+        for (uint32_t u = 0; u < E / 2; u++) w |= (uint32_t)at[u * (D / 4)] << (8 * u);
       }
       b = rec[33 * D + (dim / 32 * 4 + j) * 8 + e];
     }
   }
   const float f = b == 255 ? __builtin_nanf("") : __builtin_bit_cast(float, b << 23);
-  float x[8];
-  static_for<4>([&](auto u) {
+  float x[E];
+  static_for<E / 2>([&](auto u) {
     const f32x2_t t = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, decltype(u)::value);
     x[2 * u] = t[0] * f;
     x[2 * u + 1] = t[1] * f;
   });
   const Kv4Mat& dst = blockIdx.z == 0 ? k : v;
-  store8((T*)dst.p + (uint64_t)row * dst.row + (uint64_t)head * dst.head + sub * 8, vec, x);
+  T* p = (T*)dst.p + (uint64_t)row * dst.row + (uint64_t)head * dst.head + sub * E;
+  if (vec) {
+    typedef T vec_t __attribute__((ext_vector_type(E)));
+    vec_t y;
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) y[e] = (T)x[e];
+    *reinterpret_cast<vec_t*>(p) = y;
+  } else {
+#pragma unroll
+    for (uint32_t e = 0; e < E; e++) p[e] = (T)x[e];
+  }
 }
 
 // ---------------------------------------------------------------- attention
@@ -416,10 +428,19 @@ struct View {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-// a piece's partial result: its maximum and sum, then (on 16 bytes) its D outputs
-constexpr uint32_t kPartHead = kKv4PartHead;
+// A piece's partial result: its maximum and sum, then (on 16 bytes) its D
+// outputs. The first piece's third word says how many there are, or that the
+// only one was finished where it was made.
+constexpr uint32_t kPartHead = kKv4PartHead, kDone = 0xFFFFFFFFu;
 // pairs of a sequence up to which the few-row kernel takes it
 constexpr uint32_t kFewPairs = 16;
+// The pieces that `tiles` tiles are cut into, at most nsplit of at least
+// `least` tiles: the tiles of each but the last.
+constexpr uint32_t kFewTiles = 4, kManyTiles = 8;
+__device__ __forceinline__ uint32_t piece_tiles(uint32_t tiles, uint32_t nsplit, uint32_t least) {
+  const uint32_t n = max(1u, min(nsplit, tiles / least));
+  return (tiles + n - 1) / n;
+}
 // A running maximum is only raised once a score passes it by this much (in
 // base 2): probabilities then reach 2^kSlack, which costs f32 and bf16 no
 // digit, and most tiles rescale nothing.
@@ -549,8 +570,10 @@ __global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint
   const bool ok = q < a.c.seqs;
   const View view(last, a.c.slots);
   const uint32_t tiles = ok ? (view.live + 31) / 32 : 0u;
-  const uint32_t t0 = z * a.tps, t1 = z + 1 == a.nsplit ? tiles : min(tiles, t0 + a.tps);
-  if (a.nsplit > 1 && t0 >= t1) return;
+  const uint32_t per = piece_tiles(tiles, a.nsplit, kFewTiles);
+  const uint32_t t0 = z * per, t1 = min(tiles, t0 + per);
+  if (z && t0 >= t1) return;
+  const bool split = tiles > per;
   const uint32_t pm = m / NC, part = m % NC;
   const uint32_t t = (c0 + pm) / G, g = (c0 + pm) % G;
   const float sc = a.scale * kLog2e;
@@ -744,13 +767,14 @@ __global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint
       y += v * f;
     }
     const uint32_t row = row0 + (c0 + pp) / G, hd = head * G + (c0 + pp) % G;
-    if (a.nsplit > 1) {
-      float* out = a.part + (((uint64_t)row * a.hq + hd) * a.nsplit + z) * (D + kPartHead);
+    float* out = a.part + (((uint64_t)row * a.hq + hd) * a.nsplit + z) * (D + kPartHead);
+    if (a.nsplit > 1 && d == 0) {
+      if (z == 0) out[2] = __builtin_bit_cast(float, split ? (tiles + per - 1) / per : kDone);
+      out[0] = M;
+      out[1] = lsum;
+    }
+    if (split) {
       out[kPartHead + d] = y;
-      if (d == 0) {
-        out[0] = M;
-        out[1] = lsum;
-      }
     } else {
       float f;
       const float den = finish_sum(M, lsum, a.sink, hd, &f);
@@ -791,7 +815,9 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
   bf16x8_t(*ops)[2][OPS][64] = reinterpret_cast<bf16x8_t(*)[2][OPS][64]>(lds);   // [buffer][keys, values]
   const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, j = lane >> 4;
   const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t head = blockIdx.y, z = blockIdx.z, G = a.hq / a.c.heads;
+  // (key heads first: workgroups go round the eight XCDs, and a sequence's
+  // parts, each longer than the next, must not all meet the same ones)
+  const uint32_t head = blockIdx.x % a.c.heads, tile_i = blockIdx.x / a.c.heads, z = blockIdx.y, G = a.hq / a.c.heads;
   // the workgroup's sequence and its part of that sequence's pairs
   uint32_t i = 0, part_i = 0, before = 0;
   bool found = false;
@@ -809,12 +835,12 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
       const uint32_t o = __shfl_up(sum, k, 64);
       if (lane >= (uint32_t)k) sum += o;
     }
-    const unsigned long long hit = __ballot(before + sum > blockIdx.x);
+    const unsigned long long hit = __ballot(before + sum > tile_i);
     if (hit) {
       const int f = __ffsll((long long)hit) - 1;
       i = b + f;
       // (a sequence's last rows see the most: they start first)
-      part_i = before + __shfl(sum, f, 64) - 1 - blockIdx.x;
+      part_i = before + __shfl(sum, f, 64) - 1 - tile_i;
       found = true;
     } else {
       before += __shfl(sum, 63, 64);
@@ -835,7 +861,10 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
   const bool flat = last < a.c.slots;
   const uint32_t seen = flat ? pos + t_hi + 1 : view.live;
   const uint32_t tiles = ok ? (seen + 31) / 32 : 0u;
-  const uint32_t t0 = z * a.tps, t1 = z + 1 == a.nsplit ? tiles : min(tiles, t0 + a.tps);
+  const uint32_t per = piece_tiles(tiles, a.nsplit, kManyTiles);
+  const uint32_t t0 = z * per, t1 = min(tiles, t0 + per);
+  if (z && t0 >= t1) return;
+  const bool split = tiles > per;
 
   const uint8_t* base = record_of(a.c, ok ? q : 0, head, 0);
   // a wave's part of a record: the key codes of slots m and 16 + m, or the
@@ -1021,7 +1050,6 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
   // the outputs, 16 pairs at a time through the wave's part of LDS, so that a
   // store's lanes write whole rows
   float(*rows)[OR] = reinterpret_cast<float(*)[OR]>(lds + wv * (16 * OR * 4));
-  const bool split = a.nsplit > 1;
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
     const float ls = pair_sum(l[n]);
@@ -1034,7 +1062,9 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
     if (!split) {
       const float den = finish_sum(mx[n], ls, a.sink, hq, &f);
       inv = ok && den != 0.0f ? f / den : 0.0f;
-    } else if (on && j == 0) {
+    }
+    if (a.nsplit > 1 && on && j == 0) {
+      if (z == 0) part[2] = __builtin_bit_cast(float, split ? (tiles + per - 1) / per : kDone);
       part[0] = mx[n];
       part[1] = ls;
     }
@@ -1069,8 +1099,7 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
 
 // The pieces of a (row, query head), a wave each: weights 2^(m_z - M), then
 // the sink, then the division. D / 4 lanes take a piece's outputs, so several
-// pieces are in flight at once. The few-row kernel writes no piece past its
-// sequence's last slot; the other one writes all of them.
+// pieces are in flight at once.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a) {
   constexpr uint32_t L = D / 4, GR = 64 / L;   // lanes a piece, pieces at once
@@ -1078,20 +1107,11 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a) {
   const uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const uint32_t row = (uint32_t)(w / a.hq), hd = (uint32_t)(w % a.hq);
   if (row >= a.r.rows) return;
-  uint32_t i = row, len = 1;
-  if (a.r.off) {
-    i = find_seq(a.r.off, a.r.n, row);
-    const uint32_t o0 = a.r.off[i], o1 = a.r.off[i + 1];
-    if (row < o0 || row >= o1 || o1 > a.r.rows) return;
-    len = o1 - o0;
-  } else if (row >= a.r.n) {
-    return;
-  }
-  const uint32_t q = a.r.seq ? a.r.seq[i] : i;
-  const View view(a.r.pos[i] + len - 1, a.c.slots);
-  uint32_t nz = min(a.nsplit, ((view.live + 31) / 32 + a.tps - 1) / a.tps);
-  if (q >= a.c.seqs) nz = 0;
   const float* part = a.part + ((uint64_t)row * a.hq + hd) * a.nsplit * (D + kPartHead);
+  const uint32_t nz = __builtin_bit_cast(uint32_t, part[2]);
+  // (a row that no sequence has: its words are whatever they are)
+  if (a.r.off && (row < a.r.off[0] || row >= a.r.off[a.r.n])) return;
+  if (nz > a.nsplit) return;
   float M = -INFINITY;
   for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, part[z * (D + kPartHead)]);
   M = wmax(M);
@@ -1172,31 +1192,27 @@ hipError_t launch_kv4_read(const Kv4& c, const Kv4Rows& r, int type, const Kv4Ma
   return by_type(type, c.hd, [&](auto t, auto d) -> hipError_t {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    hipLaunchKernelGGL((k_kv4_read<T, D>), dim3((r.rows + 31) / 32, c.heads, 2), dim3(4 * D), 0, st, c, r, k, v,
+    hipLaunchKernelGGL((k_kv4_read<T, D>), dim3((r.rows + 31) / 32, c.heads, 2), dim3(32 * D * sizeof(T) / 16), 0, st, c, r, k, v,
                        (uint32_t)(on16<T>(k) && on16<T>(v)));
     return hipGetLastError();
   });
 }
 
-// Pieces of the slots: enough workgroups to fill the chip a few times over,
-// of at least a tile a wave.
-void kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live, uint32_t* nsplit,
-               uint32_t* tps) {
+// Pieces of the slots at most: enough workgroups to fill the chip a few times
+// over (a CU holds two to four), each sequence's tiles cut evenly by the
+// kernels, which know their number.
+uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live) {
   const uint64_t slots = live ? std::min<uint64_t>(live, c.slots) : c.slots;
   const uint32_t tiles = (uint32_t)((slots + 31) / 32);
   const uint64_t G = hq / c.heads;
   const uint64_t base = ragged ? ((uint64_t)rows * G + 127) / 128 * c.heads : (uint64_t)n * c.heads * ((G + 15) / 16);
-  const uint64_t want = ragged ? 512 : 1024;
-  uint32_t s = (uint32_t)std::min<uint64_t>((want + base - 1) / std::max<uint64_t>(base, 1), 128);
-  s = std::max(1u, std::min(s, tiles / 4));
-  *tps = (std::max(tiles, 1u) + s - 1) / s;
-  if (ragged) *tps = (*tps + 1) & ~1u;
-  *nsplit = (std::max(tiles, 1u) + *tps - 1) / *tps;
+  const uint64_t want = ragged ? 768 : 1024;
+  const uint64_t s = ragged ? want / std::max<uint64_t>(base, 1) : (want + base - 1) / std::max<uint64_t>(base, 1);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({s, 128, tiles / (ragged ? kManyTiles : kFewTiles)}));
 }
 
 hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {
-  if (!a.c.data || !a.r.pos || a.c.slots == 0 || a.c.heads == 0 || a.hq == 0 || a.hq % a.c.heads || a.tps == 0 ||
-      a.nsplit == 0 || a.nsplit > 65535 || (a.nsplit > 1 && !a.part))
+  if (!a.c.data || !a.r.pos || a.c.slots == 0 || a.c.heads == 0 || a.hq == 0 || a.hq % a.c.heads || a.nsplit == 0 || a.nsplit > 65535 || (a.nsplit > 1 && !a.part))
     return hipErrorInvalidValue;
   if (a.r.rows == 0 || a.r.n == 0) return hipSuccess;
   return by_type(type, a.c.hd, [&](auto t, auto d) -> hipError_t {
@@ -1214,7 +1230,7 @@ hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {
     if (a.r.off) {
       constexpr uint32_t PW = Many<T, D>::pairs;
       const uint32_t gx = (uint32_t)(((uint64_t)a.r.rows * G + PW - 1) / PW) + a.r.n;
-      hipLaunchKernelGGL((k_kv4_many<T, D>), dim3(gx, a.c.heads, a.nsplit), dim3(256), 0, st, a, vec);
+      hipLaunchKernelGGL((k_kv4_many<T, D>), dim3(gx * a.c.heads, a.nsplit), dim3(256), 0, st, a, vec);
     }
     if (a.nsplit > 1)
       hipLaunchKernelGGL((k_kv4_join<T, D>), dim3((uint32_t)(((uint64_t)a.r.rows * a.hq + 3) / 4)), dim3(256), 0, st, a);

@@ -38,34 +38,29 @@ def _check(r: int) -> None:
         raise AnaError(r, lib().ana_error(None).decode())
 
 
-def _device(t: torch.Tensor, name: str) -> int:
-    if not t.is_cuda:
-        raise ValueError(f"{name} is not on a GPU")
-    return t.device.index
+# the device's current stream as a number (torch.cuda.current_stream makes an
+# object of it first: 1.1 us of a call's 12 against 0.1)
+_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _stream(device: int) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-def _ints(t, n: int, device: int, name: str):
+def _ints(t, n: int, device: torch.device, name: str):
     """A device array of whole numbers: int32, consecutive, n of them."""
     if t is None:
         return None
-    if t.dtype != torch.int32 or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name}: a consecutive int32 tensor of {n}, not {tuple(t.shape)} {t.dtype}")
-    if t.device.index != device or not t.is_cuda:
-        raise ValueError(f"{name} is on {t.device}, not on GPU {device}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
     return t.data_ptr()
 
 
-def _mat(t: torch.Tensor, rows: int, heads: int, hd: int, dtype, device: int, name: str) -> _Mat:
-    if t.dim() != 3 or tuple(t.shape) != (rows, heads, hd) or t.dtype != dtype:
-        raise ValueError(f"{name}: {(rows, heads, hd)} {dtype}, not {tuple(t.shape)} {t.dtype}")
-    if not t.is_cuda or t.device.index != device:
-        raise ValueError(f"{name} is on {t.device}, not on GPU {device}")
+def _mat(t: torch.Tensor, shape: tuple, dtype, device: torch.device, name: str) -> _Mat:
+    if t.shape != shape or t.dtype is not dtype:
+        raise ValueError(f"{name}: {shape} {dtype}, not {tuple(t.shape)} {t.dtype}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, not on {device}")
     a, b, c = t.stride()
-    if c != 1 and hd > 1:
+    if c != 1:
         raise ValueError(f"{name}: the last axis is not consecutive")
     return _Mat(t.data_ptr(), a, b)
 
@@ -84,8 +79,11 @@ class KV4:
             raise ValueError(f"KV4: {tuple(data.shape)} is not a cache of {slots} slots")
         self.data, self.slots = data, slots
         self.seqs, self.heads, self.hd = s, h, r // 34
-        self.device = _device(data, "KV4")
-        self._c = _Kv4(data.data_ptr(), self.device, s, slots, h, r // 34)
+        if not data.is_cuda:
+            raise ValueError("KV4 is not on a GPU")
+        self.device = data.device
+        self._c = _Kv4(data.data_ptr(), self.device.index, s, slots, h, r // 34)
+        self._p = C.addressof(self._c)
 
     @classmethod
     def empty(cls, seqs: int, slots: int, heads: int, hd: int, device="cuda") -> "KV4":
@@ -95,21 +93,20 @@ class KV4:
 
 
 def _rows(cache: KV4, rows: int, pos, seq, off) -> _Rows:
-    n = pos.numel()
-    return _Rows(n, rows, _ints(seq, n, cache.device, "seq"), _ints(pos, n, cache.device, "pos"),
-                 _ints(off, n + 1, cache.device, "off"))
+    n, dev = pos.numel(), cache.device
+    return _Rows(n, rows, _ints(seq, n, dev, "seq"), _ints(pos, n, dev, "pos"), _ints(off, n + 1, dev, "off"))
 
 
 def kv4_write(cache: KV4, k: torch.Tensor, v: torch.Tensor, pos: torch.Tensor, seq=None, off=None) -> None:
     """Keys and values [rows, heads, hd] into the cache: sequence i (its
     place seq[i], or i) at positions pos[i] and on, its rows off[i] ..
     off[i + 1] - 1 (or row i alone). ana_kv4_write."""
-    rows = k.shape[0]
+    rows, dev, dtype = k.shape[0], cache.device, k.dtype
     r = _rows(cache, rows, pos, seq, off)
-    km = _mat(k, rows, cache.heads, cache.hd, k.dtype, cache.device, "k")
-    vm = _mat(v, rows, cache.heads, cache.hd, k.dtype, cache.device, "v")
-    _check(lib().ana_kv4_write(C.byref(cache._c), C.byref(r), _TYPES.get(k.dtype, -1), C.byref(km), C.byref(vm),
-                               _stream(cache.device)))
+    shape = (rows, cache.heads, cache.hd)
+    km, vm = _mat(k, shape, dtype, dev, "k"), _mat(v, shape, dtype, dev, "v")
+    _check(lib().ana_kv4_write(cache._p, C.byref(r), _TYPES.get(dtype, -1), C.byref(km), C.byref(vm),
+                               _stream(dev.index)))
 
 
 def kv4_read(cache: KV4, pos: torch.Tensor, rows: int, seq=None, off=None, dtype=torch.float32):
@@ -117,12 +114,12 @@ def kv4_read(cache: KV4, pos: torch.Tensor, rows: int, seq=None, off=None, dtype
     [rows, heads, hd]. Rows that no sequence has are left unset.
     ana_kv4_read."""
     r = _rows(cache, rows, pos, seq, off)
-    k = torch.empty((rows, cache.heads, cache.hd), dtype=dtype, device=cache.data.device)
+    h, hd, dev = cache.heads, cache.hd, cache.device
+    k = torch.empty((rows, h, hd), dtype=dtype, device=dev)
     v = torch.empty_like(k)
-    km = _mat(k, rows, cache.heads, cache.hd, dtype, cache.device, "k")
-    vm = _mat(v, rows, cache.heads, cache.hd, dtype, cache.device, "v")
-    _check(lib().ana_kv4_read(C.byref(cache._c), C.byref(r), _TYPES.get(dtype, -1), C.byref(km), C.byref(vm),
-                              _stream(cache.device)))
+    km, vm = _Mat(k.data_ptr(), h * hd, hd), _Mat(v.data_ptr(), h * hd, hd)
+    _check(lib().ana_kv4_read(cache._p, C.byref(r), _TYPES.get(dtype, -1), C.byref(km), C.byref(vm),
+                              _stream(dev.index)))
     return k, v
 
 
@@ -135,22 +132,26 @@ def kv4_attend(q: torch.Tensor, cache: KV4, pos: torch.Tensor, seq=None, off=Non
     it to be fewer than the ring's (only the split of the work depends on
     it); out: where the outputs go (rows that no sequence has stay as they
     are there). ana_kv4_attend."""
-    rows, hq = q.shape[0], q.shape[1]
+    rows, hq, hd = q.shape
+    dev, dtype = cache.device, q.dtype
     r = _rows(cache, rows, pos, seq, off)
-    qm = _mat(q, rows, hq, cache.hd, q.dtype, cache.device, "q")
+    shape = (rows, hq, cache.hd)
+    qm = _mat(q, shape, dtype, dev, "q")
     if out is None:
-        out = torch.empty((rows, hq, cache.hd), dtype=q.dtype, device=q.device)
-    om = _mat(out, rows, hq, cache.hd, q.dtype, cache.device, "out")
-    if sink is not None and (sink.dtype != torch.float32 or sink.shape != (hq,) or not sink.is_contiguous()
-                             or not sink.is_cuda or sink.device.index != cache.device):
-        raise ValueError(f"sink: a consecutive float32 tensor of {hq} on GPU {cache.device}")
-    L = lib()
-    nb = L.ana_kv4_attend_ws(C.byref(cache._c), C.byref(r), hq, live)
-    ws = torch.empty(nb, dtype=torch.uint8, device=q.device) if nb else None
-    _check(L.ana_kv4_attend(C.byref(cache._c), C.byref(r), _TYPES.get(q.dtype, -1), C.byref(qm), hq,
+        out = torch.empty(shape, dtype=dtype, device=dev)
+        om = _Mat(out.data_ptr(), hq * hd, hd)
+    else:
+        om = _mat(out, shape, dtype, dev, "out")
+    if sink is not None and (sink.dtype is not torch.float32 or sink.shape != (hq,) or not sink.is_contiguous()
+                             or sink.device != dev):
+        raise ValueError(f"sink: a consecutive float32 tensor of {hq} on {dev}")
+    L, rp = lib(), C.byref(r)
+    nb = L.ana_kv4_attend_ws(cache._p, rp, hq, live)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    _check(L.ana_kv4_attend(cache._p, rp, _TYPES.get(dtype, -1), C.byref(qm), hq,
                             cache.hd ** -0.5 if scale is None else scale,
                             None if sink is None else sink.data_ptr(), C.byref(om), live,
-                            None if ws is None else ws.data_ptr(), nb, _stream(cache.device)))
+                            None if ws is None else ws.data_ptr(), nb, _stream(dev.index)))
     return out
 
 
@@ -163,22 +164,23 @@ def logprobs(logits: torch.Tensor, tokens=None, top: int = 0):
     it, -1 for a token outside the vocabulary. ana_row_logprobs."""
     if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("logprobs: rows of logits, each consecutive")
-    device = _device(logits, "logits")
+    if not logits.is_cuda:
+        raise ValueError("logits is not on a GPU")
     n, vocab = logits.shape
-    ids = _ints(tokens, n, device, "tokens")
-    new = dict(device=logits.device)
-    ent = torch.empty(n, dtype=torch.float32, **new)
-    lp = rank = None
-    if tokens is not None:
-        lp = torch.empty(n, dtype=torch.float32, **new)
-        rank = torch.empty(n, dtype=torch.int32, **new)
-    ids_top = torch.empty((n, top), dtype=torch.int32, **new)
-    lp_top = torch.empty((n, top), dtype=torch.float32, **new)
+    dev = logits.device
+    ids = _ints(tokens, n, dev, "tokens")
     L = lib()
     nb = L.ana_row_logprobs_ws(n, vocab, top)
-    ws = torch.empty(nb, dtype=torch.uint8, **new) if nb else None
-    _check(L.ana_row_logprobs(device, _TYPES.get(logits.dtype, -1), logits.data_ptr(), logits.stride(0), n, vocab, ids,
-                              top, None if lp is None else lp.data_ptr(), ent.data_ptr(),
-                              None if rank is None else rank.data_ptr(), ids_top.data_ptr(), lp_top.data_ptr(),
-                              None if ws is None else ws.data_ptr(), nb, _stream(device)))
-    return lp, ent, rank, ids_top, lp_top
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    # the float results and the whole numbers, an allocation each, cut into
+    # the tensors that are returned
+    g = tokens is not None
+    f = torch.empty(n * (1 + g + top), dtype=torch.float32, device=dev)
+    i = torch.empty(n * (g + top), dtype=torch.int32, device=dev)
+    fp, ip = f.data_ptr(), i.data_ptr()
+    _check(L.ana_row_logprobs(dev.index, _TYPES.get(logits.dtype, -1), logits.data_ptr(), logits.stride(0), n, vocab,
+                              ids, top, fp + 4 * n if g else None, fp, ip if g else None, ip + 4 * n * g,
+                              fp + 4 * n * (1 + g), None if ws is None else ws.data_ptr(), nb, _stream(dev.index)))
+    ent, lp, tlp = f.split_with_sizes((n, n * g, n * top))
+    rank, ids = i.split_with_sizes((n * g, n * top))
+    return lp if g else None, ent, rank if g else None, ids.view(n, top), tlp.view(n, top)
