@@ -503,6 +503,18 @@ __device__ __forceinline__ uint32_t nan_blocks(const uint8_t* rec, uint32_t tile
   }
   return n;
 }
+// which of a lane's eight slots have a key that is not finite (some block of
+// it), a bit each
+template <int D>
+__device__ __forceinline__ uint32_t nan_keys(const uint8_t* rec, uint32_t j) {
+  uint32_t n = 0;
+#pragma unroll 1
+  for (uint32_t i = 0; i < 8 * (D / 32); i++) {
+    const uint32_t e = i % 8, b = i / 8;
+    n |= rec[32 * D + (b * 16 + 4 * j + e % 4) * 2 + e / 4] == 255 ? 1u << e : 0u;
+  }
+  return n;
+}
 // the value scales of slots that are not live, and of blocks that are not
 // finite, as 2^-127
 __device__ __forceinline__ void quiet_values(uint32_t (&vs)[2], uint32_t tile, uint32_t live, uint32_t j) {
@@ -514,11 +526,11 @@ __device__ __forceinline__ void quiet_values(uint32_t (&vs)[2], uint32_t tile, u
 }
 template <int D>
 __device__ __forceinline__ bool not_finite(const Raw<D>& r) {
-  return has255(r.ks) | has255(r.vs[0]) | has255(r.vs[1]);
-}
-__device__ __forceinline__ bf16x8_t nan_op() {
-  const u32x4_t n = {0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u};
-  return __builtin_bit_cast(bf16x8_t, n);
+  // (by the scales as they are used: fewer instructions than by the bytes)
+  uint32_t t = max(__builtin_bit_cast(uint32_t, scale_of(r.ks, 0)), __builtin_bit_cast(uint32_t, scale_of(r.ks, 1)));
+#pragma unroll
+  for (int e = 0; e < 8; e++) t = max(t, __builtin_bit_cast(uint32_t, scale_of(r.vs[e / 4], e % 4)));
+  return t == 0x7F800000u;
 }
 
 // u's DPP move within its quad of lanes
@@ -543,7 +555,7 @@ __device__ __forceinline__ uint32_t quad(float f) { return quad<CTRL>(__builtin_
 // costs 320 vector instructions and 24 MFMAs with NC = 1, where the vector
 // units were busy 87% of 128 us.)
 template <typename T, int D, int NC>
-__global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint32_t ncol) {
+__global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few(Kv4Attend a, uint32_t vec, uint32_t ncol) {
   constexpr int NP = Parts<T>::q, QP = NC == 1 ? NP : 1, NPP = NC == 1 ? Parts<T>::p : 1;
   constexpr int PC = 16 / NC;          // pairs a workgroup
   constexpr int OWN = NC == 1 ? 4 : 4 / NC;  // slots of four that a lane takes exponentials of
@@ -619,15 +631,14 @@ __global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint
   auto tile_of = [&](Raw<D>& r, uint32_t tile) {
     const bool whole = view.whole(tile, len - 1);
     const bool bad = __any(not_finite(r));
-    f32x4_t s[2];
+    f32x4_t s[2];   // (a key that is not finite makes its own slot's score anything)
 #pragma unroll
     for (int h = 0; h < 2; h++) {
       s[h] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
       const float ksc = scale_of(r.ks, h);
 #pragma unroll
       for (int d = 0; d < D / 32; d++) {
-        bf16x8_t ko = key_op<D>(r, h, d, ksc);
-        if (bad && ((r.ks >> (8 * h)) & 0xFF) == 255) ko = nan_op();
+        const bf16x8_t ko = key_op<D>(r, h, d, ksc);
 #pragma unroll
         for (int n = 0; n < QP; n++) s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ko, qo[n][d], s[h], 0, 0, 0);
       }
@@ -657,9 +668,11 @@ __global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint
       }
     }
     if (!whole || bad) {
+      const uint32_t nk = bad ? nan_keys<D>(base + (uint64_t)tile * (34 * D), j) : 0;
 #pragma unroll
       for (int e = 0; e < 2 * OWN; e++) {
         const uint32_t in4 = NC == 1 ? e % 4 : NC == 2 ? 2 * (e % 2) + part : part;
+        if ((nk >> (4 * (e / OWN) + in4)) & 1) x[e] = __builtin_nanf("");
         if (!view.sees(tile * 32 + 16 * (e / OWN) + 4 * j + in4, ago)) x[e] = -INFINITY;
       }
       if (bad) nan |= nan_blocks<D>(base + (uint64_t)tile * (34 * D), tile, view, ago, j);
@@ -790,20 +803,23 @@ __global__ __launch_bounds__(256) void k_kv4_few(Kv4Attend a, uint32_t vec, uint
 // read and write there is a lane's own 16 bytes; the next tile's record is
 // loaded a tile ahead, and two sets of operands leave one barrier a tile. The
 // vector units (softmax and parts) and the matrix cores bind about equally,
-// so what counts is that a SIMD holds three such waves of different
-// workgroups to overlap them. bf16 outputs take a probability rounded once to
+// so what counts is that a SIMD holds three or four such waves, of different
+// workgroups, to overlap them (16 pairs a wave, not 32, for f32: 61 -> 55 us
+// for 16 prompts of 12 heads of 64). bf16 outputs take a probability rounded once to
 // bf16, and the denominator the sum of the rounded ones (a second part was 8
 // of 24 MFMAs a tile and 16 pairs at hd 128).
 template <typename T, int D>
 struct Many {
   // pairs a wave: the queries' parts and the outputs share its registers
-  static constexpr int NQ = D == 128 && Parts<T>::q > 1 ? 1 : 2;
+  static constexpr int NQ = Parts<T>::q > 1 ? 1 : 2;
+  // waves a SIMD that the registers are kept to
+  static constexpr int waves = D == 128 ? 3 : 4;
   static constexpr int NPP = Parts<T>::q == 1 ? 1 : Parts<T>::p;
   static constexpr uint32_t pairs = 64 * NQ;
 };
 
 template <typename T, int D>
-__global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) {
+__global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend a, uint32_t vec) {
   constexpr int NP = Parts<T>::q, NPP = Many<T, D>::NPP, NQ = Many<T, D>::NQ;
   constexpr uint32_t PW = Many<T, D>::pairs;
   constexpr int KS = D / 32, OPS = D / 16;     // steps of a key operand, operands of a tile's keys (values)
@@ -893,9 +909,7 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
       for (int d = 0; d < KS; d++) {
         const uint32_t w0 = rw[d], w1 = rw[KS + d], w = half ? w1 : w0;
         const u32x4_t o = {two_of<0>(w, ksc), two_of<1>(w, ksc), two_of<2>(w, ksc), two_of<3>(w, ksc)};
-        bf16x8_t ko = __builtin_bit_cast(bf16x8_t, o);
-        if (bad && b8 == 255) ko = nan_op();
-        ops[buf][0][half * KS + d][lane] = ko;
+        ops[buf][0][half * KS + d][lane] = __builtin_bit_cast(bf16x8_t, o);
       }
     } else {
       bad = __any(has255(rs[0]) | has255(rs[1]));
@@ -950,7 +964,7 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
     // (past every position of the wave's pairs: nothing to do)
     if (!flat || tile * 32 <= wave_hi) {
       const bool whole = view.whole(tile, len - 1 - t_lo);
-      const bool bad = flag[buf][2] | flag[buf][3];
+      const bool bad_k = flag[buf][0] | flag[buf][1], bad = flag[buf][2] | flag[buf][3];
       // (f32 scores come out less their pair's maximum: the products start from it)
       f32x4_t s[NQ][2];
 #pragma unroll
@@ -974,6 +988,14 @@ __global__ __launch_bounds__(256, 3) void k_kv4_many(Kv4Attend a, uint32_t vec) 
       for (int n = 0; n < NQ; n++)
 #pragma unroll
         for (int e = 0; e < 8; e++) x[n][e] = s[n][e / 4][e % 4];
+      if (bad_k) {
+        // (such a key has made its own slot's scores anything)
+        const uint32_t nk = nan_keys<D>(base + (uint64_t)tile * (34 * D), j);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+#pragma unroll
+          for (int n = 0; n < NQ; n++) x[n][e] = (nk >> e) & 1 ? __builtin_nanf("") : x[n][e];
+      }
       if (!whole) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
