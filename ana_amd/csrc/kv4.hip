@@ -1220,17 +1220,18 @@ hipError_t launch_kv4_read(const Kv4& c, const Kv4Rows& r, int type, const Kv4Ma
   });
 }
 
-// Pieces of the slots at most: enough workgroups to fill the chip a few times
-// over (a CU holds two to four), each sequence's tiles cut evenly by the
-// kernels, which know their number.
+// Pieces of the slots at most: as many as keep to three workgroups a CU, each
+// sequence's tiles cut evenly by the kernels, which know their number (64
+// sequences of 12 heads, ragged to 2048 slots: 17 us whole, 24 in two pieces
+// with the join; two pieces of 1024 rows over 30000 positions, 252
+// workgroups whole: 1050 us, in two 642, in three 537).
 uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live) {
   const uint64_t slots = live ? std::min<uint64_t>(live, c.slots) : c.slots;
   const uint32_t tiles = (uint32_t)((slots + 31) / 32);
   const uint64_t G = hq / c.heads;
   const uint64_t base = ragged ? ((uint64_t)rows * G + 127) / 128 * c.heads : (uint64_t)n * c.heads * ((G + 15) / 16);
-  const uint64_t want = ragged ? 768 : 1024;
-  const uint64_t s = ragged ? want / std::max<uint64_t>(base, 1) : (want + base - 1) / std::max<uint64_t>(base, 1);
-  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({s, 128, tiles / (ragged ? kManyTiles : kFewTiles)}));
+  return (uint32_t)std::max<uint64_t>(
+      1, std::min<uint64_t>({768 / std::max<uint64_t>(base, 1), 128, tiles / (ragged ? kManyTiles : kFewTiles)}));
 }
 
 hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {
