@@ -30,6 +30,7 @@ namespace {
 
 typedef unsigned long long u64;
 
+constexpr uint32_t kJoinKeys = 2048;   // keys that a row's join takes into LDS
 constexpr uint32_t kHead = 8;   // a piece's words before its keys: m, c, l, w, rank
 
 // a logit's order as a whole number: larger for larger ones, -0 as +0, 0 for NaN
@@ -44,13 +45,23 @@ __device__ __forceinline__ float value_of(uint32_t o) {
 }
 __device__ __forceinline__ u64 key_of(float x, uint32_t i) { return (u64)order_of(x) << 32 | (0xFFFFFFFFu - i); }
 
+// the largest over the wave by DPP moves, as wmax's
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, ROWS, 0xF, false);
+}
+__device__ __forceinline__ uint32_t wave_max32(uint32_t v) {
+  v = max(v, dpp_u<0xB1, 0xF>(v));
+  v = max(v, dpp_u<0x4E, 0xF>(v));
+  v = max(v, dpp_u<0x141, 0xF>(v));
+  v = max(v, dpp_u<0x140, 0xF>(v));
+  v = max(v, dpp_u<0x142, 0xA>(v));
+  v = max(v, dpp_u<0x143, 0xC>(v));
+  return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
 __device__ __forceinline__ u64 wave_max64(u64 v) {
-#pragma unroll
-  for (int k = 32; k >= 1; k >>= 1) {
-    const u64 o = __shfl_xor(v, k, 64);
-    v = o > v ? o : v;
-  }
-  return v;
+  const uint32_t hi = wave_max32((uint32_t)(v >> 32));
+  return (u64)hi << 32 | wave_max32((uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
 }
 
 // the larger of two, NaN if either is
@@ -311,9 +322,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
 }
 
 // A row's pieces, a wave a row and a lane a piece: the sums brought to the
-// row's maximum, and k rounds of a maximum over the pieces' next keys.
+// row's maximum, and k rounds of a maximum over the pieces' next keys (from
+// LDS where they fit: read in turn from memory, eight rounds over five pieces
+// took 10 us for 3000 rows).
 template <typename T>
 __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S) {
+  extern __shared__ u64 keys[];   // [S][k], where they are at most kJoinKeys
   const uint32_t r = blockIdx.x, lane = threadIdx.x, k = a.top;
   const uint32_t* p = a.part + ((uint64_t)r * S + lane) * (kHead + 2 * k);
   const bool in = lane < S;
@@ -354,8 +368,18 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
     }
   }
   uint32_t at_i = 0;
+  const bool staged = S * k <= kJoinKeys;
+  if (staged) {
+    const uint32_t* row = a.part + (uint64_t)r * S * (kHead + 2 * k) + kHead;
+    for (uint32_t i = lane; i < S * k; i += 64) {
+      const uint32_t* q2 = row + (uint64_t)(i / k) * (kHead + 2 * k) + 2 * (i % k);
+      keys[i] = (u64)q2[1] << 32 | q2[0];
+    }
+    __syncthreads();
+  }
   auto next = [&]() -> u64 {
-    return in && at_i < k ? (u64)p[kHead + 2 * at_i + 1] << 32 | p[kHead + 2 * at_i] : 0ull;
+    if (!in || at_i >= k) return 0ull;
+    return staged ? keys[lane * k + at_i] : (u64)p[kHead + 2 * at_i + 1] << 32 | p[kHead + 2 * at_i];
   };
   u64 mine = k ? next() : 0;
   for (uint32_t i = 0; i < k; i++) {
@@ -369,21 +393,35 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
   }
 }
 
-// How a row is cut: whole rows of up to 32768 logits (one launch; 512 rows
-// of 32768 f32 logits take 20 us whole and 30 in pieces of 8192 with the
-// join, one row 8 and 10), longer ones in pieces of 8192, of which a CU holds
-// eight (3000 rows of 50021 bf16 logits: 110 us, and 126 in two pieces of
-// 1024 threads), or of 32768 where those would be too many for one wave to
-// join.
+// How a row is cut. Whole rows of up to 32768 logits in one launch of 1024
+// threads (512 rows of 32768 f32 logits take 20 us so, 30 in pieces of 8192
+// with the join). Longer ones in pieces of 256 threads, of which a CU holds
+// eight: each thread has up to eight vectors, and the pieces are as many as
+// leave the fewest places empty (3000 rows of 50021 bf16 logits: 104 us in
+// seven pieces of 3.5 vectors a thread, 98 in five of 4.9). Pieces of 32768
+// where those would be too many for one wave to join.
 struct Plan {
   uint32_t C, S;
-  bool wide;   // 1024 threads and up to 32768 logits a workgroup, else 256 and 8192
+  bool wide;   // 1024 threads and up to 32768 logits a workgroup, else 256
 };
-Plan plan_of(uint32_t vocab) {
+// (es: an element's bytes)
+Plan plan_of(uint32_t vocab, uint32_t es) {
+  const uint32_t step = 256 * 16 / es, cap = 8 * step;   // logits of a vector a thread, of eight
   Plan p;
-  p.wide = (vocab > 8192 && vocab <= 32768) || vocab > 64 * 8192;
-  const uint32_t cap = p.wide ? 32768u : 8192u;
-  p.S = (vocab + cap - 1) / cap;
+  p.wide = (vocab > cap && vocab <= 32768) || vocab > 64 * cap;
+  const uint32_t most = p.wide ? 32768u : cap;
+  p.S = (vocab + most - 1) / most;
+  if (!p.wide && p.S > 1) {
+    // a piece's own work is about that of half a vector a thread
+    uint32_t best = ~0u;
+    for (uint32_t s = p.S, n = p.S; s <= std::min(2 * n, 64u); s++) {
+      const uint32_t cost = s * (2 * ((vocab + s * step - 1) / (s * step)) + 1);
+      if (cost < best) {
+        best = cost;
+        p.S = s;
+      }
+    }
+  }
   p.C = ((vocab + p.S - 1) / p.S + 7) & ~7u;
   p.S = (vocab + p.C - 1) / p.C;
   return p;
@@ -392,15 +430,16 @@ Plan plan_of(uint32_t vocab) {
 }  // namespace
 
 uint64_t logprobs_part_words(uint32_t n, uint32_t vocab, uint32_t top) {
-  const Plan p = plan_of(vocab);
-  return p.S > 1 ? (uint64_t)n * p.S * (kHead + 2 * top) : 0;
+  // (for either size of element)
+  const uint32_t S = std::max(plan_of(vocab, 2).S, plan_of(vocab, 4).S);
+  return S > 1 ? (uint64_t)n * S * (kHead + 2 * top) : 0;
 }
 
 hipError_t launch_logprobs(const LogprobArgs& a, int type, hipStream_t st) {
   if (!a.logits || a.vocab == 0 || a.vocab > kLpMaxVocab || a.top > kLpMaxTop || a.top > a.vocab || a.ld < a.vocab || !a.ent)
     return hipErrorInvalidValue;
   if (a.n == 0) return hipSuccess;
-  const Plan p = plan_of(a.vocab);
+  const Plan p = plan_of(a.vocab, type == ET_F32 ? 4 : 2);
   if ((p.S > 1 && !a.part) || (uint64_t)a.n * p.S > 0x7FFFFFFFull) return hipErrorInvalidValue;
   auto go = [&](auto t) -> hipError_t {
     using T = decltype(t);
@@ -409,8 +448,10 @@ hipError_t launch_logprobs(const LogprobArgs& a, int type, hipStream_t st) {
     if (p.wide)
       hipLaunchKernelGGL((k_logprobs<T, 1024, 32 / W>), g, dim3(1024), 0, st, a, p.C, p.S);
     else
-      hipLaunchKernelGGL((k_logprobs<T, 256, 32 / W>), g, dim3(256), 0, st, a, p.C, p.S);
-    if (p.S > 1) hipLaunchKernelGGL((k_logprobs_join<T>), dim3(a.n), dim3(64), 0, st, a, p.S);
+      hipLaunchKernelGGL((k_logprobs<T, 256, 8>), g, dim3(256), 0, st, a, p.C, p.S);
+    const uint32_t keys = p.S * a.top;
+    if (p.S > 1)
+      hipLaunchKernelGGL((k_logprobs_join<T>), dim3(a.n), dim3(64), keys <= kJoinKeys ? keys * 8 : 0, st, a, p.S);
     return hipGetLastError();
   };
   switch (type) {
