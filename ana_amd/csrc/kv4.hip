@@ -73,6 +73,11 @@ __device__ __forceinline__ uint32_t find_seq(const uint32_t* off, uint32_t n, ui
   return lo;
 }
 
+// whether a sequence has a place in the cache, and positions below 2^31 (so
+// that none of its rows' passes 2^32)
+__device__ __forceinline__ bool has_place(const Kv4& c, uint32_t q, uint32_t pos) {
+  return q < c.seqs && pos < 0x80000000u;
+}
 // where a row is: its sequence's index in the call, place in the cache,
 // position, and the last position of its sequence in the call
 struct RowAt {
@@ -95,10 +100,11 @@ __device__ __forceinline__ RowAt row_at(const Kv4& c, const Kv4Rows& r, uint32_t
     a.on = row < r.n;
   }
   if (!a.on) return a;
+  const uint32_t pos = r.pos[a.i];
   a.q = r.seq ? r.seq[a.i] : a.i;
-  a.ok = a.q < c.seqs;
-  a.p = r.pos[a.i] + (row - o0);
-  a.last = r.pos[a.i] + (o1 - 1 - o0);
+  a.ok = has_place(c, a.q, pos);
+  a.p = pos + (row - o0);
+  a.last = pos + (o1 - 1 - o0);
   return a;
 }
 
@@ -447,16 +453,17 @@ __device__ __forceinline__ uint32_t piece_tiles(uint32_t tiles, uint32_t nsplit,
 constexpr float kSlack = 10.0f;
 
 // The queries' scale: f32 queries carry it (times log2 e) into their parts,
-// 16-bit ones enter as they are and only take its sign.
+// 16-bit ones enter as they are and only take its sign
+// (or, for a scale of 0, that).
 template <typename T>
 __device__ __forceinline__ float query_factor(float sc) {
   if constexpr (sizeof(T) == 4) return sc;
-  return sc < 0.0f ? -1.0f : 1.0f;
+  return sc < 0.0f ? -1.0f : sc == 0.0f ? 0.0f : 1.0f;
 }
 template <typename T>
 __device__ __forceinline__ float score_factor(float sc) {
   if constexpr (sizeof(T) == 4) return 1.0f;
-  return fabsf(sc);
+  return sc == 0.0f ? 1.0f : fabsf(sc);   // (a masked score of -inf must stay one)
 }
 // the query operand of a pair: dims j D / 4 + 8 s + e of its row, in parts
 template <typename T, int D, int NP>
@@ -577,9 +584,9 @@ __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few
     if (len > kFewPairs || len * G > kFewPairs) return;
   }
   const uint32_t q = a.r.seq ? a.r.seq[i] : i;
-  const uint32_t last = a.r.pos[i] + len - 1;
+  const uint32_t pos = a.r.pos[i], last = pos + len - 1;
   const uint32_t c0 = sub * PC, np = min(len * G - c0, (uint32_t)PC);   // the pairs here
-  const bool ok = q < a.c.seqs;
+  const bool ok = has_place(a.c, q, pos);
   const View view(last, a.c.slots);
   const uint32_t tiles = ok ? (view.live + 31) / 32 : 0u;
   const uint32_t per = piece_tiles(tiles, a.nsplit, kFewTiles);
@@ -867,8 +874,8 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
   part_i = __builtin_amdgcn_readfirstlane(part_i);
   const uint32_t row0 = a.r.off[i], len = a.r.off[i + 1] - row0;
   const uint32_t q = a.r.seq ? a.r.seq[i] : i;
-  const bool ok = q < a.c.seqs;
   const uint32_t pos = a.r.pos[i], last = pos + len - 1;
+  const bool ok = has_place(a.c, q, pos);
   const uint32_t all = len * G, c0 = part_i * PW;   // (rows x query heads < 2^31)
   const View view(last, a.c.slots);
   const uint32_t t_lo = c0 / G, t_hi = (min(all, c0 + PW) - 1) / G;

@@ -134,7 +134,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
   // f(value, index) over the thread's share of the piece, read again: the
   // rare paths, which would take the common ones' registers
   auto each = [&](auto&& f) {
-#pragma unroll 1
+#pragma unroll 4
     for (uint32_t i = tid; i < cnt; i += NT) f((float)p[i], e0 + i);
   };
 

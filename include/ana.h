@@ -347,10 +347,11 @@ typedef struct {
 } ana_kv4;
 
 /* The rows of a call, in device memory: sequence i of n has its place
- * seq[i] in the cache (seq NULL: i; a place outside 0 .. seqs - 1 is none:
- * nothing is stored for it, and its outputs are zeros) and rows off[i] ..
- * off[i + 1] - 1 of the tensors, at positions pos[i] and on (off NULL: row i
- * alone, rows == n). off does not go down, and ends at `rows` at most; rows
+ * seq[i] in the cache (seq NULL: i) and rows off[i] .. off[i + 1] - 1 of the
+ * tensors, at positions pos[i] and on (off NULL: row i alone, rows == n). A
+ * place outside 0 .. seqs - 1, or a first position outside 0 .. 2^31 - 1, is
+ * none (-1 in a padded batch): nothing is stored for the sequence, and its
+ * outputs are zeros. off does not go down, and ends at `rows` at most; rows
  * before off[0] and from off[n] on are not read, and their outputs are left
  * as they were. */
 typedef struct {

@@ -278,6 +278,12 @@ def test_attend_score_sizes(ops):
     q, q64 = rand(rs, (60, 2, 64), "f32", 30.0)
     for scale in (2.0, -0.3, 0.0):
         check_attend(ops, cache, q, q64, "f32", [10], None, [0, 60], [-50.0, 200.0], scale=scale)
+    for typ in ("bf16", "f16"):
+        for scale in (2.0, -0.3, 0.0):
+            q, q64 = rand(rs, (2, 2, 64), typ, 3.0)
+            check_attend(ops, cache, q, q64, typ, [199, 77], None, None, None, scale=scale)
+            q, q64 = rand(rs, (60, 2, 64), typ, 3.0)
+            check_attend(ops, cache, q, q64, typ, [10], None, [0, 60], [0.5, -2.0], scale=scale)
 
 
 @pytest.mark.parametrize("typ", ["f32", "bf16"])
@@ -355,6 +361,32 @@ def test_attend_rows_and_places_outside(ops):
     # the same sequence read twice
     twice = ops.kv4_attend(q[:2], cache, dev([9, 9]), seq=dev([1, 1]))
     assert torch.equal(twice[1:], ops.kv4_attend(q[1:2], cache, dev([9]), seq=dev([1])))
+
+
+def test_positions_below_zero_are_no_place(ops):
+    """A padded batch's rows at position -1 (and any other past 2^31 - 1):
+    nothing stored, zeros read and attended, also with rows that reach 0."""
+    rs = np.random.RandomState(15)
+    cache = filled(ops, rs, 3, 100, 1, 64)
+    before = cache.data.clone()
+    k, _ = rand(rs, (45, 1, 64), "f32")
+    off, pos = dev([0, 20, 25, 45]), dev([-5, -1, -2 ** 31])
+    ops.kv4_write(cache, k, k, pos, off=off)
+    ops.kv4_write(cache, k[:3], k[:3], pos)
+    assert torch.equal(cache.data, before)
+    a, b = ops.kv4_read(cache, pos, 45, off=off)
+    assert not a.any() and not b.any()
+    for typ in TYPES.values():
+        q = k.expand(45, 2, 64).to(typ).contiguous()
+        assert not ops.kv4_attend(q, cache, pos, off=off).any()
+        assert not ops.kv4_attend(q[:3], cache, pos).any()
+    # the largest position there is
+    far = dev([2 ** 31 - 1])
+    ops.kv4_write(cache, k[:1], k[:1], far, seq=dev([1]))
+    x, _ = ops.kv4_read(cache, far, 1, seq=dev([1]))
+    c, s = ref.quant(k[:1].double().cpu().numpy())
+    assert np.array_equal(x.double().cpu().numpy(), ref.values(c, s))
+    assert ops.kv4_attend(k[:1], cache, far, seq=dev([1])).isfinite().all()
 
 
 def test_attend_many_sequences(ops):
