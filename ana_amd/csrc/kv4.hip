@@ -170,7 +170,7 @@ __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k,
   const float f = __builtin_bit_cast(float, (254u - min(b, 252u)) << 23);
   // (to the nearest code, ties to the even one, past the largest to it; the
   // same in integer steps took 14 instructions a value where this takes 1.5,
-  // and 32 us where it takes 24 for 16384 rows of 8 heads of 128 in bf16)
+  // and 32 us where it takes 28 for 16384 rows of 8 heads of 128 in bf16)
   uint32_t w = 0;
   static_for<4>([&](auto u) {
     constexpr int e = 2 * decltype(u)::value;
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k,
 // (zeros for a sequence without a place in the cache). A thread takes 16
 // bytes of the outputs, so that a store's lanes write whole lines (with eight
 // f32 a thread, in two stores of every other 16 bytes, 8384 rows of 12 heads
-// of 64 took 37 us).
+// of 64 took 37 us for 20).
 template <typename T, int D>
 __global__ __launch_bounds__(32 * D * sizeof(T) / 16) void k_kv4_read(Kv4 c, Kv4Rows r, Kv4Mat k, Kv4Mat v, uint32_t vec) {
   constexpr uint32_t E = 16 / sizeof(T), TPR = D / E;   // outputs a thread, threads a row
@@ -559,8 +559,8 @@ __device__ __forceinline__ uint32_t quad(float f) { return quad<CTRL>(__builtin_
 // second, one MFMA each where NC = 1 takes one a part. A lane of the NC then
 // has exponentials to take for only 8 / NC of its slots, which its neighbours
 // get by DPP moves. (256 sequences of 2048 slots, 12 heads of 64, f32: a tile
-// costs 320 vector instructions and 24 MFMAs with NC = 1, where the vector
-// units were busy 87% of 128 us.)
+// costs 188 vector instructions and 8 MFMAs, 80 us or 5.3 TB/s with the vector
+// units busy 82% of it; with NC = 1 it was 296 and 24, 128 us.)
 template <typename T, int D, int NC>
 __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few(Kv4Attend a, uint32_t vec, uint32_t ncol) {
   constexpr int NP = Parts<T>::q, QP = NC == 1 ? NP : 1, NPP = NC == 1 ? Parts<T>::p : 1;
