@@ -2,6 +2,8 @@
 // device they run on, and the launches of kv4.hip and logprobs.hip.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
+
 #include "ana_internal.h"
 #include "kv4.h"
 #include "logprobs.h"
@@ -54,17 +56,24 @@ int check_rows(const char* fn, const ana_kv4* c, const ana_kv4_rows* r, Kv4Rows*
     return fail_call(ANA_EINVAL, "%s: %u rows of %u sequences without offsets", fn, r->rows, r->n);
   if (!r->seq && r->n > c->seqs)
     return fail_call(ANA_EINVAL, "%s: %u sequences in a cache of %u", fn, r->n, c->seqs);
-  if (r->rows > 0x7FFFFFFFu || r->n > 0x7FFFFFFFu) return fail_call(ANA_EINVAL, "%s: more than 2^31 - 1 rows", fn);
+  if (r->rows > kKv4MaxRows || r->n > kKv4MaxRows) return fail_call(ANA_EINVAL, "%s: more than 2^26 rows or sequences", fn);
   *o = Kv4Rows{r->seq, r->pos, r->off, r->n, r->rows};
   return ANA_OK;
 }
 
+// (out: no two rows' heads may share elements)
 int check_mat(const char* fn, const char* name, const ana_mat* x, int type, const ana_kv4_rows* r, uint32_t heads,
-              uint32_t hd, Kv4Mat* o) {
+              uint32_t hd, bool out, Kv4Mat* o) {
   if (!x || (!x->p && r->rows)) return fail_call(ANA_EINVAL, "%s: null %s", fn, name);
   if ((uintptr_t)x->p % size_of(type)) return fail_call(ANA_EINVAL, "%s: %s is not on an element's border", fn, name);
   if ((r->rows > 1 && x->row < hd) || (heads > 1 && x->head < hd))
     return fail_call(ANA_EINVAL, "%s: rows or heads of %s overlap", fn, name);
+  if (out && r->rows > 1 && heads > 1) {
+    const bool by_row = x->row >= x->head;   // (whole heads of a row, or whole rows of a head, lie together)
+    const uint64_t in = by_row ? x->head : x->row, cnt = by_row ? heads : r->rows;
+    if (in > (UINT64_MAX - hd) / cnt || std::max(x->row, x->head) < (cnt - 1) * in + hd)
+      return fail_call(ANA_EINVAL, "%s: rows and heads of %s overlap", fn, name);
+  }
   *o = Kv4Mat{x->p, x->row, x->head};
   return ANA_OK;
 }
@@ -95,8 +104,8 @@ extern "C" int ana_kv4_write(const ana_kv4* c, const ana_kv4_rows* r, int type, 
   if (int e = check_cache(fn, c, &kc)) return e;
   if (int e = check_rows(fn, c, r, &kr)) return e;
   if (int e = check_type(fn, type)) return e;
-  if (int e = check_mat(fn, "k", k, type, r, c->heads, c->hd, &km)) return e;
-  if (int e = check_mat(fn, "v", v, type, r, c->heads, c->hd, &vm)) return e;
+  if (int e = check_mat(fn, "k", k, type, r, c->heads, c->hd, false, &km)) return e;
+  if (int e = check_mat(fn, "v", v, type, r, c->heads, c->hd, false, &vm)) return e;
   if (r->n == 0 || r->rows == 0) return ANA_OK;
   OnDevice on(c->device);
   if (on.e != hipSuccess) return launched(fn, on.e);
@@ -112,8 +121,8 @@ extern "C" int ana_kv4_read(const ana_kv4* c, const ana_kv4_rows* r, int type, c
   if (int e = check_cache(fn, c, &kc)) return e;
   if (int e = check_rows(fn, c, r, &kr)) return e;
   if (int e = check_type(fn, type)) return e;
-  if (int e = check_mat(fn, "k", k, type, r, c->heads, c->hd, &km)) return e;
-  if (int e = check_mat(fn, "v", v, type, r, c->heads, c->hd, &vm)) return e;
+  if (int e = check_mat(fn, "k", k, type, r, c->heads, c->hd, true, &km)) return e;
+  if (int e = check_mat(fn, "v", v, type, r, c->heads, c->hd, true, &vm)) return e;
   if (r->n == 0 || r->rows == 0) return ANA_OK;
   OnDevice on(c->device);
   if (on.e != hipSuccess) return launched(fn, on.e);
@@ -122,9 +131,9 @@ extern "C" int ana_kv4_read(const ana_kv4* c, const ana_kv4_rows* r, int type, c
 
 static int check_heads(const char* fn, const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq) {
   if (hq == 0 || hq % c->heads) return fail_call(ANA_EINVAL, "%s: %u query heads over %u key heads", fn, hq, c->heads);
-  // (the launches' grids, and the pairs of a sequence)
-  if ((uint64_t)r->rows * hq > 0x7FFFFFFFull || (uint64_t)r->n * hq > 0x7FFFFFFFull)
-    return fail_call(ANA_EINVAL, "%s: more than 2^31 - 1 rows of query heads", fn);
+  // (the pairs of a sequence are counted in 32 bits)
+  if ((uint64_t)r->rows * hq > 0x7FFFFFFFull || kv4_attend_groups(c->heads, r->n, r->rows, r->off != nullptr, hq) > kKv4MaxGroups)
+    return fail_call(ANA_EINVAL, "%s: %u rows of %u query heads are more than a launch takes", fn, r->rows, hq);
   return ANA_OK;
 }
 
@@ -144,8 +153,8 @@ extern "C" int ana_kv4_attend(const ana_kv4* c, const ana_kv4_rows* r, int type,
   if (int e = check_rows(fn, c, r, &a.r)) return e;
   if (int e = check_type(fn, type)) return e;
   if (int e = check_heads(fn, c, r, hq)) return e;
-  if (int e = check_mat(fn, "q", q, type, r, hq, c->hd, &a.q)) return e;
-  if (int e = check_mat(fn, "o", o, type, r, hq, c->hd, &a.o)) return e;
+  if (int e = check_mat(fn, "q", q, type, r, hq, c->hd, false, &a.q)) return e;
+  if (int e = check_mat(fn, "o", o, type, r, hq, c->hd, true, &a.o)) return e;
   if (r->n == 0 || r->rows == 0) return ANA_OK;
   a.nsplit = kv4_split(a.c, r->n, r->rows, r->off != nullptr, hq, live);
   const uint64_t need = 4 * kv4_part_floats(r->rows, hq, c->hd, a.nsplit);
@@ -178,7 +187,8 @@ extern "C" int ana_row_logprobs(int device, int type, const void* logits, uint64
   if (n == 0) return ANA_OK;
   if (!logits || !ent || (tok && (!lp || !rank)) || (top && (!top_tok || !top_lp))) return fail_call(ANA_EINVAL, "%s: null argument", fn);
   if ((uintptr_t)logits % size_of(type)) return fail_call(ANA_EINVAL, "%s: the logits are not on an element's border", fn);
-  if ((uint64_t)n * 64 > 0x7FFFFFFFull) return fail_call(ANA_EINVAL, "%s: more than 2^25 - 1 rows", fn);
+  if (n > logprobs_max_rows(vocab))
+    return fail_call(ANA_EINVAL, "%s: %u rows (at most %u of %u logits)", fn, n, logprobs_max_rows(vocab), vocab);
   const uint64_t need = ana_row_logprobs_ws(n, vocab, top);
   if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 4))
     return fail_call(ANA_EINVAL, "%s: a workspace of %llu bytes, not %llu", fn, (unsigned long long)need,

@@ -40,6 +40,10 @@ struct Kv4Mat {
 
 enum ElemType : int { ET_F32 = 0, ET_BF16 = 1, ET_F16 = 2 };
 
+// A launch's threads along an axis are counted in 32 bits: the most rows (and
+// sequences) of a call, and workgroups of the attention.
+constexpr uint32_t kKv4MaxRows = 1u << 26, kKv4MaxGroups = (1u << 24) - 1;
+
 // the head sizes and element types that the kernels take
 inline bool kv4_fits(uint32_t hd) { return hd == 32 || hd == 64 || hd == 128; }
 
@@ -67,6 +71,8 @@ struct Kv4Attend {
 // the pieces of a call (live: the most positions a sequence holds after it,
 // as far as the caller knows; 0: the ring's slots), and the floats of
 // partials they take
+// (groups: the workgroups of its largest launch a piece, at most)
+uint64_t kv4_attend_groups(uint32_t heads, uint32_t n, uint32_t rows, bool ragged, uint32_t hq);
 uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live);
 inline uint64_t kv4_part_floats(uint32_t rows, uint32_t hq, uint32_t hd, uint32_t nsplit) {
   return nsplit > 1 ? (uint64_t)rows * hq * nsplit * (kKv4PartHead + hd) : 0;

@@ -1200,7 +1200,7 @@ hipError_t by_type(int type, uint32_t hd, F&& f) {
 
 hipError_t launch_kv4_write(const Kv4& c, const Kv4Rows& r, int type, const Kv4Mat& k, const Kv4Mat& v,
                             const float* gk, const float* gq, const Kv4Mat* q, uint32_t qheads, hipStream_t st) {
-  if (!c.data || !r.pos || c.slots == 0 || (q && type != ET_F32)) return hipErrorInvalidValue;
+  if (!c.data || !r.pos || c.slots == 0 || r.rows > kKv4MaxRows || (q && type != ET_F32)) return hipErrorInvalidValue;
   if (r.rows == 0 || r.n == 0) return hipSuccess;
   return by_type(type, c.hd, [&](auto t, auto d) -> hipError_t {
     using T = decltype(t);
@@ -1216,7 +1216,7 @@ hipError_t launch_kv4_write(const Kv4& c, const Kv4Rows& r, int type, const Kv4M
 
 hipError_t launch_kv4_read(const Kv4& c, const Kv4Rows& r, int type, const Kv4Mat& k, const Kv4Mat& v,
                            hipStream_t st) {
-  if (!c.data || !r.pos || c.slots == 0) return hipErrorInvalidValue;
+  if (!c.data || !r.pos || c.slots == 0 || r.rows > kKv4MaxRows) return hipErrorInvalidValue;
   if (r.rows == 0 || r.n == 0) return hipSuccess;
   return by_type(type, c.hd, [&](auto t, auto d) -> hipError_t {
     using T = decltype(t);
@@ -1225,6 +1225,12 @@ hipError_t launch_kv4_read(const Kv4& c, const Kv4Rows& r, int type, const Kv4Ma
                        (uint32_t)(on16<T>(k) && on16<T>(v)));
     return hipGetLastError();
   });
+}
+
+uint64_t kv4_attend_groups(uint32_t heads, uint32_t n, uint32_t rows, bool ragged, uint32_t hq) {
+  const uint64_t G = hq / heads;
+  if (!ragged) return (uint64_t)n * heads * ((G + 15) / 16);
+  return ((rows * G + 63) / 64 + n) * heads;   // (workgroups of 64 pairs or more)
 }
 
 // Pieces of the slots at most: as many as keep to three workgroups a CU, each
@@ -1244,6 +1250,7 @@ uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_
 hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {
   if (!a.c.data || !a.r.pos || a.c.slots == 0 || a.c.heads == 0 || a.hq == 0 || a.hq % a.c.heads || a.nsplit == 0 || a.nsplit > 65535 || (a.nsplit > 1 && !a.part))
     return hipErrorInvalidValue;
+  if (kv4_attend_groups(a.c.heads, a.r.n, a.r.rows, a.r.off != nullptr, a.hq) > kKv4MaxGroups) return hipErrorInvalidValue;
   if (a.r.rows == 0 || a.r.n == 0) return hipSuccess;
   return by_type(type, a.c.hd, [&](auto t, auto d) -> hipError_t {
     using T = decltype(t);

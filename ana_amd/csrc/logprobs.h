@@ -22,6 +22,8 @@ struct LogprobArgs {
 };
 // the words of workspace a call takes (0 for none)
 uint64_t logprobs_part_words(uint32_t n, uint32_t vocab, uint32_t top);
+// the most rows of a call (a launch's threads are counted in 32 bits)
+uint32_t logprobs_max_rows(uint32_t vocab);
 // (type: kv4.h's ElemType)
 hipError_t launch_logprobs(const LogprobArgs& a, int type, hipStream_t st);
 

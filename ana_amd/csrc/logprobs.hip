@@ -435,12 +435,21 @@ uint64_t logprobs_part_words(uint32_t n, uint32_t vocab, uint32_t top) {
   return S > 1 ? (uint64_t)n * S * (kHead + 2 * top) : 0;
 }
 
+uint32_t logprobs_max_rows(uint32_t vocab) {
+  uint64_t most = 0;   // threads a row, of either size of element
+  for (uint32_t es : {2u, 4u}) {
+    const Plan p = plan_of(vocab, es);
+    most = std::max<uint64_t>(most, p.S * (p.wide ? 1024u : 256u));
+  }
+  return (uint32_t)(0xFFFFFFFFull / most);
+}
+
 hipError_t launch_logprobs(const LogprobArgs& a, int type, hipStream_t st) {
   if (!a.logits || a.vocab == 0 || a.vocab > kLpMaxVocab || a.top > kLpMaxTop || a.top > a.vocab || a.ld < a.vocab || !a.ent)
     return hipErrorInvalidValue;
   if (a.n == 0) return hipSuccess;
   const Plan p = plan_of(a.vocab, type == ET_F32 ? 4 : 2);
-  if ((p.S > 1 && !a.part) || (uint64_t)a.n * p.S > 0x7FFFFFFFull) return hipErrorInvalidValue;
+  if ((p.S > 1 && !a.part) || a.n > logprobs_max_rows(a.vocab)) return hipErrorInvalidValue;
   auto go = [&](auto t) -> hipError_t {
     using T = decltype(t);
     constexpr int W = 16 / sizeof(T);

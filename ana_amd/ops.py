@@ -6,7 +6,7 @@ A ctypes mirror, as ana_amd itself is: every value is computed by libana.so.
 torch holds the tensors, allocates outputs and workspaces, and names the
 stream: the work is queued on the tensors' device's current stream, can be
 captured there, and is not waited for. Tensors of other streams are the
-caller's to order, as for any torch operation.
+caller's to order, as for any torch operation. The results have no gradient.
 """
 from __future__ import annotations
 
@@ -130,8 +130,8 @@ def kv4_attend(q: torch.Tensor, cache: KV4, pos: torch.Tensor, seq=None, off=Non
     its own that its ring holds. sink: float32 [hq]; scale: hd ** -0.5 unless
     given; live: the most positions a sequence holds, where the program knows
     it to be fewer than the ring's (only the split of the work depends on
-    it); out: where the outputs go (rows that no sequence has stay as they
-    are there). ana_kv4_attend."""
+    it); out: where the outputs go, q itself allowed (rows that no sequence has
+    stay as they are there). ana_kv4_attend."""
     rows, hq, hd = q.shape
     dev, dtype = cache.device, q.dtype
     r = _rows(cache, rows, pos, seq, off)

@@ -353,7 +353,7 @@ typedef struct {
  * none (-1 in a padded batch): nothing is stored for the sequence, and its
  * outputs are zeros. off does not go down, and ends at `rows` at most; rows
  * before off[0] and from off[n] on are not read, and their outputs are left
- * as they were. */
+ * as they were. Up to 2^26 rows and sequences. */
 typedef struct {
   uint32_t n, rows;
   const uint32_t *seq, *pos, *off;
@@ -389,8 +389,11 @@ int ana_kv4_read(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_ma
  * probabilities to 2^-16, bf16 ones of a sequence with more than 16 query
  * rows a key head rounded to bf16. `live`, where not 0, is the most positions a
  * sequence holds after the call, as far as the caller knows: it only
- * chooses how the work is split. ws: ana_kv4_attend_ws bytes of workspace
- * for the same arguments, on a 16-byte border. */
+ * chooses how the work is split. o may be q itself (the same address and
+ * strides). ws: ana_kv4_attend_ws bytes of workspace for the same arguments,
+ * on a 16-byte border. Up to 2^31 - 1 rows times hq, and with G = hq / heads
+ * fewer than 2^24 of n heads ceil(G / 16), or with off of
+ * (ceil(rows G / 64) + n) heads. */
 int ana_kv4_attend(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_mat* q, uint32_t hq, float scale,
                    const float* sink, const ana_mat* o, uint64_t live, void* ws, uint64_t ws_bytes, void* stream);
 uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq, uint64_t live);
@@ -405,7 +408,8 @@ uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq,
  * probabilities. A logit of -inf has probability 0; in a row with nothing
  * else every log probability is -inf and the entropy 0. NaN comes after
  * every number in the order; a NaN or +inf in a row makes its log
- * probabilities and entropy NaN. Sums are f32. vocab up to 2^21. ws:
+ * probabilities and entropy NaN. Sums are f32. vocab up to 2^21; up to
+ * 2^22 - 1 rows of 32768 logits (2^16 - 1 of the longest). ws:
  * ana_row_logprobs_ws bytes, on a 4-byte border. */
 int ana_row_logprobs(int device, int type, const void* logits, uint64_t ld, uint32_t n, uint32_t vocab,
                      const uint32_t* tok, uint32_t top, float* lp, float* ent, uint32_t* rank, uint32_t* top_tok,

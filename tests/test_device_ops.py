@@ -53,7 +53,8 @@ BAD_CACHES = [(None, "null cache"), (cache(data=None), "null cache"), (cache(hd=
               (cache(slots=0xFFFFFFFF), "slots"), (cache(data=A + 8), "16-byte"),
               (cache(seqs=1 << 31, slots=1 << 30, heads=60000), "beyond any memory")]
 BAD_ROWS = [(None, "null rows"), (rows(pos=None), "null positions"), (rows(rows=3), "without offsets"),
-            (rows(n=3, rows=3, seq=None), "in a cache of 2"), (rows(rows=1 << 31, off=A), "2^31")]
+            (rows(n=3, rows=3, seq=None), "in a cache of 2"), (rows(rows=1 << 31, off=A), "2^26"),
+            (rows(n=(1 << 26) + 1, rows=0, off=A), "2^26")]
 
 
 @pytest.mark.parametrize("c,why", BAD_CACHES)
@@ -86,8 +87,11 @@ def test_refuses_heads_and_workspaces():
     for hq in (0, 3, 5):
         rc, msg = attend(cache(), rows(), mat(), mat(), hq=hq)
         assert rc == ana_amd.ANA_EINVAL and "query heads" in msg
-    rc, msg = attend(cache(), rows(n=1 << 20, rows=1 << 30, off=A), mat(row=256), mat(row=256))
-    assert rc == ana_amd.ANA_EINVAL and "2^31" in msg
+    # 2^31 pairs; 2^24 workgroups of single rows; of ragged ones
+    for c, r, hq in ((cache(), rows(n=1 << 20, rows=1 << 26, off=A), 32), (cache(), rows(n=1 << 23, rows=1 << 23), 2),
+                     (cache(), rows(n=1 << 23, rows=9, off=A), 2)):
+        rc, msg = attend(c, r, mat(row=64 * hq), mat(row=64 * hq), hq=hq)
+        assert rc == ana_amd.ANA_EINVAL and "than a launch takes" in msg
     long = cache(slots=1 << 20)
     need = ana_amd.lib().ana_kv4_attend_ws(C.byref(long), C.byref(rows()), 4, 0)
     assert need > 0 and need % (2 * 4 * 16) == 0
@@ -96,6 +100,19 @@ def test_refuses_heads_and_workspaces():
         assert rc == ana_amd.ANA_EINVAL and "workspace" in msg
     # a known length needs no more of it than the ring
     assert ana_amd.lib().ana_kv4_attend_ws(C.byref(long), C.byref(rows()), 4, 40) == 0
+
+
+@pytest.mark.parametrize("m", [mat(row=64, head=64), mat(row=127, head=64), mat(row=64, head=127),
+                               mat(row=1 << 63, head=1 << 63)])
+def test_refuses_outputs_that_overlap(m):
+    """Strides that are wide enough one by one, not together."""
+    L = ana_amd.lib()
+    c, r, ok = cache(), rows(), mat()
+    for k, v in ((m, ok), (ok, m)):
+        rc = L.ana_kv4_read(C.byref(c), C.byref(r), 0, C.byref(k), C.byref(v), None)
+        assert rc == ana_amd.ANA_EINVAL and "overlap" in L.ana_error(None).decode()
+    rc, msg = attend(c, r, ok, m, hq=2)
+    assert rc == ana_amd.ANA_EINVAL and "overlap" in msg
 
 
 def test_empty_calls_touch_nothing():
@@ -124,7 +141,7 @@ def logprobs(**kw):
     (dict(top=65), "alternatives"), (dict(vocab=5, top=6), "alternatives"), (dict(ld=99), "overlap"),
     (dict(logits=None), "null"), (dict(ent=None), "null"), (dict(lp=None), "null"), (dict(rank=None), "null"),
     (dict(top_tok=None), "null"), (dict(top_lp=None), "null"), (dict(logits=A + 2), "border"),
-    (dict(n=1 << 26), "2^25"), (dict(vocab=40000, ld=40000, ws=None), "workspace"),
+    (dict(n=1 << 24), "at most 16777215"), (dict(vocab=9000, ld=9000, n=1 << 22), "at most 4194303"), (dict(vocab=40000, ld=40000, ws=None), "workspace"),
     (dict(vocab=40000, ld=40000, nws=8), "workspace")])
 def test_refuses_logprobs(kw, why):
     rc, msg = logprobs(**kw)

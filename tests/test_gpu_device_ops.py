@@ -389,6 +389,20 @@ def test_positions_below_zero_are_no_place(ops):
     assert ops.kv4_attend(k[:1], cache, far, seq=dev([1])).isfinite().all()
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("slots,hq,off", [
+    (300, 2, None), (300, 40, None), (9000, 6, None),              # single rows: few heads, many, in pieces
+    (300, 6, [0, 1, 90, 101]), (9000, 6, [0, 3, 40, 200])])        # few and many rows, heads that split a part's rows
+def test_attend_in_place(ops, typ, slots, hq, off):
+    rs = np.random.RandomState(21)
+    cache = filled(ops, rs, 3, slots, 2, 64)
+    q, _ = rand(rs, (3 if off is None else off[-1], hq, 64), typ)
+    pos, o = dev([slots - 220, 5, slots // 2]), None if off is None else dev(off)
+    want = ops.kv4_attend(q, cache, pos, off=o)
+    assert ops.kv4_attend(q, cache, pos, off=o, out=q) is q
+    assert torch.equal(q, want)
+
+
 def test_attend_many_sequences(ops):
     """More sequences than a wave has lanes, ragged, some empty."""
     rs = np.random.RandomState(11)
