@@ -13,8 +13,11 @@
 // after every number), so an order key (value bits, ~index) is unique. The
 // k-th largest of 64 group maxima is a bound that at least k logits reach and
 // few more do; those go to LDS, where each counts the keys above its own.
-// Where ties (or rows of few numbers) make them too many, or too few, k
-// rounds of a maximum over the registers find the same.
+// Where ties, or k near 64, make them too many, or rows of few numbers too
+// few, a bisection over the keys finds a bound first (500 rows of 50021 bf16
+// logits, 64 alternatives: 74 us, 280 by 64 rounds of a maximum; 256 group
+// maxima take 48 there, but with the registers of their code 3000 rows with
+// eight alternatives take 95 for 89).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -31,6 +34,7 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr uint32_t kJoinKeys = 2048;   // keys that a row's join takes into LDS
+constexpr uint32_t kJoinRank = 256;    // of them, those that it ranks by counting
 constexpr uint32_t kHead = 8;   // a piece's words before its keys: m, c, l, w, rank
 
 // a logit's order as a whole number: larger for larger ones, -0 as +0, 0 for NaN
@@ -99,10 +103,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
   __shared__ float tmax[NW][64];
   __shared__ __align__(16) float gmax[64];
   __shared__ float red[NW][3];
-  __shared__ uint32_t redu[NW];
+  __shared__ uint32_t redu[NW], reach_s[NW];
   __shared__ float bound_s;
   __shared__ uint32_t ncand;
-  __shared__ u64 cand[CAP], best[kLpMaxTop], wred[NW];
+  __shared__ u64 cand[CAP], best[kLpMaxTop];
   const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
   const uint32_t r = blockIdx.x / S, z = blockIdx.x % S;
   const T* row = (const T*)a.logits + (uint64_t)r * a.ld;
@@ -134,8 +138,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
   // f(value, index) over the thread's share of the piece, read again: the
   // rare paths, which would take the common ones' registers
   auto each = [&](auto&& f) {
+    uint32_t i = tid;
+    asm volatile("" : "+v"(i));   // (nor their addresses' registers)
 #pragma unroll 4
-    for (uint32_t i = tid; i < cnt; i += NT) f((float)p[i], e0 + i);
+    for (; i < cnt; i += NT) f((float)p[i], e0 + i);
   };
 
   float m = fmaxf(xe, -INFINITY);
@@ -153,8 +159,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
 #pragma unroll
   for (int i = 1; i < NW; i++) gm = fmaxf(gm, tmax[i][lane]);
   m = wmax(gm);
+  // the k-th largest group maximum: the least that fewer than k are above
   if (wv == NW - 1 && k) {
-    // the k-th largest group maximum: the least that fewer than k are above
     gmax[lane] = gm;
     __builtin_amdgcn_wave_barrier();
     uint32_t above = 0;
@@ -254,31 +260,60 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
       nc = ncand;
     }
     if (tid < k && tid >= want) best[tid] = 0;
-    if (nc <= CAP && nc >= want) {
-      for (uint32_t i = tid; i < nc; i += NT) {
-        const u64 mine = cand[i];
-        uint32_t over = 0;
-        for (uint32_t o = 0; o < nc; o++) over += cand[o] > mine ? 1u : 0u;
-        if (over < k) best[over] = mine;
-      }
-    } else {
-      u64 last = ~0ull;
-      for (uint32_t i = 0; i < want; i++) {
-        u64 t = 0;
-        each([&](float v, uint32_t at) {
-          const u64 q = key_of(v, at);
-          if (q < last && q > t) t = q;
-        });
-        t = wave_max64(t);
-        __syncthreads();
-        if (lane == 0) wred[wv] = t;
-        __syncthreads();
-        t = wred[0];
+    if (nc > CAP || nc < want) {
+      // a key that `want` to CAP of the piece's reach: more than CAP reach lo,
+      // fewer than want hi
+      auto reach = [&](u64 t) {
+        uint32_t n = 0;
+        each([&](float v, uint32_t at) { n += key_of(v, at) >= t; });
 #pragma unroll
-        for (int o = 1; o < NW; o++) t = wred[o] > t ? wred[o] : t;
-        if (tid == 0) best[i] = t;
-        last = t;
+        for (int mk = 32; mk >= 1; mk >>= 1) n += __shfl_xor(n, mk, 64);
+        __syncthreads();
+        if (lane == 0) reach_s[wv] = n;
+        __syncthreads();
+        n = 0;
+#pragma unroll
+        for (int o = 0; o < NW; o++) n += reach_s[o];
+        return n;
+      };
+      // (without a bound: all of a short piece, or the numbers above -inf, or
+      // -inf with them)
+      constexpr u64 finite = 0x00800000ull << 32;   // (above every key of -inf)
+      const bool few = nc < want;
+      u64 lo = 0, hi = ((u64)order_of(m) + 1) << 32, t = few ? finite : (u64)order_of(bound) << 32;
+      if (few && cnt <= CAP) {
+        t = 0;
+        nc = cnt;
       }
+      for (uint32_t n = 0; nc > CAP || nc < want; n++) {
+        if (few || n) nc = reach(t);
+        if (nc <= CAP && nc >= want) break;
+        if (nc > CAP) lo = t;
+        else hi = t;
+        if (few && n == 0 && nc < want) {
+          t = finite - (1ull << 32);
+          continue;
+        }
+        if (lo >> 32 == (hi - 1) >> 32) {   // one value: only the piece's places are left
+          const u64 o = lo >> 32 << 32;
+          lo = max(lo, o | (0xFFFFFFFFu - (e0 + cnt - 1)));
+          hi = min(hi, (o | (0xFFFFFFFFu - e0)) + 1);
+        }
+        t = lo + (hi - lo) / 2;
+      }
+      if (tid == 0) ncand = 0;
+      __syncthreads();
+      each([&](float v, uint32_t at) {
+        const u64 q = key_of(v, at);
+        if (q >= t) cand[atomicAdd(&ncand, 1u)] = q;
+      });
+      __syncthreads();
+    }
+    for (uint32_t i = tid; i < nc; i += NT) {
+      const u64 mine = cand[i];
+      uint32_t over = 0;
+      for (uint32_t o = 0; o < nc; o++) over += cand[o] > mine ? 1u : 0u;
+      if (over < k) best[over] = mine;
     }
     __syncthreads();
   }
@@ -322,9 +357,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(8))) void k_
 }
 
 // A row's pieces, a wave a row and a lane a piece: the sums brought to the
-// row's maximum, and k rounds of a maximum over the pieces' next keys (from
-// LDS where they fit: read in turn from memory, eight rounds over five pieces
-// took 10 us for 3000 rows).
+// row's maximum, and the alternatives out of the pieces' sorted keys: those
+// that reach a bound, ranked in LDS, or, where LDS does not hold the lists or
+// too many reach it, k rounds of a maximum over the lists' next ones (one row
+// of 50021 logits, 20 alternatives: 12 us with the pieces, 17 by rounds).
 template <typename T>
 __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S) {
   extern __shared__ u64 keys[];   // [S][k], where they are at most kJoinKeys
@@ -344,15 +380,15 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
   const bool given = tk < a.vocab;
   const float xt = given ? (float)((const T*)a.logits + (uint64_t)r * a.ld)[tk] : 0.0f;
   RowSums t{wmax(q.m), 0.0f, 0.0f, 0.0f};
-  // e^(x - M) = f e^(x - m), (x - M) = (x - m) + d; a piece below the
+  // e^(x - M) = f e^(x - m), (x - M) = (x - m) + dm; a piece below the
   // maximum has no entry at it
-  const float d = fmaxf(q.m - t.m, -200.0f);
+  const float dm = fmaxf(q.m - t.m, -200.0f);
   const bool at = q.m == t.m, none = q.m == -INFINITY;
-  const float f = none ? 0.0f : __expf(d);   // (a NaN in l stays one)
+  const float f = none ? 0.0f : __expf(dm);   // (a NaN in l stays one)
   float s[3];
   s[0] = at ? q.c : 0.0f;
   s[1] = at ? q.l : f * (q.c + q.l);
-  s[2] = at ? q.w : f * (q.w + d * (q.c + q.l));
+  s[2] = at ? q.w : f * (q.w + dm * (q.c + q.l));
   wsum_n(s);
   t.c = s[0];
   t.l = s[1];
@@ -367,16 +403,50 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
       a.rank[r] = given ? rk : 0xFFFFFFFFu;
     }
   }
-  uint32_t at_i = 0;
+  auto pick = [&](u64 key, uint32_t i) {
+    a.top_tok[(uint64_t)r * k + i] = 0xFFFFFFFFu - (uint32_t)key;
+    a.top_lp[(uint64_t)r * k + i] = t.lp(value_of((uint32_t)(key >> 32)), ls);
+  };
   const bool staged = S * k <= kJoinKeys;
-  if (staged) {
+  if (staged && k) {
     const uint32_t* row = a.part + (uint64_t)r * S * (kHead + 2 * k) + kHead;
     for (uint32_t i = lane; i < S * k; i += 64) {
       const uint32_t* q2 = row + (uint64_t)(i / k) * (kHead + 2 * k) + 2 * (i % k);
       keys[i] = (u64)q2[1] << 32 | q2[0];
     }
     __syncthreads();
+    // Of the pieces' d-th keys the m-th largest is one that m d of them reach,
+    // k at least; m about three quarters of the pieces makes it a close one (a piece of
+    // fewer keys has zeros behind them)
+    const uint32_t d = (4 * k + 3 * S - 1) / (3 * S), m = (k + d - 1) / d;
+    const u64 own = in ? keys[lane * k + d - 1] : 0;
+    uint32_t above = 0;
+    for (uint32_t o = 0; o < S; o++) above += keys[o * k + d - 1] > own ? 1u : 0u;
+    const u64 bound = max(1ull, ~wave_max64(in && above < m ? ~own : 0ull));
+    uint32_t nc = 0;
+    for (uint32_t i = lane; i - lane < S * k; i += 64) nc += __popcll(__ballot(i < S * k && keys[i] >= bound));
+    if (nc <= kJoinRank) {
+      // those move to the front (never past what was read), and each counts
+      // the ones above it
+      nc = 0;
+      for (uint32_t i = lane; i - lane < S * k; i += 64) {
+        const u64 q2 = i < S * k ? keys[i] : 0;
+        const unsigned long long on = __ballot(q2 >= bound);
+        if (q2 >= bound) keys[nc + __popcll(on & ((1ull << lane) - 1))] = q2;
+        nc += __popcll(on);
+        __syncthreads();
+      }
+      for (uint32_t i = lane; i < nc; i += 64) {
+        const u64 mine = keys[i];
+        uint32_t over = 0;
+#pragma unroll 4
+        for (uint32_t o = 0; o < nc; o++) over += keys[o] > mine ? 1u : 0u;
+        if (over < k) pick(mine, over);
+      }
+      return;
+    }
   }
+  uint32_t at_i = 0;
   auto next = [&]() -> u64 {
     if (!in || at_i >= k) return 0ull;
     return staged ? keys[lane * k + at_i] : (u64)p[kHead + 2 * at_i + 1] << 32 | p[kHead + 2 * at_i];
@@ -385,8 +455,7 @@ __global__ __launch_bounds__(64) void k_logprobs_join(LogprobArgs a, uint32_t S)
   for (uint32_t i = 0; i < k; i++) {
     const u64 b = wave_max64(mine);
     if (mine == b) {
-      a.top_tok[(uint64_t)r * k + i] = 0xFFFFFFFFu - (uint32_t)b;
-      a.top_lp[(uint64_t)r * k + i] = t.lp(value_of((uint32_t)(b >> 32)), ls);
+      pick(b, i);
       at_i++;
       mine = next();
     }

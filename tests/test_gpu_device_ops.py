@@ -585,6 +585,46 @@ def test_logprobs_special_rows(ops, vocab, n):
     assert abs(float(lp[7]) - w[0]) <= 1e-4 * abs(w[0]) and abs(float(ent[7]) - w[1]) <= 1e-4 * w[1]
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab,top", [(40007, 64), (40007, 20), (40007, 1), (70001, 25), (300011, 64), (600001, 64)])
+def test_logprobs_pieces_of_ties_and_masks(ops, typ, vocab, top):
+    """Rows in pieces whose alternatives no bound separates: ties, masks, NaN,
+    sorted rows, all of the largest in one piece."""
+    rs = np.random.RandomState(23)
+    x = rs.standard_normal((11, vocab)).astype(np.float32)
+    x[0] = -0.25                                              # all equal
+    x[1] = np.arange(vocab) / 4096.0                          # rising
+    x[2] = -np.arange(vocab) / 4096.0                         # falling
+    x[3] = -math.inf
+    x[3, rs.choice(vocab, 10, replace=False)] = rs.standard_normal(10)
+    x[4] = -math.inf
+    x[4, rs.choice(vocab, 700, replace=False)] = rs.standard_normal(700)
+    x[5] = math.nan
+    x[5, rs.choice(vocab, 30, replace=False)] = rs.standard_normal(30)
+    x[6] = math.nan
+    at = rs.choice(vocab, 23, replace=False)
+    x[6, at[:20]], x[6, at[20:]] = -math.inf, [1.0, 2.0, 2.0]
+    x[7, 5000:5100] += 10
+    x[8] = np.where(rs.rand(vocab) < 0.5, 3.0, 2.0)
+    x[9] = math.nan
+    x[10] = -math.inf
+    t = torch.tensor(x).to(TYPES[typ]).cuda()
+    tok = np.concatenate([rs.randint(0, vocab, 7), [5050, vocab - 1, 17, vocab // 2]])
+    lp, ent, rank, ids, tlp = ops.logprobs(t, dev(tok), top)
+    e = 2.0 ** -24
+    x64 = t.double().cpu().numpy()
+    for r in range(11):
+        w = ref.logprobs(x64[r], int(tok[r]), top)
+        assert np.array_equal(ids[r].cpu().numpy(), w[3]) and int(rank[r]) == w[2], r
+        # each exponential as in check_logprobs; a thread's chain of at most
+        # 66 sums, then 6 + 4 over the workgroup and 6 + 4 in the join
+        tol = e * (2 * w[5] + 4 + 86)
+        got, want = np.append(tlp[r].double().cpu().numpy(), float(lp[r])), np.append(w[4], w[0])
+        fin = np.isfinite(want)
+        assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got == -math.inf, want == -math.inf), r
+        assert (np.abs(got[fin] - want[fin]) <= tol + 3 * e * np.abs(want[fin])).all(), r
+
+
 def test_logprobs_token_outside_and_none(ops):
     x = torch.randn(4, 100, device="cuda")
     lp, ent, rank, ids, tlp = ops.logprobs(x, dev([100, -1, 99, 2 ** 31 - 1]), 0)
