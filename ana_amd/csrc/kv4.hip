@@ -119,8 +119,9 @@ __device__ __forceinline__ uint8_t* record_of(const Kv4& c, uint32_t q, uint32_t
 // largest magnitude comes from the quad of threads that share it, in the
 // floats' bits, where a block that is not finite shows itself too.
 // A row that a later one of the call overwrites (a ring shorter than the
-// call), and rows of a sequence that the call lists a second time, are left
-// out, so that what is stored does not depend on the order of the threads.
+// call), and rows of a sequence that the call lists a second time with a
+// place, are left out, so that what is stored does not depend on the order of
+// the threads.
 template <typename T, int D>
 __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k, Kv4Mat v, uint32_t vec,
                                                      const float* gk, const float* gq, Kv4Mat qm, uint32_t kh) {
@@ -154,7 +155,7 @@ __global__ __launch_bounds__(4 * D) void k_kv4_write(Kv4 c, Kv4Rows r, Kv4Mat k,
   if (r.seq && put) {
     uint32_t dup = 0;
     for (uint32_t j = sub; j < a.i; j += TPR)
-      if (r.seq[j] == a.q && (!r.off || r.off[j + 1] > r.off[j])) dup = 1;
+      if (r.seq[j] == a.q && has_place(c, a.q, r.pos[j]) && (!r.off || r.off[j + 1] > r.off[j])) dup = 1;
 #pragma unroll
     for (uint32_t mk = 1; mk < TPR; mk <<= 1) dup |= __shfl_xor(dup, mk, 64);
     put = !dup;

@@ -369,8 +369,9 @@ typedef struct {
 uint64_t ana_kv4_bytes(uint32_t seqs, uint32_t slots, uint32_t heads, uint32_t hd);
 
 /* Keys k and values v (of ANA_T_ type `type`) into the cache. Of a
- * sequence with more rows than slots only the last `slots` are stored; a
- * sequence that the call lists again (with rows) is stored the first time. */
+ * sequence with more rows than slots only the last `slots` are stored; of a
+ * sequence that the call lists again, the first listing that has rows and a
+ * place is. */
 int ana_kv4_write(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_mat* k, const ana_mat* v,
                   void* stream);
 

@@ -151,6 +151,32 @@ def test_write_twice_listed_and_placeless(ops):
     assert torch.equal(gk[2:5], gk[8:11])
 
 
+@pytest.mark.parametrize("typ", list(TYPES))
+@pytest.mark.parametrize("pos,seq,off,live", [
+    ([-1, 5], [0, 0], None, [1]),                                          # a padded entry ahead of the real one
+    ([-1, -9, 3, 4, 9], [2, 0, 2, 1, 2], None, [2, 3]),                    # then listed twice
+    ([-1, 5], [0, 0], [0, 1, 4], [1]),
+    ([-2 ** 31, 7, -40, 60, 0], [1, 1, 2, 2, 1], [1, 41, 44, 44, 50, 55], [1, 3])])
+def test_write_after_a_listing_without_a_place(ops, typ, pos, seq, off, live):
+    """A listing without a place (its first position below zero) takes
+    nothing from a later one of the same sequence: `live` is what is stored."""
+    rs = np.random.RandomState(16)
+    rows = len(pos) if off is None else off[-1]
+    k, k64 = rand(rs, (rows, 2, 64), typ)
+    v, v64 = rand(rs, (rows, 2, 64), typ)
+    cache = ops.KV4.empty(3, 70, 2, 64)
+    want = garbage(rs, cache)
+    args = dict(seq=dev(seq), off=None if off is None else dev(off))
+    ops.kv4_write(cache, k, v, dev(pos), **args)
+    (kc, ks), (vc, vs) = ref.quant(k64), ref.quant(v64)
+    for i in live:
+        r0, r1 = (i, i + 1) if off is None else (off[i], off[i + 1])
+        for r in range(r0, r1):
+            for h in range(2):
+                ref.put(want, seq[i], h, (pos[i] + r - r0) % 70, kc[r, h], ks[r, h], vc[r, h], vs[r, h])
+    assert np.array_equal(cache.data.cpu().numpy(), want)
+
+
 def test_strided_and_unaligned(ops):
     """q, k and v as views of one tensor, and views off every border."""
     rs = np.random.RandomState(3)
