@@ -456,10 +456,11 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
   }
   if (kv4) {
     // the partials of the largest call, of single rows or of a prefill step's
+    // (of one chunk: more have no more pieces)
     uint64_t most = 0;
     const Kv4 kc = kv4_of(c, 0);
     for (uint32_t r = 1; r <= c->rows; r++) {
-      most = std::max(most, kv4_part_floats(r, cf.heads, hd, kv4_split(kc, r, r, true, cf.heads, 0)));
+      most = std::max(most, kv4_part_floats(r, cf.heads, hd, kv4_split(kc, 1, r, true, cf.heads, 0)));
       if (r <= c->wb) most = std::max(most, kv4_part_floats(r, cf.heads, hd, kv4_split(kc, r, r, false, cf.heads, 0)));
     }
     if ((e = dalloc(&c->d_kpart, most)) != hipSuccess || (e = dalloc(&c->d_kseg, 3 * (uint64_t)c->seg_cap + 1)) != hipSuccess)

@@ -1235,17 +1235,21 @@ uint64_t kv4_attend_groups(uint32_t heads, uint32_t n, uint32_t rows, bool ragge
 }
 
 // Pieces of the slots at most: as many as keep to three workgroups a CU, each
-// sequence's tiles cut evenly by the kernels, which know their number (64
-// sequences of 12 heads, ragged to 2048 slots: 17 us whole, 24 in two pieces
-// with the join; two pieces of 1024 rows over 30000 positions, 252
-// workgroups whole: 1050 us, in two 642, in three 537).
+// sequence's tiles cut evenly by the kernels, which know its length (64 single
+// rows of 12 heads, ragged to 2048 slots: 15 us whole, 24 in two pieces with
+// the join; two pieces of 1024 rows over 30000 positions, 252 workgroups
+// whole: 1050 us, in two 642, in three 537). A ragged call has a workgroup for
+// each sequence and key head at least (64 sequences of four rows, 12 heads,
+// 1900 positions: 58 us in eight pieces, 31 whole), and one for every 128
+// pairs: f32 and f16 ones hold 64, but are as fast six a CU (1024 f32 rows
+// of 12 heads over 30000 positions: 296 us so, 375 where 64 are counted).
 uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_t hq, uint64_t live) {
   const uint64_t slots = live ? std::min<uint64_t>(live, c.slots) : c.slots;
   const uint32_t tiles = (uint32_t)((slots + 31) / 32);
   const uint64_t G = hq / c.heads;
-  const uint64_t base = ragged ? ((uint64_t)rows * G + 127) / 128 * c.heads : (uint64_t)n * c.heads * ((G + 15) / 16);
+  const uint64_t parts = ragged ? std::max<uint64_t>(std::min(n, rows), (rows * G + 127) / 128) : n * ((G + 15) / 16);
   return (uint32_t)std::max<uint64_t>(
-      1, std::min<uint64_t>({768 / std::max<uint64_t>(base, 1), 128, tiles / (ragged ? kManyTiles : kFewTiles)}));
+      1, std::min<uint64_t>({768 / std::max<uint64_t>(parts * c.heads, 1), 128, tiles / (ragged ? kManyTiles : kFewTiles)}));
 }
 
 hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {

@@ -115,6 +115,28 @@ def test_refuses_outputs_that_overlap(m):
     assert rc == ana_amd.ANA_EINVAL and "overlap" in msg
 
 
+@pytest.mark.parametrize("heads,hq,hd,slots", [(12, 12, 64, 2048), (24, 24, 64, 60000), (8, 32, 128, 131072), (1, 16, 32, 9000),
+                                               (3, 3, 64, 700), (1, 64, 128, 1 << 20)])
+@pytest.mark.parametrize("n", [1, 2, 7, 24, 64, 200, 5000])
+@pytest.mark.parametrize("each", [0, 1, 2, 4, 16, 100, 1000])
+def test_pieces_fill_the_chip_once(heads, hq, hd, slots, n, each):
+    """A call is cut into pieces only as far as three workgroups a CU: one for
+    each sequence and key head at least (0 rows each: single rows, without
+    offsets), and one for every 128 pairs. The workspace tells the pieces."""
+    c = cache(seqs=n, slots=slots, heads=heads, hd=hd)
+    r = rows(n=n, rows=n * max(each, 1), off=A if each else None)
+    ws = ana_amd.lib().ana_kv4_attend_ws(C.byref(c), C.byref(r), hq, 0)
+    one = 4 * n * max(each, 1) * hq * (4 + hd)
+    assert ws % one == 0
+    pieces = max(1, ws // one)
+    g = hq // heads
+    groups = heads * max(n * (1 if each else -(-g // 16)), n * each * g // 128)
+    assert pieces == 1 or pieces * groups <= 3 * 256
+    assert pieces <= max(1, -(-slots // 32) // (8 if each else 4))
+    # as many as that where the ring is long
+    assert pieces == 128 or pieces == max(1, -(-slots // 32) // (8 if each else 4)) or 2 * pieces * groups + 2 * groups > 3 * 256
+
+
 def test_empty_calls_touch_nothing():
     assert write(cache(), rows(n=0, rows=0), mat(), mat())[0] == 0
     assert attend(cache(), rows(n=0, rows=0), mat(row=256), mat(row=256))[0] == 0
