@@ -57,7 +57,7 @@ struct ana_ctx {
   uint64_t* d_rng = nullptr;
   unsigned long long* d_amax = nullptr;  // [wb] greedy argmax keys
   float *d_ss = nullptr, *d_pm = nullptr; // split attention scratch, ss_rows rows
-  uint32_t ss_rows = 1;
+  uint32_t ss_rows = 0;
   float* d_part = nullptr;           // fast attention's per-split partials
   size_t part_cap = 0;               // their floats
   float* SC = nullptr;               // scoring: the head's logits for up to sc_rows rows
@@ -417,9 +417,11 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
   if ((e = dalloc(&c->d_step, wb)) != hipSuccess) return bad(e);
   if ((e = dalloc(&c->d_out, wb * kOutSteps)) != hipSuccess) return bad(e);
   if ((e = dalloc(&c->d_amax, wb * kAmaxPerRow)) != hipSuccess) return bad(e);
-  c->ss_rows = std::max(c->wb, kAttnWideB);
-  if ((e = dalloc(&c->d_ss, (uint64_t)c->ss_rows * cf.heads * cf.ctx)) != hipSuccess) return bad(e);
-  if ((e = dalloc(&c->d_pm, (uint64_t)c->ss_rows * cf.heads * ((cf.ctx + kAttnTS - 1) / kAttnTS))) != hipSuccess) return bad(e);
+  if (!kv4) {   // (4-bit rings' attention has d_kpart alone)
+    c->ss_rows = std::max(c->wb, kAttnWideB);
+    if ((e = dalloc(&c->d_ss, (uint64_t)c->ss_rows * cf.heads * cf.ctx)) != hipSuccess) return bad(e);
+    if ((e = dalloc(&c->d_pm, (uint64_t)c->ss_rows * cf.heads * ((cf.ctx + kAttnTS - 1) / kAttnTS))) != hipSuccess) return bad(e);
+  }
   if ((e = dalloc(&c->QKV, (uint64_t)c->rows * 3 * d)) != hipSuccess) return bad(e);
   if ((e = dalloc(&c->Z, (uint64_t)c->rows * d)) != hipSuccess) return bad(e);
   if ((e = dalloc(&c->O, (uint64_t)c->rows * d)) != hipSuccess) return bad(e);
@@ -447,9 +449,11 @@ extern "C" int ana_open(const char* path, const ana_opts* opts, ana_ctx** out) {
   if (c->mode != ANA_EXACT_FP32) {
     // the fast kernels' scratch: attention partials for every row of a step,
     // the GLA scan's regions and tables
-    c->part_cap = attn_fast_part_floats(wrap_rows, cf.heads, cf.ctx, hd);
-    if ((e = dalloc(&c->d_part, c->part_cap)) != hipSuccess ||
-        (e = dalloc(&c->d_gla, gla_scan_floats(c->rows, c->gsub_cap, c->seg_cap, d, cf.heads))) != hipSuccess ||
+    if (!kv4) {
+      c->part_cap = attn_fast_part_floats(wrap_rows, cf.heads, cf.ctx, hd);
+      if ((e = dalloc(&c->d_part, c->part_cap)) != hipSuccess) return bad(e);
+    }
+    if ((e = dalloc(&c->d_gla, gla_scan_floats(c->rows, c->gsub_cap, c->seg_cap, d, cf.heads))) != hipSuccess ||
         (e = dalloc(&c->d_gtab, c->gsub_cap)) != hipSuccess || (e = dalloc(&c->d_atab, c->atab_cap)) != hipSuccess)
       return bad(e);
     c->gla = gla_scan_carve(c->d_gla, c->rows, c->gsub_cap, c->seg_cap, d, cf.heads);

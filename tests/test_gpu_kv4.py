@@ -1,6 +1,7 @@
 """Contexts whose softmax rings are held in 4 bits (ANA_KV4), against the
 model in 64 bits over the rings that the context itself holds, and the log
 probabilities of ana_logprobs and ana_score_logprobs_n against the logits."""
+import ctypes as C
 import math
 
 import numpy as np
@@ -219,6 +220,31 @@ def test_close_to_fp32_rings(models):
             x, y = x[:60].reshape(-1, 32), y[:60].reshape(-1, 32)
             top = np.abs(x).max(-1, keepdims=True)
             assert (np.abs(x - y) <= top * (2.0 / 7.0) + 1e-6).all()
+
+
+@pytest.mark.parametrize("mode", [ana_amd.FAST_FP32, ana_amd.BF16], ids=["fast_fp32", "bf16"])
+def test_memory(tmp_path, mode):
+    """A context with 4-bit rings holds less than one with fp32 rings by the
+    rings' difference at least: nothing else of it is larger, and none of the
+    fp32 rings' scratch is there."""
+    c = cf.Config(vocab=258, ctx=2048, d=256, f=512, layers=4, heads=4, rglru=True, qk=True, sinks=True, tied=True)
+    path, n = str(tmp_path / "long.ftc2"), 32
+    ckpt.write(path, c, ckpt.init_params(c, "normal", 5))
+    def free():
+        a, b = C.c_size_t(), C.c_size_t()
+        assert ana_amd.lib().hipMemGetInfo(C.byref(a), C.byref(b)) == 0
+        return a.value
+
+    held = []
+    for m in (mode, mode | ana_amd.KV4):
+        with ana_amd.Decoder(path, max_seqs=n, numerics=m):
+            pass   # (what the first context of a kind leaves behind)
+        before = free()
+        with ana_amd.Decoder(path, max_seqs=n, numerics=m):
+            held.append(before - free())
+    layers = sum(c.is_softmax(i) for i in range(c.layers))
+    rings = n * layers * (2 * c.ctx * c.d * 4 - c.heads * (c.ctx // 32) * 34 * c.hd)
+    assert held[0] - held[1] >= rings, (held, rings)
 
 
 def test_refused(models, tmp_path):
