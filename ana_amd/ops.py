@@ -7,6 +7,10 @@ torch holds the tensors, allocates outputs and workspaces, and names the
 stream: the work is queued on the tensors' device's current stream, can be
 captured there, and is not waited for. Tensors of other streams are the
 caller's to order, as for any torch operation. The results have no gradient.
+
+torch brings a HIP runtime of its own, which libana.so shares where torch is
+loaded first. Loaded after libana.so it starts a second one, which finds no
+GPU: import torch, or this module, before the first call of ana_amd.
 """
 from __future__ import annotations
 
@@ -15,6 +19,17 @@ import ctypes as C
 import torch
 
 from . import ANA_OK, AnaError, lib
+
+
+def _runtimes() -> set:
+    """The HIP runtimes that are loaded, by file."""
+    with open("/proc/self/maps") as f:
+        return {x.split()[-1] for x in f if "libamdhip64.so" in x}
+
+
+if len(_runtimes()) > 1:
+    raise ImportError("ana_amd.ops: torch was loaded after libana.so and has another HIP runtime than it "
+                      f"({', '.join(sorted(_runtimes()))}): import torch before the first call of ana_amd")
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 

@@ -3,6 +3,9 @@ mirror refuse, before a device is touched, and the 64-bit forms that the GPU
 tests compare with."""
 import ctypes as C
 import math
+import os
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -189,6 +192,21 @@ def test_mirror_refuses_host_tensors_and_shapes():
         ops.logprobs(torch.zeros(2, 5))
     with pytest.raises(ValueError, match="consecutive"):
         ops.logprobs(torch.zeros(5, 4).t())
+
+
+@pytest.mark.parametrize("first,ok", [("ana_amd.ops, ana_amd; ana_amd.lib()", True), ("torch, ana_amd; ana_amd.lib()", True),
+                                      ("ana_amd; ana_amd.lib()", False)])
+def test_mirror_refuses_a_second_runtime(first, ok):
+    """torch's HIP runtime loaded after libana.so's, where they are not the
+    same file, would find no GPU."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = f"import {first}; import torch, glob, os; n = glob.glob(os.path.dirname(torch.__file__) + '/lib/libamdhip64*'); " \
+           "print('own' if n else 'shared', flush=True); import ana_amd.ops; print('loaded')"
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=110)
+    if ok or r.stdout.startswith("shared"):
+        assert r.stdout.endswith("loaded\n"), r.stderr
+    else:
+        assert r.stdout == "own\n" and "import torch before the first call of ana_amd" in r.stderr
 
 
 # ---------------------------------------------------------------- the 64-bit forms
