@@ -1223,6 +1223,13 @@ static double attn_bytes_of(const ana_ctx* c, const uint32_t* pos, uint32_t n, u
   return b;
 }
 
+// the 4-bit rings' operators take positions below 2^31 (above, a row has no place)
+static int check_positions(ana_ctx* c, const char* fn, uint32_t i, uint32_t pos, uint32_t len) {
+  if (!c->kv4 || (uint64_t)pos + len <= 0x80000000ull) return ANA_OK;
+  return fail(c, ANA_EINVAL, "%s: positions %u .. %llu of sequence entry %u (4-bit rings: below 2^31)", fn, pos,
+              (unsigned long long)pos + len - 1, i);
+}
+
 static int check_seqs(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq) {
   if (n == 0 || n > c->max_seqs || !seq) return fail(c, ANA_EINVAL, "%s: %u sequences (1..%u)", fn, n, c->max_seqs);
   std::vector<uint8_t> seen(c->max_seqs, 0);
@@ -1302,8 +1309,10 @@ extern "C" int ana_feed(ana_ctx* c, uint32_t n, const uint32_t* seq, const uint3
   if (!c) return ANA_EINVAL;
   if (int r = check_seqs(c, "ana_feed", n, seq)) return r;
   if (!pos || !tok) return fail(c, ANA_EINVAL, "ana_feed: null argument");
-  for (uint32_t i = 0; i < n; i++)
+  for (uint32_t i = 0; i < n; i++) {
     if (tok[i] >= c->cfg.vocab) return fail(c, ANA_EINVAL, "ana_feed: token %u outside the vocabulary", tok[i]);
+    if (int r = check_positions(c, "ana_feed", i, pos[i], 1)) return r;
+  }
   HIPCHK(c, hipSetDevice(c->device));
   if (n == 1 && !fast_mode(c) && c->persist && !c->persist_off && !c->feed_off) {
     const int r = feed_persist(c, seq[0], pos[0], tok[0]);
@@ -1408,6 +1417,7 @@ static int feeds_n(ana_ctx* c, const char* fn, uint32_t n, const uint32_t* seq, 
     flen[i] = score ? (len[i] ? len[i] - 1 : 0) : len[i];
     coff[i] = ctot;
     ctot += score ? flen[i] : 0;
+    if (int r = check_positions(c, fn, i, pos[i], flen[i])) return r;
   }
   for (uint64_t i = 0; i < total; i++)
     if (toks[i] >= c->cfg.vocab) return fail(c, ANA_EINVAL, "%s: token %u outside the vocabulary", fn, toks[i]);
@@ -1746,8 +1756,10 @@ static int check_generate(ana_ctx* c, const char* fn, uint32_t n, const uint32_t
   if (!pos || !tok || (steps && !out)) return fail(c, ANA_EINVAL, "%s: null argument", fn);
   const bool greedy = !s || s->temperature <= 0.0f;
   if (!greedy && !rng) return fail(c, ANA_EINVAL, "%s: sampling needs rng state", fn);
-  for (uint32_t i = 0; i < n; i++)
+  for (uint32_t i = 0; i < n; i++) {
     if (tok[i] >= c->cfg.vocab) return fail(c, ANA_EINVAL, "%s: token %u outside the vocabulary", fn, tok[i]);
+    if (int r = check_positions(c, fn, i, pos[i], steps)) return r;
+  }
   return ANA_OK;
 }
 

@@ -63,8 +63,8 @@ extern "C" {
  * 2048, 12.6 MB a layer and sequence become 1.7 MB). Every row attends
  * to keys and values as the rings hold them, its own too; all else is the mode's. The
  * rounding is the checkpoint's to bear: the modes' tolerances do not cover it. Head
- * dimensions of 32 and 64; the one-sequence loops take the step graphs. ANA_EUNSUP with
- * ANA_EXACT_FP32 */
+ * dimensions of 32 and 64, positions below 2^31 (ANA_EINVAL past them); the one-sequence
+ * loops take the step graphs. ANA_EUNSUP with ANA_EXACT_FP32 */
 #define ANA_KV4 0x100
 
 /* bend/Config.bend:7-10 */

@@ -259,6 +259,34 @@ def test_refused(models, tmp_path):
         ana_amd.Decoder(small, numerics=ana_amd.FAST_FP32 | ana_amd.KV4)
 
 
+@pytest.mark.parametrize("mode", [ana_amd.FAST_FP32, ana_amd.BF16], ids=["fast_fp32", "bf16"])
+def test_last_positions(models, mode):
+    """The largest position of a 4-bit ring is stored and attended; calls that
+    reach past it are refused before they change anything."""
+    c, path, w = models["mid"]
+    far = 2 ** 31 - 1
+    with ana_amd.Decoder(path, max_seqs=2, numerics=mode | ana_amd.KV4) as dec:
+        rows = [Row(c, w) for _ in range(2)]
+        dec.feeds(0, far - 2, [5, 6])
+        for t, tok in enumerate((5, 6)):
+            rows[0].feed(tok, far - 2 + t, rings(dec, 0, c))
+        before = [dec.state(0, i) for i in range(c.layers + 1)]
+        for call in (lambda: dec.feed([0], [far + 1], [7]), lambda: dec.feed([1, 0], [0, 2 ** 32 - 1], [7, 7]),
+                     lambda: dec.feeds(0, far, [7, 8]), lambda: dec.feeds_n([1, 0], [0, far - 1], [[3], [7, 8, 9]]),
+                     lambda: dec.generate([0], [far], [7], 2), lambda: dec.score_n([0], [far], [[7, 8, 9]]),
+                     lambda: dec.score_logprobs_n([0], [2 ** 32 - 2], [[7, 8]])):
+            with pytest.raises(ana_amd.AnaError, match="below 2\\^31"):
+                call()
+        assert all(np.array_equal(x, dec.state(0, i)) for i, x in enumerate(before)) and not dec.state(1, 3).any()
+        dec.feed([0], [far], [7])
+        ring = rings(dec, 0, c)
+        want, kv = rows[0].feed(7, far, ring)
+        held(c, kv, ring, far % c.ctx, 1e-4 if mode == ana_amd.FAST_FP32 else 4e-2)
+        assert rel(dec.logits([0])[0], want) <= TOL[mode]
+    with ana_amd.Decoder(path, numerics=mode) as dec:   # (fp32 rings take every position)
+        dec.feed([0], [far + 1], [7])
+
+
 # ---------------------------------------------------------------- log probabilities of a context
 
 MODES = [ana_amd.EXACT_FP32, ana_amd.FAST_FP32, ana_amd.BF16, ana_amd.FAST_FP32 | ana_amd.KV4]
