@@ -1,5 +1,6 @@
 """The operators on device memory (ana_amd.ops) on the GPU, against their
 definitions in 64 bits (device_ops_ref)."""
+import ctypes
 import math
 
 import numpy as np
@@ -284,6 +285,96 @@ def test_attend_split(ops, n, hq, hkv, hd, slots, pos):
     assert (both[:m] - one).abs().max() <= 1e-5 * one.abs().max()
 
 
+def pieces_of(ops, cache, n, rows, ragged, hq, live=0):
+    """The pieces that a call's slots are cut into at most, by its workspace."""
+    r = ops._Rows(n, rows, None, 1, 1 if ragged else None)
+    ws = ana_amd.lib().ana_kv4_attend_ws(cache._p, ctypes.byref(r), hq, live)
+    return max(1, ws // (4 * rows * hq * (4 + cache.hd)))
+
+
+# (type, query heads, key heads, hd, slots, pos, off)
+LONG = [
+    ("f32", 2, 2, 64, 20000, [19001], None), ("bf16", 8, 2, 128, 9000, [8999, 30000], None),
+    ("f16", 3, 3, 32, 40000, [33333], None), ("bf16", 20, 1, 64, 6000, [5017], None),
+    ("f32", 6, 1, 128, 7000, [6999, 3001, 70], None),
+    ("f32", 2, 1, 64, 9001, [9000, 4000], [0, 3, 8]), ("bf16", 4, 2, 64, 9000, [8200], [0, 4]),      # few rows
+    ("f16", 4, 1, 128, 5000, [4990, 17], [0, 2, 6]),
+    ("f32", 2, 2, 64, 12000, [11000, 3000], [0, 70, 120]), ("bf16", 4, 1, 128, 8000, [7000], [0, 90]),  # many
+    ("f16", 2, 1, 32, 20000, [19000], [0, 64])]
+
+
+@pytest.mark.parametrize("typ,hq,hkv,hd,slots,pos,off", LONG)
+def test_long_rings_count_every_slot_once(ops, typ, hq, hkv, hd, slots, pos, off):
+    """Keys of zero: every seen slot weighs 1, and an output is the mean of
+    the values, whose sums are exact (multiples of 1/2 below 2^22), in
+    probabilities, over the pieces and in the join. What is left is a
+    reciprocal, a product and the output's rounding. A slot that is lost, or
+    counted twice, moves the mean (itself a value over the root of their
+    number) by a value over their number."""
+    rs = np.random.RandomState(17)
+    n, rows = len(pos), len(pos) if off is None else off[-1]
+    cache = ops.KV4.empty(n, slots, hkv, hd)
+    codes = rs.randint(0, 256, tuple(cache.data.shape)).astype(np.uint8)
+    codes[..., :16 * hd] = 0
+    codes[..., 32 * hd:] = 127
+    cache.data.copy_(torch.tensor(codes))
+    assert pieces_of(ops, cache, n, rows, off is not None, hq) > 1
+    q, _ = rand(rs, (rows, hq, hd), typ)
+    G, e = hq // hkv, 2.0 ** -24
+    for sink in (None, 0.0):
+        sk = None if sink is None else torch.zeros(hq, device="cuda")
+        got = ops.kv4_attend(q, cache, dev(pos), off=None if off is None else dev(off), sink=sk).double().cpu().numpy()
+        for i in range(n):
+            r0, r1 = (i, i + 1) if off is None else (off[i], off[i + 1])
+            last = pos[i] + r1 - r0 - 1
+            idx = np.arange(slots)
+            at = last - (last - idx) % slots
+            for h in range(hkv):
+                _, V = ref.get(codes, i, h, slots)
+                by_at = np.zeros((r1 - r0, hd))
+                for r in range(r0, r1):
+                    see = (at >= 0) & (at <= pos[i] + r - r0)
+                    by_at[r - r0] = V[see].sum(0) / (see.sum() + (0 if sink is None else 1))
+                want = by_at[:, None, :]
+                g = got[r0:r1, h * G:(h + 1) * G]
+                tol = np.abs(want) * (2 * e + e * e + (0.0 if typ == "f32" else ref.EPS[typ] * (1 + 3 * e))) + \
+                    (2.0 ** -25 if typ == "f16" else 0.0)
+                assert (np.abs(g - want) <= tol).all(), (i, h, sink)
+
+
+@pytest.mark.parametrize("typ", list(TYPES))
+@pytest.mark.parametrize("rows", [1, 3, 40])
+def test_long_rings_find_every_tile(ops, typ, rows):
+    """A query that matches one slot's key takes that slot's value, whichever
+    tile it is in, over the pieces' different maxima (the last row of each of
+    the call's sequences; the ones before it look elsewhere)."""
+    rs = np.random.RandomState(18)
+    slots, hd = 6000 + 13, 64
+    cache = filled(ops, rs, 1, slots, 1, hd)
+    K, V = ref.get(cache.data.cpu().numpy(), 0, 0, slots)
+    tiles = -(-slots // 32)
+    find = np.minimum(np.arange(tiles) * 32 + rs.randint(0, 32, tiles), slots - 1)
+    per = 12
+    for at in range(0, tiles, per):
+        slot = find[at:at + per]
+        n = len(slot)
+        q64 = rs.standard_normal((n, rows, 2, hd))
+        q64[:, -1] = 4.0 * K[slot][:, None]
+        q = torch.tensor(q64.reshape(n * rows, 2, hd)).to(TYPES[typ]).cuda()
+        off = None if rows == 1 else dev(np.arange(n + 1) * rows)
+        pos = dev([slots - rows] * n)
+        seq = dev([0] * n)
+        if at == 0:
+            assert pieces_of(ops, cache, n, n * rows, rows > 1, 2) > 1
+        got = ops.kv4_attend(q, cache, pos, seq=seq, off=off).double().cpu().numpy().reshape(n, rows, 2, hd)[:, -1]
+        x = q.double().cpu().numpy().reshape(n, rows, 2, hd)[:, -1] @ K.T * hd ** -0.5
+        p = np.exp(x - x.max(-1, keepdims=True))
+        want = p @ V / p.sum(-1, keepdims=True)
+        # (the slot's weight is all but 1: what a wrong piece gives is off by the values' own size)
+        assert (p.max(-1) / p.sum(-1) > 0.99).all()
+        assert (np.abs(got - want) <= 0.02 * np.abs(V).max()).all(), at
+
+
 def test_attend_piece_of_a_long_ring(ops):
     """A prompt's piece over a long past: its slots split, then joined."""
     rs = np.random.RandomState(6)
@@ -506,6 +597,52 @@ def test_deterministic(ops):
     q, _ = rand(rs, (3, 8, 64), "f32")
     a = [ops.kv4_attend(q, cache, dev([2999, 100, 1500])) for _ in range(5)]
     assert all(torch.equal(a[0], x) for x in a)
+
+
+def test_two_calls_at_once(ops):
+    """Two streams' calls side by side, then two graphs replayed side by
+    side: each has its own workspaces, and gives what it gives alone."""
+    rs = np.random.RandomState(19)
+    work = []
+    for i in range(2):
+        cache = filled(ops, rs, 2, 9000, 2, 64)
+        q, _ = rand(rs, (2, 4, 64), "f32")
+        rows, _ = rand(rs, (2, 50021), "f32", 3.0)
+        work.append((cache, q, dev([8999 - i, 4000]), rows, dev([7, 40000 + i])))
+
+    def one(w):
+        cache, q, pos, rows, tok = w
+        return [ops.kv4_attend(q, cache, pos), *ops.logprobs(rows, tok, 20)]
+
+    assert pieces_of(ops, work[0][0], 2, 2, False, 4) > 1
+    want = [one(w) for w in work]
+    assert not torch.equal(want[0][0], want[1][0])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(12):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(one(work[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for g in got[i] for a, b in zip(g, want[i])), i
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], [None] * 2
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            outs[i] = one(work[i])
+    for step in range(4):
+        for w in work:
+            w[1].mul_(1.25)
+            w[3].mul_(0.75)
+        want = [one(w) for w in work]
+        torch.cuda.synchronize()
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+        torch.cuda.synchronize()
+        for i in range(2):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], want[i])), (step, i)
 
 
 # ---------------------------------------------------------------- log probabilities

@@ -1,7 +1,7 @@
 """Contexts whose softmax rings are held in 4 bits (ANA_KV4), against the
 model in 64 bits over the rings that the context itself holds, and the log
 probabilities of ana_logprobs and ana_score_logprobs_n against the logits."""
-import ctypes as C
+import ctypes
 import math
 
 import numpy as np
@@ -11,6 +11,7 @@ import ana_amd
 import device_ops_ref as ref
 from ana_amd import ckpt
 from ana_amd import config as cf
+from ana_amd import ops
 
 pytestmark = pytest.mark.gpu
 
@@ -222,6 +223,98 @@ def test_close_to_fp32_rings(models):
             assert (np.abs(x - y) <= top * (2.0 / 7.0) + 1e-6).all()
 
 
+@pytest.fixture(scope="module")
+def long_model(tmp_path_factory):
+    """A window of 35 tiles: attention over it is cut into pieces."""
+    c = cf.Config(vocab=258, ctx=1100, d=256, f=512, layers=4, heads=4, rglru=True, qk=True, sinks=True, tied=True)
+    w = ckpt.init_params(c, "normal", 7, trained=True)
+    path = str(tmp_path_factory.mktemp("kv4long") / "long.ftc2")
+    ckpt.write(path, c, w)
+    for n, rows, off in ((1, 1, False), (3, 3, False), (3, 600, True)):   # single rows; a prefill step's
+        k = ops._Kv4(16, 0, 3, c.ctx, c.heads, c.hd)
+        r = ops._Rows(n, rows, 1, 1, 1 if off else None)
+        assert ana_amd.lib().ana_kv4_attend_ws(ctypes.byref(k), ctypes.byref(r), c.heads, 0) >= 2 * 4 * rows * c.heads * (4 + c.hd)
+    return c, path, np.asarray(w, dtype=np.float64)
+
+
+@pytest.mark.parametrize("mode", [ana_amd.FAST_FP32, ana_amd.BF16], ids=["fast_fp32", "bf16"])
+def test_rings_in_pieces(long_model, mode):
+    """Prompts over a long past (every row's log probability), then single
+    tokens of one and of several sequences, past the wrap too, against the
+    64-bit model over the context's own rings."""
+    c, path, w = long_model
+    lens = [1097, 600, 941]
+    toks = [tokens(k + 8, 90 + i, c.vocab) for i, k in enumerate(lens)]
+    with ana_amd.Decoder(path, max_seqs=3, numerics=mode | ana_amd.KV4) as dec:
+        rows, past, fed = [Row(c, w) for _ in range(3)], [0] * 3, [0] * 3
+        for cut in (260, 10 ** 6):
+            # (a window scores the token after its last fed one)
+            win = [toks[i][past[i]:min(lens[i], past[i] + cut) + 1] for i in range(3)]
+            got = dec.score_logprobs_n([0, 1, 2], past, win, top=2)
+            for i in range(3):
+                ring = rings(dec, i, c)
+                for t in range(len(win[i]) - 1):
+                    want, kv = rows[i].feed(win[i][t], past[i] + t, ring)
+                    if t % 23 == 0 or t + 2 >= len(win[i]):
+                        held(c, kv, ring, past[i] + t, 1e-4 if mode == ana_amd.FAST_FP32 else 4e-2)
+                    # a logit's error counts twice: in the token's own and in the sum's
+                    tol = 2 * TOL[mode] * np.abs(want).max() + 1e-5
+                    m = want.max()
+                    lp = want[win[i][t + 1]] - m - math.log(np.exp(want - m).sum())
+                    assert abs(got[i].logprob[t] - lp) <= tol, (i, past[i] + t)
+                past[i] += len(win[i]) - 1
+        for t in range(8):
+            for seqs in ([1], [2, 0]):
+                dec.feed(seqs, [past[i] for i in seqs], [toks[i][past[i]] for i in seqs])
+                for i, lg in zip(seqs, dec.logits(seqs)):
+                    want, _ = rows[i].feed(toks[i][past[i]], past[i], rings(dec, i, c))
+                    assert rel(lg, want) <= TOL[mode], (i, past[i])
+                    past[i] += 1
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_loops_over_pieces(long_model, n):
+    """The token loops (captured steps) over windows in pieces, past the wrap
+    too: feeds and picks one at a time give the same."""
+    c, path, _ = long_model
+    lens = [1080, 350, 800][:n]
+    toks = [tokens(k + 1, 70 + i, c.vocab) for i, k in enumerate(lens)]
+    seqs = list(range(n))
+    mode = ana_amd.FAST_FP32 | ana_amd.KV4
+    with ana_amd.Decoder(path, max_seqs=n, numerics=mode) as a, ana_amd.Decoder(path, max_seqs=n, numerics=mode) as b:
+        for d in (a, b):
+            d.feeds_n(seqs, [0] * n, [t[:-1] for t in toks])
+        cur = [t[-1] for t in toks]
+        out = [a.generate(seqs, lens, cur, 20), None]
+        out[1] = a.generate(seqs, [k + 20 for k in lens], [int(t) for t in out[0][:, -1]], 20)   # the graph again
+        for k in range(40):
+            b.feed(seqs, [p + k for p in lens], cur)
+            cur = [int(t) for t in b.top(seqs)]
+            assert cur == [int(t) for t in out[k // 20][:, k % 20]], k
+        assert np.array_equal(a.logits(seqs), b.logits(seqs))
+        for i in seqs:
+            assert np.array_equal(a.state(i, 3), b.state(i, 3))
+
+
+@pytest.mark.parametrize("n", [1, 3])
+def test_loops_that_allocate_nothing(long_model, n):
+    """ana_generate_noalloc over 4-bit rings in pieces: the loop's picks."""
+    c, path, _ = long_model
+    lens = [1085, 350, 800][:n]
+    toks = [tokens(k + 1, 70 + i, c.vocab) for i, k in enumerate(lens)]
+    seqs = np.arange(n, dtype=np.uint32)
+    mode, u32 = ana_amd.FAST_FP32 | ana_amd.KV4, ctypes.POINTER(ctypes.c_uint32)
+    with ana_amd.Decoder(path, max_seqs=n, numerics=mode) as a, ana_amd.Decoder(path, max_seqs=n, numerics=mode) as b:
+        for d in (a, b):
+            d.feeds_n(list(seqs), [0] * n, [t[:-1] for t in toks])
+        cur = np.array([t[-1] for t in toks], dtype=np.uint32)
+        want = a.generate(list(seqs), lens, [int(t) for t in cur], 25)
+        out = np.zeros((n, 25), dtype=np.uint32)
+        args = [x.ctypes.data_as(u32) for x in (seqs, np.array(lens, dtype=np.uint32), cur)]
+        assert ana_amd.lib().ana_generate_noalloc(b.h, n, *args, 25, None, None, out.ctypes.data_as(u32)) == 0
+        assert np.array_equal(out, want)
+
+
 @pytest.mark.parametrize("mode", [ana_amd.FAST_FP32, ana_amd.BF16], ids=["fast_fp32", "bf16"])
 def test_memory(tmp_path, mode):
     """A context with 4-bit rings holds less than one with fp32 rings by the
@@ -231,8 +324,8 @@ def test_memory(tmp_path, mode):
     path, n = str(tmp_path / "long.ftc2"), 32
     ckpt.write(path, c, ckpt.init_params(c, "normal", 5))
     def free():
-        a, b = C.c_size_t(), C.c_size_t()
-        assert ana_amd.lib().hipMemGetInfo(C.byref(a), C.byref(b)) == 0
+        a, b = ctypes.c_size_t(), ctypes.c_size_t()
+        assert ana_amd.lib().hipMemGetInfo(ctypes.byref(a), ctypes.byref(b)) == 0
         return a.value
 
     held = []
@@ -364,6 +457,32 @@ def test_score_logprobs(models, mode):
             dec.reset(s)
         none = dec.score_logprobs_n(seqs, zero, toks)
         assert none[0].top.shape == (39, 0) and np.array_equal(none[0].rank, got[0].rank)
+
+
+@pytest.mark.parametrize("mode", MODES, ids=["exact", "fast_fp32", "bf16", "fast_kv4"])
+def test_score_logprobs_repeats(models, mode):
+    """The same windows scored twice, and (exact mode) one by one: the same
+    numbers, bit for bit."""
+    c, path, _ = models["mid"]
+    lens = [40, 1, 2, 70, 0]
+    toks = [tokens(k, 60 + i, c.vocab) for i, k in enumerate(lens)]
+    with ana_amd.Decoder(path, max_seqs=5, prefill_chunk=16, numerics=mode) as dec:
+        seqs = list(range(5))
+        got = []
+        for _ in range(2):
+            got.append(dec.score_logprobs_n(seqs, [0] * 5, toks, top=5))
+            for s in seqs:
+                dec.reset(s)
+        for a, b in zip(*got):
+            for f in ("logprob", "entropy", "rank", "top", "top_logprob"):
+                assert np.array_equal(getattr(a, f), getattr(b, f)), f
+        assert got[0][0].logprob.std() > 0.1 and got[0][3].logprob.std() > 0.1
+        if mode == ana_amd.EXACT_FP32:
+            # (its rows' logits do not depend on what is fed beside them)
+            for i in (0, 3):
+                one = dec.score_logprobs_n([i], [0], [toks[i]], top=5)[0]
+                for f in ("logprob", "entropy", "rank", "top", "top_logprob"):
+                    assert np.array_equal(getattr(one, f), getattr(got[0][i], f)), f
 
 
 def test_logprobs_refused(models):
