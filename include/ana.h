@@ -319,9 +319,11 @@ int ana_manifest_read(const char* path, ana_manifest* out);
  * current device is left as it was. Any thread may call them; after a
  * nonzero answer ana_error(NULL) holds the calling thread's message.
  *
- * Tensors are [rows][heads][hd] with any strides between rows and between
- * heads, counted in elements, the last axis consecutive. Addresses and
- * strides on 16 bytes are read and written fastest. */
+ * Tensors are [rows][heads][hd], the strides between rows and between heads
+ * counted in elements, the last axis consecutive. Strides of hd elements or
+ * more, in any order; a tensor whose rows or heads share elements (a
+ * broadcast one, stride 0) is refused with ANA_EINVAL, an input as an output.
+ * Addresses and strides on 16 bytes are read and written fastest. */
 #define ANA_T_F32 0
 #define ANA_T_BF16 1
 #define ANA_T_F16 2
@@ -330,9 +332,12 @@ int ana_manifest_read(const char* path, ana_manifest* out);
  * (position p in slot p mod slots), `heads` key heads of hd = 32, 64 or 128
  * values. MXFP4: a value is an E2M1 code (0, 0.5, 1, 1.5, 2, 3, 4 or 6 and a
  * sign), and 32 values next to each other along a head share a scale byte b,
- * 2^(b - 127). A block with largest magnitude a takes the least scale from
- * 2^-125 on with a <= 7 scale, a value the nearest code, ties to the even
- * one; a block with an infinity or a NaN in it becomes NaN (b = 255).
+ * 2^(b - 127). A block with largest magnitude a takes the least scale of
+ * 2^-125 .. 2^125 with a <= 7 scale (past that the largest, and values past
+ * its 6 are that), a value the nearest code, ties to the even one; a block
+ * with an infinity or a NaN in it becomes NaN (b = 255). So stored scale bytes
+ * are 2 .. 252 and 255, and every value is a bfloat16; a cache from elsewhere
+ * keeps to them (zeros stand for slots that hold nothing).
  * data holds ana_kv4_bytes bytes on a 16-byte border, for each sequence and
  * head ceil(slots / 32) records of 32 slots and 34 hd bytes:
  *   keys    [4 j][16 m][2 h][hd / 8]  slot 16 h + m, dims j hd / 4 ..
@@ -387,8 +392,9 @@ int ana_kv4_read(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_ma
  * e^sink[a]), sink (hq floats) NULL for none; 0 where it sees nothing.
  * What a row does not see, NaN included, does not change it. In f32 the
  * products are exact up to their f32 sums; 16-bit outputs take
- * probabilities to 2^-16, bf16 ones of a sequence with more than 16 query
- * rows a key head rounded to bf16. `live`, where not 0, is the most positions a
+ * probabilities to 2^-16, but bf16 ones of a sequence with more than 16 query
+ * rows a key head (rows times hq / heads) each rounded to bf16, which adds to
+ * an output as much again as its own rounding: a call's rows decide which. `live`, where not 0, is the most positions a
  * sequence holds after the call, as far as the caller knows: it only
  * chooses how the work is split. o may be q itself (the same address and
  * strides). ws: ana_kv4_attend_ws bytes of workspace for the same arguments,
