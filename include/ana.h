@@ -406,7 +406,7 @@ int ana_kv4_attend(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_
 uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq, uint64_t live);
 
 /* Of n rows of `vocab` logits (of ANA_T_ type `type`, ld elements from row
- * to row), in one read of them: lp[i], the log probability of the given
+ * to row, vocab or more), in one read of them: lp[i], the log probability of the given
  * token tok[i] (NaN for a token outside the vocabulary), and rank[i], the
  * tokens before it in the order of value, then of lower index (0: it is the
  * greedy pick; 2^32 - 1 outside the vocabulary); tok NULL: neither is

@@ -342,6 +342,45 @@ def test_long_rings_count_every_slot_once(ops, typ, hq, hkv, hd, slots, pos, off
                 assert (np.abs(g - want) <= tol).all(), (i, h, sink)
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("slots,pos,seq,off", [
+    (5000, [4000, -1, 4990, 10], [1, 0, 9, 2], [5, 8, 11, 14, 17]),            # few rows; two without a place
+    (5000, [4000, 70, -3, 4980], [1, 0, 2, 2], [7, 60, 100, 140, 200]),        # many
+    (700, [3000, 5, 100], [0, 2, 1], [1, 750, 753, 1500]),                     # longer than the ring: rows that see nothing
+    (5000, [3000, -1, 9, 4999], [3, 0, 1, 0], None)])
+def test_long_rings_rows_outside(ops, typ, slots, pos, seq, off):
+    """Calls in pieces: rows of no sequence stay, rows without a place are
+    zeros, rows that see nothing are zeros with a sink and without, and the
+    others are what they are whole (the 64-bit test has those)."""
+    rs = np.random.RandomState(24)
+    n, rows = len(pos), len(pos) if off is None else off[-1] + 9
+    cache = filled(ops, rs, 4, slots, 2, 64)
+    q, _ = rand(rs, (rows, 4, 64), typ)
+    args = dict(seq=dev(seq), off=None if off is None else dev(off))
+    assert pieces_of(ops, cache, n, rows, off is not None, 4) > 1
+    assert pieces_of(ops, cache, n, rows, off is not None, 4, live=1) == 1
+    for sink in (None, torch.tensor(rs.randn(4), dtype=torch.float32, device="cuda")):
+        got, whole = (torch.full((rows, 4, 64), 3.0, dtype=TYPES[typ], device="cuda") for _ in range(2))
+        ops.kv4_attend(q, cache, dev(pos), sink=sink, out=got, **args)
+        ops.kv4_attend(q, cache, dev(pos), sink=sink, out=whole, live=1, **args)
+        some = torch.zeros(rows, dtype=torch.bool, device="cuda")     # rows of a sequence
+        sees = some.clone()
+        for i in range(n):
+            r0, r1 = (i, i + 1) if off is None else (off[i], off[i + 1])
+            some[r0:r1] = True
+            sees[max(r0, r1 - slots):r1] = 0 <= pos[i] and 0 <= seq[i] < 4
+        assert (got[~some] == 3).all() and not got[some & ~sees].any()
+        assert got[sees].abs().amax((1, 2)).min() > 0
+        a, b = got[sees].double(), whole[sees].double()
+        # each within attend_tolerance of the formula: scores of sizes up to 10 and
+        # sums of up to `slots`, against sum p |v| (below the largest value), twice
+        v = ops.kv4_read(cache, dev([0] * 4), 4 * slots, off=dev(np.arange(5) * slots))[1].abs().max()
+        tol = 2 * (2 * slots + 4096) * 2.0 ** -24 * v
+        if typ == "bf16":
+            tol = tol + 2 * (2 * 2.0 ** -8 * v + 2.0 ** -8 * b.abs())
+        assert ((a - b).abs() <= tol).all()
+
+
 @pytest.mark.parametrize("typ", list(TYPES))
 @pytest.mark.parametrize("rows", [1, 3, 40])
 def test_long_rings_find_every_tile(ops, typ, rows):
