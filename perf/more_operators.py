@@ -1,0 +1,620 @@
+"""More operators on device memory whose speed is measured: their inputs, their
+plain form, the calls of ana_amd.ops, and their results in 64 bits. Together
+they are what a decode step of many answers to one prompt asks of a program
+that holds its own tensors.
+
+Three kinds of case, one operator's pass each:
+
+- "rope": queries and keys of each head, RMS-normed (or not), with their
+  positions' rotation, in one pass. qk_rope.
+- "shared": softmax attention of query rows over a 4-bit cache, where groups
+  of rows also see one long prefix that they have in common. kv4_attend_shared.
+- "sample": a token of each row of logits from a given random number, with a
+  temperature, top-k, top-p and min-p. sample.
+
+A case is a dict of plain values. For "rope" and "shared":
+
+- n sequences, hq query heads over hkv key heads of hd values;
+- past: the tokens the first sequence holds before the call; the others' go
+  down evenly to past - past_spread;
+- rows: the tokens of the first sequence in the call (0: one token of each
+  sequence, the decode form); the others' go down evenly to rows -
+  rows_spread;
+- type: the tensors' ("f32", "bf16", "f16").
+
+"rope" has rot, the dimensions of a head that turn, norm, and near: whether a
+pair is two neighbours or one of each half. "shared" has rings of `slots`
+positions for the sequences' own tokens, m groups of sequences with a prefix
+each (the first of `prefix` tokens, the others' going down evenly to prefix -
+prefix_spread), and sink: whether each query head has a sink logit.
+
+For "sample": n rows of `vocab` logits, pad more elements between rows, the
+logits' type, and t, k, p, q: temperature, top-k, top-p and min-p (k 0, p 1, q
+0: none); mixed: every row has settings of its own around these, some rows
+greedy.
+
+The cache's bytes. A cache is uint8 [seqs, hkv, ceil(slots / 32), 34 hd]: a
+record holds 32 slots of one head. A value is an E2M1 code (sign, then 0, 0.5,
+1, 1.5, 2, 3, 4, 6), 32 values next to each other along a head share an E8M0
+scale (a byte b stands for 2^(b - 127)). With D = hd and the even dimension in
+a byte's low half, a record is
+
+    keys    [4 j][16 m][2 h][D / 8 bytes]   slot 16 h + m, dims j D / 4 ...
+    values  [4 j][16 m][8 e][D / 32 bytes]  slot 16 (e / 4) + 4 j + e % 4, dims m D / 16 ...
+    scales of the keys    [D / 32 blocks][16 m][2 h]
+    scales of the values  [D / 32 blocks][4 j][8 e]
+"""
+import math
+
+import numpy as np
+import torch
+
+own = False
+
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+BYTES = {"f32": 4, "bf16": 2, "f16": 2}
+EPS = 1e-5
+
+
+# ---------------------------------------------------------------- the cases
+
+def _rope(name, type, n, hq, hkv, hd, rot, norm, near, past, past_spread, rows, rows_spread):
+    c = {"kind": "rope", "type": type, "n": n, "hq": hq, "hkv": hkv, "hd": hd, "rot": rot, "norm": norm, "near": near,
+         "past": past, "past_spread": past_spread, "rows": rows, "rows_spread": rows_spread}
+    return dict(c, name=name) if name else c
+
+
+def _shared(name, type, n, hq, hkv, hd, slots, past, past_spread, rows, rows_spread, m, prefix, prefix_spread, sink):
+    c = {"kind": "shared", "type": type, "n": n, "hq": hq, "hkv": hkv, "hd": hd, "slots": slots, "past": past,
+         "past_spread": past_spread, "rows": rows, "rows_spread": rows_spread, "m": m, "prefix": prefix,
+         "prefix_spread": prefix_spread, "sink": sink}
+    return dict(c, name=name) if name else c
+
+
+def _sample(name, type, n, vocab, pad, t, k, p, q, mixed):
+    c = {"kind": "sample", "type": type, "n": n, "vocab": vocab, "pad": pad, "t": t, "k": k, "p": p, "q": q,
+         "mixed": mixed}
+    return dict(c, name=name) if name else c
+
+
+def listed():
+    return [
+        # one user's token: a call whose latency counts (12 heads of 64, as
+        # the 115M model has them)
+        _rope("rope_1", "f32", 1, 12, 12, 64, 64, True, False, 300, 0, 0, 0),
+        # a decode step of 64 conversations of all lengths, grouped queries
+        _rope("rope_64_step", "bf16", 64, 32, 8, 128, 128, True, False, 30000, 29000, 0, 0),
+        # a prefill step of 16 ragged prompts, half of each head turned
+        _rope("rope_16_prompts", "f32", 16, 12, 12, 64, 32, True, True, 0, 0, 640, 250),
+        # the next piece of four long documents, without norms
+        _rope("rope_4_pieces", "bf16", 4, 32, 8, 128, 128, False, False, 100001, 60000, 4096, 0),
+        # eight answers to one user's prompt: latency again
+        _shared("shared_8_answers", "f32", 8, 12, 12, 64, 512, 40, 30, 0, 0, 1, 700, 0, True),
+        # 64 agent episodes behind one system prompt (the 115M model's heads)
+        _shared("shared_64_agents", "f32", 64, 12, 12, 64, 2048, 500, 450, 0, 0, 1, 1400, 0, True),
+        # 256 answers about one long document, query heads sharing keys
+        _shared("shared_256_document", "bf16", 256, 32, 8, 128, 4096, 2000, 1900, 0, 0, 1, 32001, 0, False),
+        # the next turns of 48 conversations behind three system prompts
+        _shared("shared_48_turns", "bf16", 48, 16, 4, 128, 4096, 600, 600, 200, 190, 3, 8000, 5000, False),
+        # one user's pick: vocabulary 32768, as the 115M model's
+        _sample("sample_1", "f32", 1, 32768, 0, 0.8, 40, 0.95, 0.0, False),
+        # a serving batch, each request with settings of its own
+        _sample("sample_512_mixed", "f32", 512, 32768, 0, 0.9, 50, 0.9, 0.02, True),
+        # four rows of a wide vocabulary, the nucleus alone
+        _sample("sample_4_wide", "f32", 4, 200003, 0, 0.7, 0, 0.95, 0.0, False),
+        # rollouts in 16 bits, an odd vocabulary, padded rows: ties everywhere
+        _sample("sample_3000_odd", "bf16", 3000, 50021, 3, 1.0, 0, 0.9, 0.01, False),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    kind = rng.choice(["rope", "shared", "shared", "sample", "sample"])
+    type = rng.choice(["f32", "f32", "bf16", "f16"])
+    if kind == "sample":
+        vocab = _log(rng, 200, 200000)
+        n = _log(rng, 1, min(4000, 150000000 // vocab))
+        k = rng.choice([0, 0, 1, _log(rng, 2, 64), _log(rng, 65, 2000)])
+        return _sample("", type, n, vocab, rng.choice([0, 0, 1, 5]), round(rng.uniform(0.3, 1.5), 2), min(k, vocab),
+                       rng.choice([1.0, 0.5, 0.9, 0.95]), rng.choice([0.0, 0.0, 0.02, 0.1]), rng.random() < 0.3)
+    if kind == "rope":
+        hd = 16 * rng.randrange(1, 17)
+        rot = hd if rng.random() < 0.6 else 16 * rng.randrange(1, hd // 16 + 1)
+        hkv = rng.randrange(1, 13)
+        hq = hkv * rng.choice([1, 1, 2, 4])
+        rows, n = rng.choice([0, _log(rng, 2, 4000)]), _log(rng, 1, 256)
+        n = max(1, min(n, 80000000 // (max(rows, 1) * (hq + hkv) * hd)))
+        past = rng.choice([0, _log(rng, 1, 1000000)])
+        return _rope("", type, n, hq, hkv, hd, rot, rng.random() < 0.6, rng.random() < 0.4, past,
+                     rng.randrange(0, past) if past else 0, rows, rng.randrange(0, rows) if rows else 0)
+    hd = rng.choice([32, 64, 64, 128])
+    hkv = _log(rng, 1, 1024 // hd)
+    hq = hkv * rng.choice([1, 1, 2, 4, 8] if hkv * hd <= 512 else [1, 1, 2])
+    m, prefix = rng.choice([1, 1, 2, 5]), _log(rng, 10, 40000)
+    if rng.random() < 0.6:
+        # single tokens; their own rings may have wrapped
+        n, slots = _log(rng, m, 256), _log(rng, 33, 5000)
+        slots = max(33, min(slots, 600000000 // (n * hkv * hd)))
+        past = _log(rng, 1, 2 * slots)
+        past_spread, rows, rows_spread = rng.randrange(0, past), 0, 0
+    else:
+        n, rows = _log(rng, m, 48), _log(rng, 2, 400)
+        rows_spread = rng.randrange(0, rows)
+        past = rng.choice([0, min(_log(rng, 1, 3000), 100000000 // (n * rows * hq))])
+        past_spread = rng.randrange(0, past) if past else 0
+        slots = past + rows + rng.randrange(0, 100)
+    prefix = max(10, min(prefix, 250000000 // (n * max(rows, 1) * hq)))
+    return _shared("", type, n, hq, hkv, hd, slots, past, past_spread, rows, rows_spread, m, prefix,
+                   rng.randrange(0, prefix), rng.random() < 0.5)
+
+
+# ---------------------------------------------------------------- the inputs
+
+def _device():
+    return "cuda" if torch.cuda.is_available() else "cpu"
+
+
+def _lengths(case):
+    """Each sequence's tokens before the call, and in it."""
+    n = case["n"]
+    past = [case["past"] - case["past_spread"] * i // n for i in range(n)]
+    rows = [max(1, case["rows"] - case["rows_spread"] * i // n) for i in range(n)]
+    return past, rows
+
+
+def _groups(case):
+    """Each group's prefix, and its first sequence (and the end)."""
+    m = case["m"]
+    return ([case["prefix"] - case["prefix_spread"] * g // m for g in range(m)],
+            [case["n"] * g // m for g in range(m + 1)])
+
+
+def _generator(seed):
+    g = torch.Generator(device=_device())
+    g.manual_seed(seed)
+    return g
+
+
+def _normal(g, shape, type):
+    return torch.randn(shape, generator=g, device=g.device, dtype=torch.float32).to(TYPES[type])
+
+
+def _offsets(lengths, dev):
+    return torch.tensor(np.concatenate([[0], np.cumsum(lengths)]), dtype=torch.int32, device=dev)
+
+
+def _prepare_sample(case, g):
+    n, vocab, dev = case["n"], case["vocab"], g.device
+    # a head's logits: most tokens far below the few that come into question,
+    # more sharply in some rows than in others
+    x = torch.randn((n, vocab + case["pad"]), generator=g, device=dev, dtype=torch.float32)
+    sharp = torch.rand((n, 1), generator=g, device=dev) * 4.0 + 1.0
+    s = {"case": case, "logits": x.mul_(sharp).to(TYPES[case["type"]])[:, :vocab],
+         "u": torch.rand(n, generator=g, device=dev), "t": case["t"], "k": case["k"], "p": case["p"], "q": case["q"]}
+    if case["mixed"]:
+        r = torch.rand((5, n), generator=g, device=dev)
+        # every eighth row or so greedy, a third each with a top-k of its own
+        # and without, half with top-p, some with min-p
+        s["t"] = torch.where(r[0] < 0.125, 0.0, case["t"] * (0.5 + r[1]))
+        k = (case["k"] * 2.0 * r[2]).int() + 1
+        s["k"] = torch.where(r[3] < 0.33, 0, k).to(torch.int32)
+        s["p"] = torch.where(r[4] < 0.5, 1.0, 1.0 - (1.0 - case["p"]) * 2.0 * r[1]).clamp(min=0.05)
+        s["q"] = torch.where(r[2] < 0.5, 0.0, case["q"] * r[3])
+    return s
+
+
+def prepare(case, seed):
+    g = _generator(seed)
+    dev = g.device
+    if case["kind"] == "sample":
+        return _prepare_sample(case, g)
+    n, hq, hkv, hd = case["n"], case["hq"], case["hkv"], case["hd"]
+    past, rows = _lengths(case)
+    total = sum(rows)
+    s = {"case": case, "pos": torch.tensor(past, dtype=torch.int32, device=dev), "off": None, "total": total,
+         "past": past, "rows": rows}
+    if case["rows"]:
+        s["off"] = _offsets(rows, dev)
+    if case["kind"] == "rope":
+        # queries and keys as the projection leaves them, next to the values
+        x = _normal(g, (total, hq + 2 * hkv, hd), case["type"])
+        s["q"], s["k"] = x[:, :hq], x[:, hq:hq + hkv]
+        i = torch.arange(case["rot"] // 2, dtype=torch.float64, device=dev)
+        s["freq"] = (10000.0 ** (-2.0 * i / case["rot"])).float()
+        s["gq"] = s["gk"] = None
+        if case["norm"]:
+            s["gq"], s["gk"] = torch.randn((2, hd), generator=g, device=dev) * 0.2
+        return s
+    slots, (plen, goff) = case["slots"], _groups(case)
+    # the sequences, and the prefixes, sit in their caches in any order
+    s["seq"] = torch.randperm(n, generator=g, device=dev).to(torch.int32)
+    s["pseq"] = torch.randperm(case["m"], generator=g, device=dev).to(torch.int32)
+    s["plen"], s["pn"], s["goff"] = torch.tensor(plen, dtype=torch.int32, device=dev), plen, goff
+    s["poff"] = _offsets([sum(rows[a:b]) for a, b in zip(goff, goff[1:])], dev)
+    s["q"] = _normal(g, (total, hq, hd), case["type"])
+    s["sink"] = torch.randn(hq, generator=g, device=dev) if case["sink"] else None
+    s["scale"] = 1.0 / math.sqrt(hd)
+    s["data"] = _filled(g, n, hkv, hd, slots, max(p + r for p, r in zip(past, rows)))
+    s["pdata"] = _filled(g, case["m"], hkv, hd, case["prefix"], case["prefix"])
+    if own:
+        from ana_amd import ops
+        s["cache"], s["pre"] = ops.KV4(s["data"], slots), ops.KV4(s["pdata"], case["prefix"])
+    return s
+
+
+def _filled(g, n, hkv, hd, slots, live):
+    """A cache whose live slots hold keys and values as a model makes them."""
+    data = torch.zeros((n, hkv, -(-slots // 32), 34 * hd), dtype=torch.uint8, device=g.device)
+    tiles = -(-min(slots, live) // 32)
+    for i in range(n):
+        k = torch.randn((hkv, tiles * 32, hd), generator=g, device=g.device)
+        v = torch.randn((hkv, tiles * 32, hd), generator=g, device=g.device)
+        _put(data[i], k, v)
+    return data
+
+
+# ---------------------------------------------------------------- the plain form
+
+def _codes(x):
+    """Blocks of 32 values [..., 32] as codes 0 .. 15 and a scale byte each."""
+    a = x.abs().amax(-1)
+    bits = a.view(torch.int32)
+    e = ((bits >> 23) - 2 + ((bits & 0x7FFFFF) > 0x600000).to(torch.int32)).clamp(2, 252)
+    m = (x * ((254 - e) << 23).view(torch.float32).unsqueeze(-1)).abs()
+    # a tie goes to the even code: the borders 0.25, 1.25, 2.5 and 5 stay below
+    c = ((m > 0.25).to(torch.uint8) + (m >= 0.75).to(torch.uint8) + (m > 1.25).to(torch.uint8)
+         + (m >= 1.75).to(torch.uint8) + (m > 2.5).to(torch.uint8) + (m >= 3.5).to(torch.uint8)
+         + (m > 5.0).to(torch.uint8))
+    return c + (torch.signbit(x).to(torch.uint8) << 3), e.to(torch.uint8)
+
+
+def _pairs(c):
+    """Codes packed two a byte, the first in the low half."""
+    return c[..., 0::2] | (c[..., 1::2] << 4)
+
+
+def _parts(data):
+    """The four parts of a cache's records as views [..., their extents]."""
+    hd = data.shape[-1] // 34
+    return (data[..., :16 * hd].unflatten(-1, (4, 16, 2, hd // 8)),
+            data[..., 16 * hd:32 * hd].unflatten(-1, (4, 16, 2, 4, hd // 32)),
+            data[..., 32 * hd:33 * hd].unflatten(-1, (hd // 32, 16, 2)),
+            data[..., 33 * hd:].unflatten(-1, (hd // 32, 4, 2, 4))), data.shape[:-1], hd
+
+
+def _put(data, k, v):
+    """k and v [hkv, slots, hd] from slot 0 of one sequence's records (whole
+    tiles of 32 slots)."""
+    tiles = k.shape[1] // 32
+    (ko, vo, ks, vs), _, hd = _parts(data[:, :tiles])
+    h = k.shape[0]
+    ck, ek = _codes(k.view(h, tiles, 32, hd // 32, 32))
+    cv, ev = _codes(v.view(h, tiles, 32, hd // 32, 32))
+    # slot 16 h + m, dim j hd / 4 + ...
+    ko.copy_(_pairs(ck.reshape(h, tiles, 2, 16, 4, hd // 4)).permute(0, 1, 4, 3, 2, 5))
+    # slot 16 x + 4 j + y, dim m hd / 16 + ...
+    vo.copy_(_pairs(cv.reshape(h, tiles, 2, 4, 4, 16, hd // 16)).permute(0, 1, 3, 5, 2, 4, 6))
+    ks.copy_(ek.view(h, tiles, 2, 16, hd // 32).permute(0, 1, 4, 3, 2))
+    vs.copy_(ev.view(h, tiles, 2, 4, 4, hd // 32).permute(0, 1, 5, 3, 2, 4))
+
+
+_LEVELS = [0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0]
+
+
+def _values(codes, scales, table):
+    """Bytes [..., 16] of blocks and their scale bytes [...] as values [..., 32]."""
+    x = torch.stack([table[(codes & 15).int()], table[(codes >> 4).int()]], -1).flatten(-2)
+    return x * (scales.int() << 23).view(torch.float32).unsqueeze(-1)
+
+
+def _unpack(data):
+    """The keys and values [..., slots, hd] of records [..., tiles, 34 hd]."""
+    (ko, vo, ks, vs), lead, hd = _parts(data)
+    t = torch.tensor(_LEVELS + [-x for x in _LEVELS], dtype=torch.float32, device=data.device)
+    nd = len(lead)
+    a = list(range(nd))
+    kc = ko.permute(*a, nd + 2, nd + 1, nd, nd + 3).reshape(*lead, 32, hd // 32, 16)
+    vc = vo.permute(*a, nd + 2, nd, nd + 3, nd + 1, nd + 4).reshape(*lead, 32, hd // 32, 16)
+    kc = _values(kc, ks.permute(*a, nd + 2, nd + 1, nd).reshape(*lead, 32, hd // 32), t)
+    vc = _values(vc, vs.permute(*a, nd + 2, nd + 1, nd + 3, nd).reshape(*lead, 32, hd // 32), t)
+    flat = (*lead[:-1], lead[-1] * 32, hd)
+    return kc.reshape(flat), vc.reshape(flat)
+
+
+def _turned(x, gain, cos, sin, case):
+    """Rows of heads, normed and turned: cos and sin [rows, 1, rot / 2]."""
+    y = x.float()
+    if gain is not None:
+        y = y * torch.rsqrt((y * y).mean(-1, keepdim=True) + EPS) * (1.0 + gain)
+    r = case["rot"]
+    if case["near"]:
+        a, b = y[..., 0:r:2], y[..., 1:r:2]
+        t = torch.stack([a * cos - b * sin, b * cos + a * sin], -1).flatten(-2)
+    else:
+        a, b = y[..., :r // 2], y[..., r // 2:r]
+        t = torch.cat([a * cos - b * sin, b * cos + a * sin], -1)
+    return torch.cat([t, y[..., r:]], -1).to(x.dtype)
+
+
+def _plain_rope(s):
+    case, pos = s["case"], s["pos"].long()
+    if s["off"] is not None:
+        i = torch.repeat_interleave(torch.arange(case["n"], device=pos.device), s["off"].diff(),
+                                    output_size=s["total"])
+        pos = pos[i] + torch.arange(s["total"], device=pos.device) - s["off"].long()[i]
+    angle = pos.double()[:, None, None] * s["freq"].double()
+    cos, sin = torch.cos(angle).float(), torch.sin(angle).float()
+    return _turned(s["q"], s["gq"], cos, sin, case), _turned(s["k"], s["gk"], cos, sin, case)
+
+
+def _join(scores, values, sink):
+    """One softmax over several sets of scores [..., r, slots] (-inf where
+    they do not count), each with its values [..., slots, hd]; sink [..., 1]."""
+    top = scores[0].amax(-1, keepdim=True)
+    for sc in scores[1:]:
+        top = torch.maximum(top, sc.amax(-1, keepdim=True))
+    if sink is not None:
+        top = torch.maximum(top, sink)
+    den = 0.0 if sink is None else torch.exp(sink - top)
+    o = 0.0
+    for sc, v in zip(scores, values):
+        e = torch.exp(sc - top)
+        den = den + e.sum(-1, keepdim=True)
+        o = o + torch.matmul(e, v)
+    return o / den
+
+
+def _plain_shared(s):
+    case = s["case"]
+    n, hq, hkv, hd, slots = case["n"], case["hq"], case["hkv"], case["hd"], case["slots"]
+    G = hq // hkv
+    q, data = s["q"].float() * s["scale"], s["data"]
+    out, r0 = torch.empty_like(s["q"]), 0
+    for g in range(case["m"]):
+        i0, i1 = s["goff"][g], s["goff"][g + 1]
+        T = sum(s["rows"][i0:i1])
+        pk, pv = _unpack(s["pdata"].index_select(0, s["pseq"][g:g + 1].long())[0])
+        pk, pv = pk[:, :s["pn"][g]], pv[:, :s["pn"][g]]
+        qg = q[r0:r0 + T].view(T, hkv, G, hd).transpose(0, 1).reshape(hkv, T * G, hd)
+        far = torch.matmul(qg, pk.transpose(-1, -2))
+        sink = None if s["sink"] is None else s["sink"].view(hkv, 1, G).expand(hkv, T, G).reshape(hkv, T * G, 1)
+        if s["off"] is None:
+            # every sequence's own tokens at once, over as many slots as the
+            # longest has live
+            live = min(slots, max(s["past"][i0:i1]) + 1)
+            k, v = _unpack(data[:, :, :-(-live // 32)][s["seq"][i0:i1].long()])
+            near = torch.matmul(qg.view(hkv, T, G, hd).transpose(0, 1), k.transpose(-1, -2))
+            at = torch.arange(near.shape[-1], device=q.device)
+            seen = at < torch.clamp(s["pos"][i0:i1].long() + 1, max=slots).view(T, 1, 1, 1)
+            near = torch.where(seen, near, -math.inf)
+            # (the prefix's sums for all rows, the own ones row by row)
+            top = torch.maximum(far.amax(-1, keepdim=True),
+                                near.amax(-1, keepdim=True).transpose(0, 1).reshape(hkv, T * G, 1))
+            if sink is not None:
+                top = torch.maximum(top, sink)
+            e = torch.exp(far - top)
+            f = torch.exp(near - top.view(hkv, T, G, 1).transpose(0, 1))
+            den = e.sum(-1, keepdim=True) + f.sum(-1, keepdim=True).transpose(0, 1).reshape(hkv, T * G, 1)
+            if sink is not None:
+                den = den + torch.exp(sink - top)
+            o = torch.matmul(e, pv) + torch.matmul(f, v).transpose(0, 1).reshape(hkv, T * G, hd)
+            out[r0:r0 + T] = (o / den).view(hkv, T, G, hd).transpose(0, 1).reshape(T, hq, hd).to(out.dtype)
+        else:
+            a0 = 0
+            for i in range(i0, i1):
+                t, last = s["rows"][i], s["past"][i] + s["rows"][i] - 1
+                live = min(slots, last + 1)
+                k, v = _unpack(data[:, :, :-(-live // 32)].index_select(0, s["seq"][i:i + 1].long())[0])
+                near = torch.matmul(qg[:, a0 * G:(a0 + t) * G], k.transpose(-1, -2))
+                at = torch.arange(near.shape[-1], device=q.device)
+                at = torch.where(at < slots, last - (last - at) % slots, -1)     # the position a slot holds
+                p = s["past"][i] + torch.arange(t, device=q.device).repeat_interleave(G)
+                near = torch.where((at >= 0) & (at <= p[:, None]), near, -math.inf)
+                w = slice(a0 * G, (a0 + t) * G)
+                o = _join([far[:, w], near], [pv, v], None if sink is None else sink[:, w])
+                out[r0 + a0:r0 + a0 + t] = o.view(hkv, t, G, hd).transpose(0, 1).reshape(t, hq, hd).to(out.dtype)
+                a0 += t
+        r0 += T
+    return out
+
+
+def _settings(s, lo, hi, dev):
+    """Temperature, top-k, top-p and min-p of rows lo .. hi - 1, [rows, 1]
+    each, in 64 bits."""
+    out = []
+    for key in "tkpq":
+        x = s[key]
+        if torch.is_tensor(x):
+            x = x[lo:hi].unsqueeze(-1)
+        else:
+            # (a program's number goes to the kernels as a float)
+            x = torch.full((hi - lo, 1), float(np.float32(x)), device=dev)
+        out.append(x.double())
+    return out
+
+
+def _plain_sample(s):
+    # in 64 bits throughout: a token is a whole number, and whether a mass
+    # passes its border decides it
+    case, dev = s["case"], s["logits"].device
+    n, vocab = case["n"], case["vocab"]
+    tokens = torch.empty(n, dtype=torch.int32, device=dev)
+    lp = torch.empty(n, dtype=torch.float32, device=dev)
+    at = torch.arange(vocab, device=dev)
+    step = max(1, 30000000 // vocab)
+    for lo in range(0, n, step):
+        hi = min(n, lo + step)
+        x = s["logits"][lo:hi].double()
+        t, k, p, q = _settings(s, lo, hi, dev)
+        greedy = t <= 0.0
+        k = torch.where(greedy, 1.0, torch.where((k < 1.0) | (k > vocab), float(vocab), k))
+        x, place = torch.sort(x, dim=-1, descending=True, stable=True)
+        z = (x - x[:, :1]) / torch.where(greedy, 1.0, t)
+        w = torch.where(at < k, torch.exp(z), 0.0)
+        mass = torch.cumsum(w, -1)
+        keep = (mass - w < p * mass[:, -1:]) | (p >= 1.0)
+        keep[:, 0] = True
+        w = torch.where(keep & (w >= q), w, 0.0)
+        # back to the order of the indices
+        w = torch.zeros_like(w).scatter_(1, place, w)
+        mass = torch.cumsum(w, -1)
+        target = s["u"][lo:hi].double().unsqueeze(-1) * mass[:, -1:]
+        i = (mass <= target).sum(-1, keepdim=True).clamp(max=vocab - 1)
+        tokens[lo:hi] = i.squeeze(-1).to(torch.int32)
+        lp[lo:hi] = (torch.log(torch.gather(w, 1, i)) - torch.log(mass[:, -1:])).squeeze(-1).float()
+    return tokens, lp
+
+
+def run(s):
+    case = s["case"]
+    if not own:
+        return {"rope": _plain_rope, "shared": _plain_shared, "sample": _plain_sample}[case["kind"]](s)
+    from ana_amd import ops
+    if case["kind"] == "rope":
+        return ops.qk_rope(s["q"], s["k"], s["pos"], s["freq"], off=s["off"], gq=s["gq"], gk=s["gk"], eps=EPS,
+                           near=case["near"])
+    if case["kind"] == "shared":
+        return ops.kv4_attend_shared(s["q"], s["cache"], s["pos"], s["pre"], s["plen"], pseq=s["pseq"], poff=s["poff"],
+                                     seq=s["seq"], off=s["off"], sink=s["sink"], scale=s["scale"])
+    return ops.sample(s["logits"], s["u"], temperature=s["t"], top_k=s["k"], top_p=s["p"], min_p=s["q"])
+
+
+# ---------------------------------------------------------------- what a pass cannot do without
+
+def work(case):
+    b = BYTES[case["type"]]
+    if case["kind"] == "sample":
+        n, v = case["n"], case["vocab"]
+        # the maximum, an exponential and a sum a logit
+        return {"bytes": n * (v * b + 12.0), "flops": 4.0 * n * v}
+    past, rows = _lengths(case)
+    total, hd, hkv, hq = sum(rows), case["hd"], case["hkv"], case["hq"]
+    if case["kind"] == "rope":
+        one = float(total) * (hq + hkv) * hd
+        return {"bytes": 2.0 * one * b, "flops": one * (7.0 if case["norm"] else 3.0)}
+    code = 34.0 / 32.0 * hd * hkv              # a position's keys and values in the cache
+    plen, goff = _groups(case)
+    by, fl = 2.0 * total * hq * hd * b, 0.0
+    for g, pn in enumerate(plen):
+        by += code * pn
+        fl += 4.0 * hq * hd * pn * sum(rows[goff[g]:goff[g + 1]])
+    for p, r in zip(past, rows):
+        last = p + r - 1
+        by += code * min(case["slots"], last + 1)
+        # a row sees the positions up to its own that the ring still holds
+        first = max(0, last + 1 - case["slots"])
+        fl += 4.0 * hq * hd * sum(range(p + 1 - first, last + 2 - first))
+    return {"bytes": by, "flops": fl}
+
+
+# ---------------------------------------------------------------- in 64 bits
+
+def _record_bytes(hd, dev):
+    """Where in a record each slot's and dimension's key and value codes are
+    (the byte, the bits' shift) and their blocks' scales."""
+    s, d = np.meshgrid(np.arange(32), np.arange(hd), indexing="ij")
+    j, h, m = d // (hd // 4), s // 16, s % 16
+    key = ((j * 16 + m) * 2 + h) * (hd // 8) + d % (hd // 4) // 2
+    jv, ev, mv = s % 16 // 4, s // 16 * 4 + s % 4, d // (hd // 16)
+    val = 16 * hd + ((jv * 16 + mv) * 8 + ev) * (hd // 32) + d % (hd // 16) // 2
+    ks = 32 * hd + (d // 32 * 16 + m) * 2 + h
+    vs = 33 * hd + (d // 32 * 4 + jv) * 8 + ev
+    return [torch.from_numpy(a.reshape(-1)).to(dev) for a in (key, val, ks, vs, d % 2 * 4)]
+
+
+def _read64(rec, at, count):
+    """Records [tiles, 34 hd] as `count` keys and values [count, hd] in 64 bits."""
+    key, val, ks, vs, shift = at
+    levels = torch.tensor(_LEVELS + [-x for x in _LEVELS], dtype=torch.float64, device=rec.device)
+    two = torch.exp2(torch.arange(256, dtype=torch.float64, device=rec.device) - 127.0)
+    hd = rec.shape[-1] // 34
+    return [(levels[(rec[:, c].long() >> shift) & 15] * two[rec[:, b].long()]).view(-1, hd)[:count]
+            for c, b in ((key, ks), (val, vs))]
+
+
+def _shared64(case, s):
+    hq, hkv, hd, slots = case["hq"], case["hkv"], case["hd"], case["slots"]
+    G, dev = hq // hkv, s["q"].device
+    at = _record_bytes(hd, dev)
+    first = np.concatenate([[0], np.cumsum(s["rows"])])
+    out = torch.empty((s["total"], hq, hd), dtype=torch.float64, device=dev)
+    for g in range(case["m"]):
+        for h in range(hkv):
+            pk, pv = _read64(s["pdata"][int(s["pseq"][g]), h], at, s["pn"][g])
+            pk = pk.t().contiguous()
+            for i in range(s["goff"][g], s["goff"][g + 1]):
+                T, last = s["rows"][i], s["past"][i] + s["rows"][i] - 1
+                live = min(slots, last + 1)
+                k, v = _read64(s["data"][int(s["seq"][i]), h, :-(-live // 32)], at, live)
+                idx = torch.arange(live, device=dev)
+                turn = last // slots * slots
+                pos = torch.where(idx <= last - turn, turn + idx, turn - slots + idx)
+                hide = (pos[None, :] > (s["past"][i] + torch.arange(T, device=dev))[:, None]).repeat_interleave(G, 0)
+                r = slice(int(first[i]), int(first[i]) + T)
+                x = s["q"][r, h * G:(h + 1) * G].double().reshape(T * G, hd)
+                sc = [x @ pk * s["scale"], (x @ k.t().contiguous() * s["scale"]).masked_fill(hide, -math.inf)]
+                if s["sink"] is not None:
+                    sc.append(s["sink"][h * G:(h + 1) * G].double().repeat(T).unsqueeze(-1))
+                w = torch.softmax(torch.cat(sc, -1), -1)
+                pn = s["pn"][g]
+                out[r, h * G:(h + 1) * G] = (w[:, :pn] @ pv + w[:, pn:pn + live] @ v).view(T, G, hd)
+    return out
+
+
+def _rope64(case, s):
+    pos = np.concatenate([p + np.arange(r) for p, r in zip(s["past"], s["rows"])])
+    dev = s["q"].device
+    turns = torch.tensor(pos, dtype=torch.float64, device=dev)[:, None] * s["freq"].double()
+    wave = torch.polar(torch.ones_like(turns), turns).unsqueeze(1)
+    r = case["rot"]
+    out = []
+    for x, gain in ((s["q"], s["gq"]), (s["k"], s["gk"])):
+        y = x.double()
+        if gain is not None:
+            y = y / torch.sqrt(y.square().sum(-1, keepdim=True) / case["hd"] + EPS) * (1.0 + gain.double())
+        y = y.clone()
+        a, b = (slice(0, r, 2), slice(1, r, 2)) if case["near"] else (slice(0, r // 2), slice(r // 2, r))
+        c = torch.complex(y[..., a].clone(), y[..., b].clone()) * wave
+        y[..., a], y[..., b] = c.real, c.imag
+        out.append(y)
+    return tuple(out)
+
+
+def _sample64(case, s):
+    """Row by row: the kept set from the sorted values, the walk through it."""
+    n, vocab = case["n"], case["vocab"]
+    x = s["logits"].double()
+    u, tokens, lp = s["u"].double().tolist(), [], []
+    t, k, p, q = ([float(v) for v in (s[a].double().tolist() if torch.is_tensor(s[a]) else [np.float32(s[a])] * n)]
+                  for a in "tkpq")
+    for r in range(n):
+        row = x[r]
+        if t[r] <= 0.0 or k[r] == 1.0:
+            tokens.append(int((row == row.max()).nonzero()[0]))
+            lp.append(0.0)
+            continue
+        # the first places in the order of value, then index
+        v, i = torch.sort(-row, stable=True)
+        cnt = int(k[r]) if 0 < k[r] < vocab else vocab
+        w = torch.exp((v[0] - v[:cnt]) / t[r])
+        if p[r] < 1.0:
+            # the least count whose mass reaches p of all
+            c = torch.cumsum(w, 0)
+            cnt = min(cnt, int(torch.searchsorted(c, p[r] * c[-1:])) + 1)
+        w = w[:cnt]
+        w = w[w >= q[r]]
+        i, back = torch.sort(i[:len(w)])
+        c = torch.cumsum(w[back], 0)
+        at = min(int(torch.searchsorted(c, u[r] * c[-1:], right=True)), len(w) - 1)
+        tokens.append(int(i[at]))
+        lp.append(float(torch.log(w[back][at] / c[-1])))
+    dev = x.device
+    return torch.tensor(tokens, dtype=torch.int32, device=dev), torch.tensor(lp, dtype=torch.float64, device=dev)
+
+
+def exact(case, seed):
+    s = prepare(case, seed)
+    return {"rope": _rope64, "shared": _shared64, "sample": _sample64}[case["kind"]](case, s)
