@@ -10,7 +10,8 @@ Three kinds of case, one operator's pass each:
 - "shared": softmax attention of query rows over a 4-bit cache, where groups
   of rows also see one long prefix that they have in common. kv4_attend_shared.
 - "sample": a token of each row of logits from a given random number, with a
-  temperature, top-k, top-p and min-p. sample.
+  temperature, top-k, top-p and min-p: the one at which the running mass,
+  likeliest tokens first, passes that share of what is kept. sample.
 
 A case is a dict of plain values. For "rope" and "shared":
 
@@ -458,12 +459,10 @@ def _plain_sample(s):
         keep = (mass - w < p * mass[:, -1:]) | (p >= 1.0)
         keep[:, 0] = True
         w = torch.where(keep & (w >= q), w, 0.0)
-        # back to the order of the indices
-        w = torch.zeros_like(w).scatter_(1, place, w)
         mass = torch.cumsum(w, -1)
         target = s["u"][lo:hi].double().unsqueeze(-1) * mass[:, -1:]
-        i = (mass <= target).sum(-1, keepdim=True).clamp(max=vocab - 1)
-        tokens[lo:hi] = i.squeeze(-1).to(torch.int32)
+        i = torch.minimum((mass <= target).sum(-1, keepdim=True), (w > 0.0).sum(-1, keepdim=True) - 1)
+        tokens[lo:hi] = torch.gather(place, 1, i).squeeze(-1).to(torch.int32)
         lp[lo:hi] = (torch.log(torch.gather(w, 1, i)) - torch.log(mass[:, -1:])).squeeze(-1).float()
     return tokens, lp
 
@@ -584,7 +583,7 @@ def _rope64(case, s):
 
 
 def _sample64(case, s):
-    """Row by row: the kept set from the sorted values, the walk through it."""
+    """Row by row: the kept places of the sorted values, the walk along them."""
     n, vocab = case["n"], case["vocab"]
     x = s["logits"].double()
     u, tokens, lp = s["u"].double().tolist(), [], []
@@ -606,11 +605,10 @@ def _sample64(case, s):
             cnt = min(cnt, int(torch.searchsorted(c, p[r] * c[-1:])) + 1)
         w = w[:cnt]
         w = w[w >= q[r]]
-        i, back = torch.sort(i[:len(w)])
-        c = torch.cumsum(w[back], 0)
+        c = torch.cumsum(w, 0)
         at = min(int(torch.searchsorted(c, u[r] * c[-1:], right=True)), len(w) - 1)
         tokens.append(int(i[at]))
-        lp.append(float(torch.log(w[back][at] / c[-1])))
+        lp.append(float(torch.log(w[at] / c[-1])))
     dev = x.device
     return torch.tensor(tokens, dtype=torch.int32, device=dev), torch.tensor(lp, dtype=torch.float64, device=dev)
 
