@@ -96,6 +96,15 @@ SIGNATURES = {
     "ana_kv4_attend": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_uint32, C.c_float, C.c_void_p,
                                  C.c_void_p, C.c_uint64, C.c_void_p, C.c_uint64, C.c_void_p]),
     "ana_kv4_attend_ws": (C.c_uint64, [C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint64]),
+    "ana_kv4_attend_shared": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_uint32,
+                                        C.c_float, C.c_void_p, C.c_void_p, C.c_uint64, C.c_uint64, C.c_void_p,
+                                        C.c_uint64, C.c_void_p]),
+    "ana_kv4_attend_shared_ws": (C.c_uint64, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint32, C.c_uint64,
+                                              C.c_uint64]),
+    "ana_qk_rope": (C.c_int, [C.c_int, C.c_uint32, C.c_void_p, C.c_int, C.c_void_p, C.c_uint32, C.c_void_p, C.c_void_p,
+                              C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "ana_row_sample": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p]),
     "ana_row_logprobs": (C.c_int, [C.c_int, C.c_int, C.c_void_p, C.c_uint64, C.c_uint32, C.c_uint32, C.c_void_p,
                                    C.c_uint32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
                                    C.c_void_p, C.c_uint64, C.c_void_p]),

@@ -16,7 +16,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libana.so")
 SOURCES = ["ana.hip", "kernels_exact.hip", "kernels_fast.hip", "gemm_wide.hip", "gemm_split.hip", "attn_rows.hip", "gemm_rows.hip", "sampler.hip", "decode_persist.hip",
-           "kv4.hip", "logprobs.hip", "device_ops.hip",
+           "kv4.hip", "rope.hip", "logprobs.hip", "sample.hip", "device_ops.hip",
            "ftc2.cpp", "bpe.cpp"]
 OBJDIR = os.path.join(HERE, "_build")
 

@@ -67,6 +67,10 @@ struct Kv4Attend {
   const float* sink;   // [hq] or nullptr
   float* part;         // partials [rows][hq][nsplit][kKv4PartHead + hd], when nsplit > 1
   uint32_t nsplit;     // pieces that a sequence's slots are cut into at most
+  // (set by the launches) a pair's places in `part`, the first of this kernel's
+  // pieces, and whether pieces go there even where there is only one
+  uint32_t nz, z0;
+  bool raw;
 };
 // the pieces of a call (live: the most positions a sequence holds after it,
 // as far as the caller knows; 0: the ring's slots), and the floats of
@@ -78,5 +82,14 @@ inline uint64_t kv4_part_floats(uint32_t rows, uint32_t hq, uint32_t hd, uint32_
   return nsplit > 1 ? (uint64_t)rows * hq * nsplit * (kKv4PartHead + hd) : 0;
 }
 hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st);
+
+// Attention where groups of rows also see a prefix that they share: group i of
+// pre has rows off[i] .. off[i + 1] - 1 (off NULL: one group, of all rows), and
+// they see the first pos[i] positions of its place in pc, as far as that ring
+// holds them. part: kv4_part_floats of nsplit + psplit pieces.
+uint64_t kv4_prefix_groups(uint32_t heads, uint32_t n, uint32_t rows, uint32_t hq);
+uint32_t kv4_prefix_split(const Kv4& pc, uint32_t n, uint32_t rows, uint32_t hq, uint64_t live);
+hipError_t launch_kv4_attend_shared(const Kv4Attend& a, const Kv4& pc, const Kv4Rows& pre, uint32_t psplit, int type,
+                                    hipStream_t st);
 
 }  // namespace ana

@@ -6,6 +6,7 @@
 
 #include "kv4.h"
 #include "mfma.h"
+#include "rows.h"
 #include "wave.h"
 
 namespace ana {
@@ -55,22 +56,6 @@ __device__ __forceinline__ void store8(T* p, bool vec, const float (&x)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; e++) p[e] = (T)x[e];
   }
-}
-
-// the last i < n with off[i] <= r (0 when there is none), for the whole wave:
-// 64 of the remaining places at a time
-__device__ __forceinline__ uint32_t find_seq(const uint32_t* off, uint32_t n, uint32_t r) {
-  const uint32_t lane = threadIdx.x & 63;
-  uint32_t lo = 0, cnt = n;
-  while (cnt > 1) {
-    const uint32_t step = (cnt + 63) / 64, k = lane * step;
-    const bool t = k < cnt && off[lo + k] <= r;
-    const uint32_t c = __popcll(__ballot(t));
-    if (c == 0) break;
-    lo += (c - 1) * step;
-    cnt = min(step, cnt - (c - 1) * step);
-  }
-  return lo;
 }
 
 // whether a sequence has a place in the cache, and positions below 2^31 (so
@@ -449,6 +434,8 @@ __device__ __forceinline__ uint32_t piece_tiles(uint32_t tiles, uint32_t nsplit,
   const uint32_t n = max(1u, min(nsplit, tiles / least));
   return (tiles + n - 1) / n;
 }
+// (none of no tiles, for which there is still one workgroup)
+__device__ __forceinline__ uint32_t pieces_of(uint32_t tiles, uint32_t per) { return tiles ? (tiles + per - 1) / per : 0u; }
 // A running maximum is only raised once a score passes it by this much (in
 // base 2): probabilities then reach 2^kSlack, which costs f32 and bf16 no
 // digit, and most tiles rescale nothing.
@@ -594,7 +581,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few
   const uint32_t per = piece_tiles(tiles, a.nsplit, kFewTiles);
   const uint32_t t0 = z * per, t1 = min(tiles, t0 + per);
   if (z && t0 >= t1) return;
-  const bool split = tiles > per;
+  const bool split = a.raw || tiles > per;
   const uint32_t pm = m / NC, part = m % NC;
   const uint32_t t = (c0 + pm) / G, g = (c0 + pm) % G;
   const float sc = a.scale * kLog2e;
@@ -789,9 +776,9 @@ __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few
       y += v * f;
     }
     const uint32_t row = row0 + (c0 + pp) / G, hd = head * G + (c0 + pp) % G;
-    float* out = a.part + (((uint64_t)row * a.hq + hd) * a.nsplit + z) * (D + kPartHead);
-    if (a.nsplit > 1 && d == 0) {
-      if (z == 0) out[2] = __builtin_bit_cast(float, split ? (tiles + per - 1) / per : kDone);
+    float* out = a.part + (((uint64_t)row * a.hq + hd) * a.nz + z) * (D + kPartHead);
+    if (a.nz > 1 && d == 0) {
+      if (z == 0) out[2] = __builtin_bit_cast(float, split ? pieces_of(tiles, per) : kDone);
       out[0] = M;
       out[1] = lsum;
     }
@@ -829,7 +816,11 @@ struct Many {
   static constexpr uint32_t pairs = 64 * NQ;
 };
 
-template <typename T, int D>
+//
+// PRE: the sequences are groups of rows, and what they see is a prefix that
+// they share: the first pos[i] positions of the group's place, all of them for
+// every row. Groups of any size are taken.
+template <typename T, int D, bool PRE>
 __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend a, uint32_t vec) {
   constexpr int NP = Parts<T>::q, NPP = Many<T, D>::NPP, NQ = Many<T, D>::NQ;
   constexpr uint32_t PW = Many<T, D>::pairs;
@@ -852,9 +843,9 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
   for (uint32_t b = 0; b < a.r.n && !found; b += 64) {
     uint32_t nt = 0;
     if (b + lane < a.r.n) {
-      const uint32_t o0 = a.r.off[b + lane], o1 = a.r.off[b + lane + 1];
+      const uint32_t o0 = PRE && !a.r.off ? 0 : a.r.off[b + lane], o1 = PRE && !a.r.off ? a.r.rows : a.r.off[b + lane + 1];
       const uint32_t pairs = o1 > o0 && o1 <= a.r.rows ? (o1 - o0) * G : 0;
-      nt = pairs > kFewPairs ? (pairs + PW - 1) / PW : 0;
+      nt = PRE || pairs > kFewPairs ? (pairs + PW - 1) / PW : 0;
     }
     uint32_t sum = nt;
 #pragma unroll 1
@@ -876,22 +867,22 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
   if (!found) return;
   i = __builtin_amdgcn_readfirstlane(i);
   part_i = __builtin_amdgcn_readfirstlane(part_i);
-  const uint32_t row0 = a.r.off[i], len = a.r.off[i + 1] - row0;
+  const uint32_t row0 = PRE && !a.r.off ? 0 : a.r.off[i], len = (PRE && !a.r.off ? a.r.rows : a.r.off[i + 1]) - row0;
   const uint32_t q = a.r.seq ? a.r.seq[i] : i;
-  const uint32_t pos = a.r.pos[i], last = pos + len - 1;
-  const bool ok = has_place(a.c, q, pos);
+  const uint32_t pos = a.r.pos[i], last = PRE ? max(pos, 1u) - 1 : pos + len - 1;
+  const bool ok = has_place(a.c, q, pos) && !(PRE && pos == 0);
   const uint32_t all = len * G, c0 = part_i * PW;   // (rows x query heads < 2^31)
   const View view(last, a.c.slots);
   const uint32_t t_lo = c0 / G, t_hi = (min(all, c0 + PW) - 1) / G;
   // before the ring wraps, slots past the last row's position hold nothing
   // that any of the pairs sees
-  const bool flat = last < a.c.slots;
+  const bool flat = !PRE && last < a.c.slots;
   const uint32_t seen = flat ? pos + t_hi + 1 : view.live;
   const uint32_t tiles = ok ? (seen + 31) / 32 : 0u;
   const uint32_t per = piece_tiles(tiles, a.nsplit, kManyTiles);
   const uint32_t t0 = z * per, t1 = min(tiles, t0 + per);
   if (z && t0 >= t1) return;
-  const bool split = tiles > per;
+  const bool split = a.raw || tiles > per;
 
   const uint8_t* base = record_of(a.c, ok ? q : 0, head, 0);
   // a wave's part of a record: the key codes of slots m and 16 + m, or the
@@ -946,7 +937,7 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
     const uint32_t c = c0 + (wv * NQ + n) * 16 + m;
     const bool on = c < all;
     const uint32_t t = on ? c / G : t_lo, g = on ? c % G : 0;
-    ago[n] = len - 1 - t;
+    ago[n] = PRE ? 0 : len - 1 - t;
     query_ops<T, D, NP>(a.q, row0 + t, head * G + g, j, on, vec, query_factor<T>(sc), qo[n]);
   }
   // the last slot that a pair of this wave sees, where the ring has not wrapped
@@ -973,8 +964,8 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
     const bool more = tile + 1 < t1;
     if (more) load(tile + 1);
     // (past every position of the wave's pairs: nothing to do)
-    if (!flat || tile * 32 <= wave_hi) {
-      const bool whole = view.whole(tile, len - 1 - t_lo);
+    if (PRE ? w0 < all : !flat || tile * 32 <= wave_hi) {
+      const bool whole = view.whole(tile, PRE ? 0 : len - 1 - t_lo);
       const bool bad_k = flag[buf][0] | flag[buf][1], bad = flag[buf][2] | flag[buf][3];
       // (f32 scores come out less their pair's maximum: the products start from it)
       f32x4_t s[NQ][2];
@@ -1091,13 +1082,13 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
     const uint32_t c = c0 + (wv * NQ + n) * 16 + m;
     const bool on = c < all;
     const uint32_t row = on ? row0 + c / G : row0, hq = on ? head * G + c % G : 0;
-    float* part = a.part + (((uint64_t)row * a.hq + hq) * a.nsplit + z) * (D + kPartHead);
+    float* part = a.part + (((uint64_t)row * a.hq + hq) * a.nz + a.z0 + z) * (D + kPartHead);
     if (!split) {
       const float den = finish_sum(mx[n], ls, a.sink, hq, &f);
       inv = ok && den != 0.0f ? f / den : 0.0f;
     }
-    if (a.nsplit > 1 && on && j == 0) {
-      if (z == 0) part[2] = __builtin_bit_cast(float, split ? (tiles + per - 1) / per : kDone);
+    if (a.nz > 1 && on && j == 0) {
+      if (z == 0) part[2] = __builtin_bit_cast(float, split ? pieces_of(tiles, per) : kDone);
       part[0] = mx[n];
       part[1] = ls;
     }
@@ -1132,28 +1123,40 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
 
 // The pieces of a (row, query head), a wave each: weights 2^(m_z - M), then
 // the sink, then the division. D / 4 lanes take a piece's outputs, so several
-// pieces are in flight at once.
-template <typename T, int D>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a) {
+// pieces are in flight at once. PRE: the pieces of the row's own positions,
+// then (from nsplit on) those of the prefix that its group in `pre` shares.
+template <typename T, int D, bool PRE>
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a, Kv4Rows pre) {
   constexpr uint32_t L = D / 4, GR = 64 / L;   // lanes a piece, pieces at once
   const uint32_t lane = threadIdx.x & 63;
   const uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const uint32_t row = (uint32_t)(w / a.hq), hd = (uint32_t)(w % a.hq);
   if (row >= a.r.rows) return;
-  const float* part = a.part + ((uint64_t)row * a.hq + hd) * a.nsplit * (D + kPartHead);
-  const uint32_t nz = __builtin_bit_cast(uint32_t, part[2]);
+  const float* part = a.part + ((uint64_t)row * a.hq + hd) * a.nz * (D + kPartHead);
+  uint32_t nz = __builtin_bit_cast(uint32_t, part[2]);
   // (a row that no sequence has: its words are whatever they are)
   if (a.r.off && (row < a.r.off[0] || row >= a.r.off[a.r.n])) return;
   if (nz > a.nsplit) return;
+  const uint32_t own = nz;
+  if constexpr (PRE) {
+    bool has = pre.n != 0;
+    if (has && pre.off) {
+      const uint32_t g = find_seq(pre.off, pre.n, row);
+      has = row >= pre.off[g] && row < pre.off[g + 1] && pre.off[g + 1] <= a.r.rows;
+    }
+    if (has && nz) nz += min(__builtin_bit_cast(uint32_t, part[a.nsplit * (D + kPartHead) + 2]), a.nz - a.nsplit);
+  }
+  // where piece z is (the own pieces may be fewer than their places)
+  auto piece = [&](uint32_t z) { return part + (PRE && z >= own ? z - own + a.nsplit : z) * (D + kPartHead); };
   float M = -INFINITY;
-  for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, part[z * (D + kPartHead)]);
+  for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, piece(z)[0]);
   M = wmax(M);
   const uint32_t g = lane / L, d = lane % L * 4;
   float l = 0.0f;
   f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 4
   for (uint32_t z = g; z < nz; z += GR) {
-    const float* p = part + z * (D + kPartHead);
+    const float* p = piece(z);
     const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p + kPartHead + d);
     const float m = p[0];
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
@@ -1255,30 +1258,85 @@ uint32_t kv4_split(const Kv4& c, uint32_t n, uint32_t rows, bool ragged, uint32_
       1, std::min<uint64_t>({768 / std::max<uint64_t>(parts * c.heads, 1), 128, tiles / (ragged ? kManyTiles : kFewTiles)}));
 }
 
-hipError_t launch_kv4_attend(const Kv4Attend& a, int type, hipStream_t st) {
-  if (!a.c.data || !a.r.pos || a.c.slots == 0 || a.c.heads == 0 || a.hq == 0 || a.hq % a.c.heads || a.nsplit == 0 || a.nsplit > 65535 || (a.nsplit > 1 && !a.part))
-    return hipErrorInvalidValue;
-  if (kv4_attend_groups(a.c.heads, a.r.n, a.r.rows, a.r.off != nullptr, a.hq) > kKv4MaxGroups) return hipErrorInvalidValue;
+namespace {
+
+bool attend_fits(const Kv4Attend& a) {
+  return a.c.data && a.r.pos && a.c.slots && a.c.heads && a.hq && a.hq % a.c.heads == 0 && a.nsplit && a.nsplit <= 65535 &&
+         kv4_attend_groups(a.c.heads, a.r.n, a.r.rows, a.r.off != nullptr, a.hq) <= kKv4MaxGroups;
+}
+// the sequences' own positions: the outputs, or what the join takes
+template <typename T, int D>
+void launch_own(const Kv4Attend& a, hipStream_t st) {
+  const uint32_t vec = on16<T>(a.q) && on16<T>(a.o);
+  const uint32_t G = a.hq / a.c.heads;
+  // a pair's columns: one a part, where single rows leave the room
+  constexpr int NC = sizeof(T) == 4 ? 4 : 2;
+  const bool wide = !a.r.off && G * NC <= 16;
+  const uint32_t ncol = a.r.off ? 1 : (G + 15) / 16;
+  const dim3 grid(a.r.n * a.c.heads * ncol, a.nsplit);
+  if (wide) hipLaunchKernelGGL((k_kv4_few<T, D, NC>), grid, dim3(256), 0, st, a, vec, 1u);
+  else hipLaunchKernelGGL((k_kv4_few<T, D, 1>), grid, dim3(256), 0, st, a, vec, ncol);
+  if (a.r.off) {
+    constexpr uint32_t PW = Many<T, D>::pairs;
+    const uint32_t gx = (uint32_t)(((uint64_t)a.r.rows * G + PW - 1) / PW) + a.r.n;
+    hipLaunchKernelGGL((k_kv4_many<T, D, false>), dim3(gx * a.c.heads, a.nsplit), dim3(256), 0, st, a, vec);
+  }
+}
+template <typename T, int D, bool PRE>
+void launch_join(const Kv4Attend& a, const Kv4Rows& pre, hipStream_t st) {
+  hipLaunchKernelGGL((k_kv4_join<T, D, PRE>), dim3((uint32_t)(((uint64_t)a.r.rows * a.hq + 3) / 4)), dim3(256), 0, st, a, pre);
+}
+
+}  // namespace
+
+hipError_t launch_kv4_attend(const Kv4Attend& call, int type, hipStream_t st) {
+  Kv4Attend a = call;
+  a.nz = a.nsplit;
+  a.z0 = 0;
+  a.raw = false;
+  if (!attend_fits(a) || (a.nsplit > 1 && !a.part)) return hipErrorInvalidValue;
   if (a.r.rows == 0 || a.r.n == 0) return hipSuccess;
   return by_type(type, a.c.hd, [&](auto t, auto d) -> hipError_t {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    const uint32_t vec = on16<T>(a.q) && on16<T>(a.o);
-    const uint32_t G = a.hq / a.c.heads;
-    // a pair's columns: one a part, where single rows leave the room
-    constexpr int NC = sizeof(T) == 4 ? 4 : 2;
-    const bool wide = !a.r.off && G * NC <= 16;
-    const uint32_t ncol = a.r.off ? 1 : (G + 15) / 16;
-    const dim3 grid(a.r.n * a.c.heads * ncol, a.nsplit);
-    if (wide) hipLaunchKernelGGL((k_kv4_few<T, D, NC>), grid, dim3(256), 0, st, a, vec, 1u);
-    else hipLaunchKernelGGL((k_kv4_few<T, D, 1>), grid, dim3(256), 0, st, a, vec, ncol);
-    if (a.r.off) {
-      constexpr uint32_t PW = Many<T, D>::pairs;
-      const uint32_t gx = (uint32_t)(((uint64_t)a.r.rows * G + PW - 1) / PW) + a.r.n;
-      hipLaunchKernelGGL((k_kv4_many<T, D>), dim3(gx * a.c.heads, a.nsplit), dim3(256), 0, st, a, vec);
-    }
-    if (a.nsplit > 1)
-      hipLaunchKernelGGL((k_kv4_join<T, D>), dim3((uint32_t)(((uint64_t)a.r.rows * a.hq + 3) / 4)), dim3(256), 0, st, a);
+    launch_own<T, D>(a, st);
+    if (a.nsplit > 1) launch_join<T, D, false>(a, Kv4Rows{}, st);
+    return hipGetLastError();
+  });
+}
+
+uint64_t kv4_prefix_groups(uint32_t heads, uint32_t n, uint32_t rows, uint32_t hq) {
+  return ((uint64_t)rows * (hq / heads) / 64 + 1 + n) * heads;
+}
+
+uint32_t kv4_prefix_split(const Kv4& pc, uint32_t n, uint32_t rows, uint32_t hq, uint64_t live) {
+  return kv4_split(pc, n, rows, true, hq, live);
+}
+
+hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const Kv4Rows& pre, uint32_t psplit, int type,
+                                    hipStream_t st) {
+  Kv4Attend a = call;
+  a.nz = a.nsplit + psplit;
+  a.z0 = 0;
+  a.raw = true;
+  if (!attend_fits(a) || !a.part || !pc.data || pc.slots == 0 || pc.heads != a.c.heads || pc.hd != a.c.hd || !pre.pos ||
+      psplit == 0 || psplit > 65535 || (!pre.off && pre.n != 1) || pre.rows != a.r.rows ||
+      kv4_prefix_groups(pc.heads, pre.n, pre.rows, a.hq) > kKv4MaxGroups)
+    return hipErrorInvalidValue;
+  if (a.r.rows == 0 || a.r.n == 0) return hipSuccess;
+  return by_type(type, a.c.hd, [&](auto t, auto d) -> hipError_t {
+    using T = decltype(t);
+    constexpr int D = decltype(d)::value, PW = Many<T, D>::pairs;
+    Kv4Attend p = a;
+    p.c = pc;
+    p.r = pre;
+    p.nsplit = psplit;
+    p.z0 = a.nsplit;
+    const uint32_t gx = (uint32_t)(((uint64_t)pre.rows * (a.hq / pc.heads) + PW - 1) / PW) + (pre.off ? pre.n : 0);
+    hipLaunchKernelGGL((k_kv4_many<T, D, true>), dim3(gx * pc.heads, psplit), dim3(256), 0, st, p,
+                       (uint32_t)(on16<T>(a.q) && on16<T>(a.o)));
+    launch_own<T, D>(a, st);
+    launch_join<T, D, true>(a, pre, st);
     return hipGetLastError();
   });
 }

@@ -25,29 +25,16 @@
 #include "kv4.h"
 #include "logprobs.h"
 #include "mfma.h"
+#include "order.h"
 #include "wave.h"
 
 namespace ana {
 
 namespace {
 
-typedef unsigned long long u64;
-
 constexpr uint32_t kJoinKeys = 2048;   // keys that a row's join takes into LDS
 constexpr uint32_t kJoinRank = 256;    // of them, those that it ranks by counting
 constexpr uint32_t kHead = 8;   // a piece's words before its keys: m, c, l, w, rank
-
-// a logit's order as a whole number: larger for larger ones, -0 as +0, 0 for NaN
-__device__ __forceinline__ uint32_t order_of(float x) {
-  if (x != x) return 0;
-  const uint32_t u = __builtin_bit_cast(uint32_t, x + 0.0f);
-  return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-}
-__device__ __forceinline__ float value_of(uint32_t o) {
-  if (o == 0) return __builtin_nanf("");
-  return __builtin_bit_cast(float, (o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
-}
-__device__ __forceinline__ u64 key_of(float x, uint32_t i) { return (u64)order_of(x) << 32 | (0xFFFFFFFFu - i); }
 
 // the largest over the wave by DPP moves, as wmax's
 template <int CTRL, int ROWS>

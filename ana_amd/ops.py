@@ -1,6 +1,8 @@
 """libana's operators on device memory, over torch tensors (include/ana.h,
-"operators on device memory"): keys and values in 4 bits, attention over
-them, and the log probabilities of rows of logits.
+"operators on device memory"): queries and keys normed and turned by their
+positions, keys and values in 4 bits, attention over them, also behind a
+prefix that sequences share, and of rows of logits the log probabilities and
+tokens from given random numbers.
 
 A ctypes mirror, as ana_amd itself is: every value is computed by libana.so.
 torch holds the tensors, allocates outputs and workspaces, and names the
@@ -48,6 +50,16 @@ class _Mat(C.Structure):
     _fields_ = [("p", C.c_void_p), ("row", C.c_uint64), ("head", C.c_uint64)]
 
 
+class _Rope(C.Structure):
+    _fields_ = [("freq", C.c_void_p), ("rot", C.c_uint32), ("near", C.c_int), ("gq", C.c_void_p), ("gk", C.c_void_p),
+                ("eps", C.c_float)]
+
+
+class _Draw(C.Structure):
+    _fields_ = [("temperature", C.c_float), ("top_p", C.c_float), ("min_p", C.c_float), ("top_k", C.c_uint32),
+                ("temperatures", C.c_void_p), ("top_ps", C.c_void_p), ("min_ps", C.c_void_p), ("top_ks", C.c_void_p)]
+
+
 def _check(r: int) -> None:
     if r != ANA_OK:
         raise AnaError(r, lib().ana_error(None).decode())
@@ -60,10 +72,14 @@ _stream = torch._C._cuda_getCurrentRawStream
 
 def _ints(t, n: int, device: torch.device, name: str):
     """A device array of whole numbers: int32, consecutive, n of them."""
+    return _array(t, n, torch.int32, device, name)
+
+
+def _array(t, n: int, dtype, device: torch.device, name: str):
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{name}: a consecutive int32 tensor of {n}, not {tuple(t.shape)} {t.dtype}")
+    if t.dtype is not dtype or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name}: a consecutive {str(dtype)[6:]} tensor of {n}, not {tuple(t.shape)} {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     return t.data_ptr()
@@ -138,6 +154,12 @@ def kv4_read(cache: KV4, pos: torch.Tensor, rows: int, seq=None, off=None, dtype
     return k, v
 
 
+def _sink(sink, hq: int, dev: torch.device):
+    if sink is not None and (sink.dtype is not torch.float32 or sink.shape != (hq,) or not sink.is_contiguous()
+                             or sink.device != dev):
+        raise ValueError(f"sink: a consecutive float32 tensor of {hq} on {dev}")
+
+
 def kv4_attend(q: torch.Tensor, cache: KV4, pos: torch.Tensor, seq=None, off=None, sink=None, scale=None, live: int = 0,
                out=None) -> torch.Tensor:
     """Softmax attention of query rows [rows, hq, hd] over the cache, whose
@@ -157,9 +179,7 @@ def kv4_attend(q: torch.Tensor, cache: KV4, pos: torch.Tensor, seq=None, off=Non
         om = _Mat(out.data_ptr(), hq * hd, hd)
     else:
         om = _mat(out, shape, dtype, dev, "out")
-    if sink is not None and (sink.dtype is not torch.float32 or sink.shape != (hq,) or not sink.is_contiguous()
-                             or sink.device != dev):
-        raise ValueError(f"sink: a consecutive float32 tensor of {hq} on {dev}")
+    _sink(sink, hq, dev)
     L, rp = lib(), C.byref(r)
     nb = L.ana_kv4_attend_ws(cache._p, rp, hq, live)
     ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
@@ -168,6 +188,116 @@ def kv4_attend(q: torch.Tensor, cache: KV4, pos: torch.Tensor, seq=None, off=Non
                             None if sink is None else sink.data_ptr(), C.byref(om), live,
                             None if ws is None else ws.data_ptr(), nb, _stream(dev.index)))
     return out
+
+
+def kv4_attend_shared(q: torch.Tensor, cache: KV4, pos: torch.Tensor, prefix: KV4, plen: torch.Tensor, pseq=None,
+                      poff=None, seq=None, off=None, sink=None, scale=None, live: int = 0, plive: int = 0,
+                      out=None) -> torch.Tensor:
+    """kv4_attend where groups of rows also see a prefix that they share: group
+    g has rows poff[g] .. poff[g + 1] - 1 (poff None: one group of all rows) and
+    sees the first plen[g] positions of place pseq[g] (or g) of the cache
+    `prefix`, besides each row's own sequence in `cache`. plen, pseq: int32
+    [groups]; plive: the longest prefix, where the program knows it to be less
+    than the ring's. A call of its own takes its workspace anew; captured into
+    a graph, it is the graph's. ana_kv4_attend_shared."""
+    rows, hq, hd = q.shape
+    dev, dtype = cache.device, q.dtype
+    r = _rows(cache, rows, pos, seq, off)
+    if prefix.device != dev:
+        raise ValueError(f"prefix is on {prefix.device}, not on {dev}")
+    p = _rows(prefix, rows, plen, pseq, poff)
+    shape = (rows, hq, cache.hd)
+    qm = _mat(q, shape, dtype, dev, "q")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=dev)
+        om = _Mat(out.data_ptr(), hq * hd, hd)
+    else:
+        om = _mat(out, shape, dtype, dev, "out")
+    _sink(sink, hq, dev)
+    L, rp, pp = lib(), C.byref(r), C.byref(p)
+    nb = L.ana_kv4_attend_shared_ws(cache._p, rp, prefix._p, pp, hq, live, plive)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev)
+    _check(L.ana_kv4_attend_shared(cache._p, rp, prefix._p, pp, _TYPES.get(dtype, -1), C.byref(qm), hq,
+                                   cache.hd ** -0.5 if scale is None else scale,
+                                   None if sink is None else sink.data_ptr(), C.byref(om), live, plive, ws.data_ptr(), nb,
+                                   _stream(dev.index)))
+    return out
+
+
+def qk_rope(q: torch.Tensor, k, pos: torch.Tensor, freq: torch.Tensor, off=None, gq=None, gk=None, eps: float = 1e-5,
+            near: bool = False, out=None):
+    """Queries [rows, hq, hd] and keys [rows, hk, hd] (k None: queries alone)
+    with each head RMS-normed (gq, gk: float32 [hd], the gain being 1 + g; None:
+    not) and its first 2 len(freq) values turned by position times freq, a
+    float32 tensor, in pairs of one of each half or, near, of neighbours.
+    Sequence i is at positions pos[i] and on, its rows off[i] .. off[i + 1] - 1
+    (or row i alone). out: where they go, a pair of tensors, q and k themselves
+    allowed; new ones otherwise. (q, k). ana_qk_rope."""
+    if not q.is_cuda:
+        raise ValueError("q is not on a GPU")
+    rows, hq, hd = q.shape
+    dev, dtype, n, hk = q.device, q.dtype, pos.numel(), 0 if k is None else k.shape[1]
+    if freq.dim() != 1:
+        raise ValueError("freq: one axis")
+    r = _Rows(n, rows, None, _ints(pos, n, dev, "pos"), _ints(off, n + 1, dev, "off"))
+    f = _Rope(_array(freq, freq.numel(), torch.float32, dev, "freq"), 2 * freq.numel(), near,
+              _array(gq, hd, torch.float32, dev, "gq"), _array(gk, hd, torch.float32, dev, "gk"), eps)
+    qm = _mat(q, (rows, hq, hd), dtype, dev, "q")
+    km = None if k is None else _mat(k, (rows, hk, hd), dtype, dev, "k")
+    if out is None:
+        # (one allocation: 2 us a call less than two)
+        both = torch.empty(rows * (hq + hk) * hd, dtype=dtype, device=dev)
+        qo, ko = both.split_with_sizes((rows * hq * hd, rows * hk * hd))
+        qo, ko = qo.view(rows, hq, hd), None if k is None else ko.view(rows, hk, hd)
+    else:
+        qo, ko = out
+    qom = _mat(qo, (rows, hq, hd), dtype, dev, "q's output")
+    kom = None if k is None else _mat(ko, (rows, hk, hd), dtype, dev, "k's output")
+    _check(lib().ana_qk_rope(dev.index, hd, C.byref(r), _TYPES.get(dtype, -1), C.byref(f), hq, C.byref(qm), C.byref(qom),
+                             hk, None if km is None else C.byref(km), None if kom is None else C.byref(kom),
+                             _stream(dev.index)))
+    return qo, ko
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    """A token of each row of logits [n, vocab] from the given random numbers u
+    (float32 [n], 0 up to 1), and its log probability among what is kept:
+    (tokens int32 [n], logprob float32 [n]). Each setting is a number, or a
+    tensor of n for the rows' own (float32; top_k int32): temperature (0 takes
+    the likeliest), top_k (0: all), top_p (1: all), min_p (0: all), in that
+    order. Tokens follow each other by value, then lower index; the one at
+    which the running probability passes u is drawn. ana_row_sample."""
+    if logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("sample: rows of logits, each consecutive")
+    if not logits.is_cuda:
+        raise ValueError("logits is not on a GPU")
+    n, vocab = logits.shape
+    dev = logits.device
+    d = _Draw(1.0, 1.0, 0.0, 0)
+    if isinstance(temperature, torch.Tensor):
+        d.temperatures = _array(temperature, n, torch.float32, dev, "temperature")
+    else:
+        d.temperature = temperature
+    if isinstance(top_k, torch.Tensor):
+        d.top_ks = _array(top_k, n, torch.int32, dev, "top_k")
+    elif top_k < 0:
+        raise ValueError(f"top_k: {top_k}")
+    else:
+        d.top_k = min(top_k, vocab)
+    if isinstance(top_p, torch.Tensor):
+        d.top_ps = _array(top_p, n, torch.float32, dev, "top_p")
+    else:
+        d.top_p = top_p
+    if isinstance(min_p, torch.Tensor):
+        d.min_ps = _array(min_p, n, torch.float32, dev, "min_p")
+    else:
+        d.min_p = min_p
+    up = _array(u, n, torch.float32, dev, "u")
+    tok = torch.empty(n, dtype=torch.int32, device=dev)
+    lp = torch.empty(n, dtype=torch.float32, device=dev)
+    _check(lib().ana_row_sample(dev.index, _TYPES.get(logits.dtype, -1), logits.data_ptr(), logits.stride(0), n, vocab,
+                                up, C.byref(d), tok.data_ptr(), lp.data_ptr(), _stream(dev.index)))
+    return tok, lp
 
 
 def logprobs(logits: torch.Tensor, tokens=None, top: int = 0):

@@ -405,6 +405,77 @@ int ana_kv4_attend(const ana_kv4* c, const ana_kv4_rows* r, int type, const ana_
                    const float* sink, const ana_mat* o, uint64_t live, void* ws, uint64_t ws_bytes, void* stream);
 uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq, uint64_t live);
 
+/* ana_kv4_attend where groups of rows also see a prefix that they have in
+ * common (the prompt of many answers, a system prompt), held and read once for
+ * all: group i of pre->n has rows pre->off[i] .. pre->off[i + 1] - 1 of the
+ * tensors (off NULL: n is 1, and all rows are its), and each of them sees the
+ * first pre->pos[i] positions of place pre->seq[i] (NULL: i) of the cache pc,
+ * those of them that its ring holds, besides its own sequence's in c. One
+ * softmax goes over both. pre->rows == r->rows. Rows of no group, a group
+ * whose place is none, and one whose length is 0 or not below 2^31 see their
+ * own positions alone; a sequence whose place in c is none has zeros. pc has
+ * c's heads and head size, and may be c. pre->off as r->off; up to 2^26
+ * groups. plive as live, of the prefixes. bf16 outputs' probabilities over a
+ * prefix are each rounded to bf16, over the own positions as there. ws:
+ * ana_kv4_attend_shared_ws bytes for the same arguments, on a 16-byte border. */
+int ana_kv4_attend_shared(const ana_kv4* c, const ana_kv4_rows* r, const ana_kv4* pc, const ana_kv4_rows* pre, int type,
+                          const ana_mat* q, uint32_t hq, float scale, const float* sink, const ana_mat* o, uint64_t live,
+                          uint64_t plive, void* ws, uint64_t ws_bytes, void* stream);
+uint64_t ana_kv4_attend_shared_ws(const ana_kv4* c, const ana_kv4_rows* r, const ana_kv4* pc, const ana_kv4_rows* pre,
+                                  uint32_t hq, uint64_t live, uint64_t plive);
+
+/* How a head's values turn with its row's position: of the first `rot` (a
+ * multiple of 16, hd at most; 0: none) the pairs (i, i + rot / 2), or with
+ * near (2 i, 2 i + 1), by position times freq[i] (rot / 2 floats), in radians:
+ * (a, b) becomes (a cos t - b sin t, b cos t + a sin t). gq and gk (hd
+ * floats; NULL: no norm): before that each head of q, of k, is RMS-normed, x /
+ * sqrt(mean x^2 + eps) * (1 + g), as a context's qk-norm. */
+typedef struct {
+  const float* freq;
+  uint32_t rot;
+  int near;
+  const float *gq, *gk;
+  float eps;
+} ana_rope;
+
+/* Queries q [rows][hq][hd] and keys k [rows][hk][hd], normed and turned, to qo
+ * and ko (which may be q and k themselves: the same address and strides),
+ * in one pass; hd a multiple of 16 up to 256, either of hq and hk may be 0
+ * (its tensors are not looked at). r->seq is not read. A sequence whose first
+ * position is none has zeros; rows of no sequence are left as they were.
+ * Angles are right to f32's last bit at every position. Up to 2^26 rows and
+ * sequences. */
+int ana_qk_rope(int device, uint32_t hd, const ana_kv4_rows* r, int type, const ana_rope* f, uint32_t hq, const ana_mat* q,
+                const ana_mat* qo, uint32_t hk, const ana_mat* k, const ana_mat* ko, void* stream);
+
+/* How tokens are drawn: one setting for every row, or (arrays of n, where not
+ * NULL) each row its own. temperature 0: the likeliest token. top_k: the first
+ * k tokens by value, then lower index (0, or the vocabulary and more: all).
+ * top_p: of these, the fewest first ones whose mass is top_p of theirs or more
+ * (1: all). min_p: of these, the ones of min_p or more of the likeliest one's
+ * probability (0: all). The first is always kept. In the arrays a temperature
+ * that is not above 0 is 0, a top_p of 1 or more (or NaN) is 1, of 0 or less
+ * 0, a min_p above 1 is 1 and one not above 0 (or NaN) is 0. */
+typedef struct {
+  float temperature, top_p, min_p;
+  uint32_t top_k;
+  const float *temperatures, *top_ps, *min_ps;
+  const uint32_t* top_ks;
+} ana_draw;
+
+/* A token of each of n rows of `vocab` logits (of ANA_T_ type `type`, ld
+ * elements from row to row, vocab or more) from a given number u[i], 0 <= u <
+ * 1 (others count as the nearest): tok[i], the first in the order of value,
+ * then lower index, at which the running probability of what is kept, e^(x /
+ * temperature) over its sum, passes u; and lp[i], the log of its own (0 for a
+ * temperature of 0). Probabilities below 2^-43 of the likeliest one's are 0, and
+ * the sums are exact in units of 2^-42 of it, so that a row's token does not
+ * depend on the other rows or on how the work is split. -inf and NaN are never
+ * drawn; tokens at +inf are alike and have all; with no number above -inf tok
+ * is 2^32 - 1 and lp NaN. Up to 2^21 logits and 2^22 - 1 rows. */
+int ana_row_sample(int device, int type, const void* logits, uint64_t ld, uint32_t n, uint32_t vocab, const float* u,
+                   const ana_draw* s, uint32_t* tok, float* lp, void* stream);
+
 /* Of n rows of `vocab` logits (of ANA_T_ type `type`, ld elements from row
  * to row, vocab or more), in one read of them: lp[i], the log probability of the given
  * token tok[i] (NaN for a token outside the vocabulary), and rank[i], the
