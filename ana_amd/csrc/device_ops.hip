@@ -278,8 +278,14 @@ extern "C" int ana_qk_rope(int device, uint32_t hd, const ana_kv4_rows* r, int t
   return launched(fn, launch_rope(a, type, (hipStream_t)stream));
 }
 
+extern "C" uint64_t ana_row_sample_ws(uint32_t n, uint32_t vocab) {
+  if (vocab == 0 || vocab > kSampleMaxVocab || n > kSampleMaxRows) return 0;
+  return 8 * sample_ws_words(n, vocab);
+}
+
 extern "C" int ana_row_sample(int device, int type, const void* logits, uint64_t ld, uint32_t n, uint32_t vocab,
-                              const float* u, const ana_draw* s, uint32_t* tok, float* lp, void* stream) {
+                              const float* u, const ana_draw* s, uint32_t* tok, float* lp, void* ws, uint64_t ws_bytes,
+                              void* stream) {
   const char* fn = "ana_row_sample";
   if (int e = check_type(fn, type)) return e;
   if (vocab == 0 || vocab > kSampleMaxVocab)
@@ -293,10 +299,14 @@ extern "C" int ana_row_sample(int device, int type, const void* logits, uint64_t
   if (n == 0) return ANA_OK;
   if (!logits || !u || !tok || !lp) return fail_call(ANA_EINVAL, "%s: null argument", fn);
   if ((uintptr_t)logits % size_of(type)) return fail_call(ANA_EINVAL, "%s: the logits are not on an element's border", fn);
+  const uint64_t need = ana_row_sample_ws(n, vocab);
+  if (need && (!ws || ws_bytes < need || (uintptr_t)ws % 8))
+    return fail_call(ANA_EINVAL, "%s: a workspace of %llu bytes on an 8-byte border, not %llu", fn, (unsigned long long)need,
+                     (unsigned long long)(ws ? ws_bytes : 0));
   OnDevice on(device);
   if (on.e != hipSuccess) return launched(fn, on.e);
   SampleArgs a{logits, n > 1 ? ld : vocab, n, vocab, u, s->temperature, s->top_p, s->min_p, s->top_k,
-               s->temperatures, s->top_ps, s->min_ps, s->top_ks, tok, lp};
+               s->temperatures, s->top_ps, s->min_ps, s->top_ks, tok, lp, (u64*)ws};
   return launched(fn, launch_sample(a, type, (hipStream_t)stream));
 }
 

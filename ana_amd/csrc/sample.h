@@ -5,6 +5,7 @@
 #include <cstdint>
 
 #include "kv4.h"
+#include "order.h"
 
 namespace ana {
 
@@ -23,7 +24,13 @@ struct SampleArgs {
   const uint32_t* ks;
   uint32_t* tok;      // [n]
   float* lp;          // [n]
+  u64* part;          // sample_ws_words words
 };
+// a split row's words in `part`: its bins, the mass of min-p's tokens, S pieces' group maxima
+constexpr uint32_t kSampleBins = 2048;
+__host__ __device__ inline uint64_t sample_part_words(uint32_t S) { return kSampleBins + 1 + 32 * (uint64_t)S; }
+// the words of workspace a call takes (0 for none)
+uint64_t sample_ws_words(uint32_t n, uint32_t vocab);
 // (type: kv4.h's ElemType)
 hipError_t launch_sample(const SampleArgs& a, int type, hipStream_t st);
 

@@ -295,8 +295,12 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     up = _array(u, n, torch.float32, dev, "u")
     tok = torch.empty(n, dtype=torch.int32, device=dev)
     lp = torch.empty(n, dtype=torch.float32, device=dev)
-    _check(lib().ana_row_sample(dev.index, _TYPES.get(logits.dtype, -1), logits.data_ptr(), logits.stride(0), n, vocab,
-                                up, C.byref(d), tok.data_ptr(), lp.data_ptr(), _stream(dev.index)))
+    L = lib()
+    nb = L.ana_row_sample_ws(n, vocab)
+    ws = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+    _check(L.ana_row_sample(dev.index, _TYPES.get(logits.dtype, -1), logits.data_ptr(), logits.stride(0), n, vocab, up,
+                            C.byref(d), tok.data_ptr(), lp.data_ptr(), None if ws is None else ws.data_ptr(), nb,
+                            _stream(dev.index)))
     return tok, lp
 
 

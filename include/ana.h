@@ -472,9 +472,11 @@ typedef struct {
  * the sums are exact in units of 2^-42 of it, so that a row's token does not
  * depend on the other rows or on how the work is split. -inf and NaN are never
  * drawn; tokens at +inf are alike and have all; with no number above -inf tok
- * is 2^32 - 1 and lp NaN. Up to 2^21 logits and 2^22 - 1 rows. */
+ * is 2^32 - 1 and lp NaN. Up to 2^21 logits and 2^22 - 1 rows. ws:
+ * ana_row_sample_ws bytes, on an 8-byte border (0 bytes but for few long rows). */
 int ana_row_sample(int device, int type, const void* logits, uint64_t ld, uint32_t n, uint32_t vocab, const float* u,
-                   const ana_draw* s, uint32_t* tok, float* lp, void* stream);
+                   const ana_draw* s, uint32_t* tok, float* lp, void* ws, uint64_t ws_bytes, void* stream);
+uint64_t ana_row_sample_ws(uint32_t n, uint32_t vocab);
 
 /* Of n rows of `vocab` logits (of ANA_T_ type `type`, ld elements from row
  * to row, vocab or more), in one read of them: lp[i], the log probability of the given

@@ -122,11 +122,11 @@ def test_empty_shared():
 
 def sample(**kw):
     d = dict(type=0, logits=A, ld=100, n=2, vocab=100, u=A, tok=A, lp=A, t=1.0, p=1.0, q=0.0, k=0, ts=None, ps=None, qs=None,
-             ks=None, s=True)
+             ks=None, s=True, ws=A, nws=1 << 40)
     d.update(kw)
     s = ops._Draw(d["t"], d["p"], d["q"], d["k"], d["ts"], d["ps"], d["qs"], d["ks"]) if d["s"] else None
     rc = ana_amd.lib().ana_row_sample(0, d["type"], d["logits"], d["ld"], d["n"], d["vocab"], d["u"], by(s), d["tok"],
-                                      d["lp"], None)
+                                      d["lp"], d["ws"], d["nws"], None)
     return rc, error()
 
 
@@ -139,6 +139,18 @@ def sample(**kw):
 def test_refuses_sample(kw, why):
     rc, msg = sample(**kw)
     assert rc == ana_amd.ANA_EINVAL and why in msg
+
+
+def test_sample_workspace():
+    """Few long rows take one."""
+    L = ana_amd.lib()
+    assert L.ana_row_sample_ws(1, 32000) == 0 and L.ana_row_sample_ws(3000, 200000) == 0 and L.ana_row_sample_ws(0, 200000) == 0
+    need = L.ana_row_sample_ws(2, 200000)
+    assert need > 2 * 8 * 2048
+    for kw in (dict(ws=None), dict(nws=need - 1), dict(ws=A + 4)):
+        rc, msg = sample(vocab=200000, ld=200000, **kw)
+        assert rc == ana_amd.ANA_EINVAL and "workspace" in msg
+    assert L.ana_row_sample_ws(1, 0) == 0 and L.ana_row_sample_ws(1, (1 << 21) + 1) == 0
 
 
 def test_empty_sample():
