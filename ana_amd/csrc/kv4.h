@@ -67,10 +67,12 @@ struct Kv4Attend {
   const float* sink;   // [hq] or nullptr
   float* part;         // partials [rows][hq][nsplit][kKv4PartHead + hd], when nsplit > 1
   uint32_t nsplit;     // pieces that a sequence's slots are cut into at most
-  // (set by the launches) a pair's places in `part`, the first of this kernel's
-  // pieces, and whether pieces go there even where there is only one
+  // (set by the launches) a pair's places in `part` and the first of this
+  // kernel's pieces; whether groups of the rows share prefixes, and theirs, whose
+  // pieces come after the nsplit of a row's own
   uint32_t nz, z0;
-  bool raw;
+  bool shared;
+  Kv4Rows pre;
 };
 // the pieces of a call (live: the most positions a sequence holds after it,
 // as far as the caller knows; 0: the ring's slots), and the floats of

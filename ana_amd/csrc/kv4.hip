@@ -429,7 +429,7 @@ constexpr uint32_t kPartHead = kKv4PartHead, kDone = 0xFFFFFFFFu;
 constexpr uint32_t kFewPairs = 16;
 // The pieces that `tiles` tiles are cut into, at most nsplit of at least
 // `least` tiles: the tiles of each but the last.
-constexpr uint32_t kFewTiles = 4, kManyTiles = 8;
+constexpr uint32_t kFewTiles = 4, kManyTiles = 8, kPrefixTiles = 2;
 __device__ __forceinline__ uint32_t piece_tiles(uint32_t tiles, uint32_t nsplit, uint32_t least) {
   const uint32_t n = max(1u, min(nsplit, tiles / least));
   return (tiles + n - 1) / n;
@@ -529,6 +529,48 @@ __device__ __forceinline__ bool not_finite(const Raw<D>& r) {
   return t == 0x7F800000u;
 }
 
+// A shared prefix's pieces of a row's pair, whose places in the partials start
+// at `part`: how many there are (none for a row of no group).
+template <int D>
+__device__ __forceinline__ uint32_t prefix_pieces(const Kv4Attend& a, const float* part, uint32_t row) {
+  if (a.pre.n == 0) return 0;
+  if (a.pre.off) {
+    const uint32_t g = find_from(a.pre.off, a.pre.n, row, 0), o1 = a.pre.off[g + 1];
+    if (row < a.pre.off[g] || row >= o1 || o1 > a.r.rows) return 0;
+  }
+  return min(__builtin_bit_cast(uint32_t, part[a.nsplit * (D + kPartHead) + 2]), a.nz - a.nsplit);
+}
+__device__ __forceinline__ float weight_of(float m, float M) { return m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M); }
+
+// nz pieces, the z-th at piece(z), by a wave: their maximum M, and the sums of
+// their denominators and (for dims 4 (lane % (D / 4)) ..) outputs, weighted
+// 2^(m_z - M). D / 4 lanes take a piece's outputs, so several are in flight at
+// once.
+template <int D, typename F>
+__device__ __forceinline__ void sum_pieces(uint32_t nz, F&& piece, uint32_t lane, float& M, float& l, f32x4_t& o) {
+  constexpr uint32_t L = D / 4, GR = 64 / L;   // lanes a piece, pieces at once
+  M = -INFINITY;
+  for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, piece(z)[0]);
+  M = wmax(M);
+  l = 0.0f;
+  o = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
+  for (uint32_t z = lane / L; z < nz; z += GR) {
+    const float* p = piece(z);
+    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p + kPartHead + lane % L * 4);
+    const float m = p[0];
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
+    l += p[1] * f;
+    o += y * f;
+  }
+#pragma unroll
+  for (uint32_t mk = L; mk < 64; mk <<= 1) {
+    l += __shfl_xor(l, mk, 64);
+#pragma unroll
+    for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], mk, 64);
+  }
+}
+
 // u's DPP move within its quad of lanes
 template <int CTRL>
 __device__ __forceinline__ uint32_t quad(uint32_t u) {
@@ -550,13 +592,17 @@ __device__ __forceinline__ uint32_t quad(float f) { return quad<CTRL>(__builtin_
 // get by DPP moves. (256 sequences of 2048 slots, 12 heads of 64, f32: a tile
 // costs 188 vector instructions and 8 MFMAs, 80 us or 5.3 TB/s with the vector
 // units busy 82% of it; with NC = 1 it was 296 and 24, 128 us.)
-template <typename T, int D, int NC>
+// PRE: rows of which groups share prefixes, whose pieces (k_kv4_many's) a
+// sequence in one piece takes in where its waves meet, as a fifth.
+template <typename T, int D, int NC, bool PRE>
 __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few(Kv4Attend a, uint32_t vec, uint32_t ncol) {
   constexpr int NP = Parts<T>::q, QP = NC == 1 ? NP : 1, NPP = NC == 1 ? Parts<T>::p : 1;
   constexpr int PC = 16 / NC;          // pairs a workgroup
   constexpr int OWN = NC == 1 ? 4 : 4 / NC;  // slots of four that a lane takes exponentials of
   __shared__ float om[4][16][D + 4];
-  __shared__ float mm[4][16], ll[4][16];
+  constexpr int NM = PRE ? 5 : 4;   // results that meet
+  __shared__ __align__(16) float pm_o[PRE ? PC : 1][D];
+  __shared__ float mm[NM][16], ll[NM][16];
   const uint32_t tid = threadIdx.x, lane = tid & 63, m = lane & 15, j = lane >> 4;
   const uint32_t wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   uint32_t w = blockIdx.x;
@@ -581,7 +627,7 @@ __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few
   const uint32_t per = piece_tiles(tiles, a.nsplit, kFewTiles);
   const uint32_t t0 = z * per, t1 = min(tiles, t0 + per);
   if (z && t0 >= t1) return;
-  const bool split = a.raw || tiles > per;
+  const bool split = tiles > per;
   const uint32_t pm = m / NC, part = m % NC;
   const uint32_t t = (c0 + pm) / G, g = (c0 + pm) % G;
   const float sc = a.scale * kLog2e;
@@ -760,10 +806,26 @@ __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few
       const uint32_t d = j * (D / 4) + i4 * (D / 16) + t16;
       om[wv][m][d] = (nan >> (d / 32)) & 1 ? __builtin_nanf("") : o[t16][i4];
     }
+  if constexpr (PRE) {
+    for (uint32_t pp = wv; pp < np; pp += 4) {
+      const uint32_t row = row0 + (c0 + pp) / G, hd = head * G + (c0 + pp) % G;
+      const float* p = a.part + ((uint64_t)row * a.hq + hd) * a.nz * (D + kPartHead);
+      float M, ls;
+      f32x4_t y;
+      sum_pieces<D>(ok && !split ? prefix_pieces<D>(a, p, row) : 0u,
+                    [&](uint32_t u) { return p + (a.nsplit + u) * (D + kPartHead); }, lane, M, ls, y);
+      if (lane < D / 4) *reinterpret_cast<f32x4_t*>(&pm_o[pp][lane * 4]) = y;
+      if (lane == 0) {
+        mm[NM - 1][pp] = M;
+        ll[NM - 1][pp] = ls;
+      }
+    }
+  }
   __syncthreads();
   for (uint32_t k = tid; k < np * D; k += 256) {
     const uint32_t pp = k / D, d = k % D;
-    const float M = fmaxf(fmaxf(mm[0][pp], mm[1][pp]), fmaxf(mm[2][pp], mm[3][pp]));
+    float M = fmaxf(fmaxf(mm[0][pp], mm[1][pp]), fmaxf(mm[2][pp], mm[3][pp]));
+    if constexpr (PRE) M = fmaxf(M, mm[NM - 1][pp]);
     float lsum = 0.0f, y = 0.0f;
 #pragma unroll
     for (int u = 0; u < 4; u++) {
@@ -774,6 +836,11 @@ __global__ __launch_bounds__(256, (D == 128 ? 3 : 4) - (NC == 1)) void k_kv4_few
 #pragma unroll
       for (int n = 1; n < NC; n++) v += om[u][pp * NC + n][d];
       y += v * f;
+    }
+    if constexpr (PRE) {
+      const float f = mm[NM - 1][pp] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(mm[NM - 1][pp] - M);
+      lsum += ll[NM - 1][pp] * f;
+      y += pm_o[pp][d] * f;
     }
     const uint32_t row = row0 + (c0 + pp) / G, hd = head * G + (c0 + pp) % G;
     float* out = a.part + (((uint64_t)row * a.hq + hd) * a.nz + z) * (D + kPartHead);
@@ -879,10 +946,10 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
   const bool flat = !PRE && last < a.c.slots;
   const uint32_t seen = flat ? pos + t_hi + 1 : view.live;
   const uint32_t tiles = ok ? (seen + 31) / 32 : 0u;
-  const uint32_t per = piece_tiles(tiles, a.nsplit, kManyTiles);
+  const uint32_t per = piece_tiles(tiles, a.nsplit, PRE ? kPrefixTiles : kManyTiles);
   const uint32_t t0 = z * per, t1 = min(tiles, t0 + per);
   if (z && t0 >= t1) return;
-  const bool split = a.raw || tiles > per;
+  const bool split = PRE || tiles > per;
 
   const uint8_t* base = record_of(a.c, ok ? q : 0, head, 0);
   // a wave's part of a record: the key codes of slots m and 16 + m, or the
@@ -1076,13 +1143,39 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
   float(*rows)[OR] = reinterpret_cast<float(*)[OR]>(lds + wv * (16 * OR * 4));
 #pragma unroll
   for (int n = 0; n < NQ; n++) {
-    const float ls = pair_sum(l[n]);
+    float ls = pair_sum(l[n]);
     const uint32_t nn = pair_or(nan[n]);
     float f = 1.0f, inv = 1.0f;
     const uint32_t c = c0 + (wv * NQ + n) * 16 + m;
     const bool on = c < all;
     const uint32_t row = on ? row0 + c / G : row0, hq = on ? head * G + c % G : 0;
     float* part = a.part + (((uint64_t)row * a.hq + hq) * a.nz + a.z0 + z) * (D + kPartHead);
+    if (!PRE && a.shared && !split && ok && on) {
+      // what the row sees of its group's prefix
+      const uint32_t np = prefix_pieces<D>(a, part, row);
+      const float* p = part + a.nsplit * (D + kPartHead);
+      float top = mx[n];
+      for (uint32_t u = 0; u < np; u++) top = fmaxf(top, p[u * (D + kPartHead)]);
+      const float w0 = weight_of(mx[n], top);
+      mx[n] = top;
+      ls *= w0;
+#pragma unroll
+      for (int d = 0; d < OPS; d++) o[n][d] *= w0;
+#pragma unroll 1
+      for (uint32_t u = 0; u < np; u++) {
+        const float* e = p + u * (D + kPartHead);
+        const float w = weight_of(e[0], top);
+        ls += e[1] * w;
+#pragma unroll
+        for (int i4 = 0; i4 < 4; i4++)
+#pragma unroll
+          for (int t = 0; t < OPS; t += 2) {
+            const float2 y = *reinterpret_cast<const float2*>(e + kPartHead + j * (D / 4) + i4 * OPS + t);
+            o[n][t][i4] = fmaf(y.x, w, o[n][t][i4]);
+            o[n][t + 1][i4] = fmaf(y.y, w, o[n][t + 1][i4]);
+          }
+      }
+    }
     if (!split) {
       const float den = finish_sum(mx[n], ls, a.sink, hq, &f);
       inv = ok && den != 0.0f ? f / den : 0.0f;
@@ -1122,12 +1215,10 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
 }
 
 // The pieces of a (row, query head), a wave each: weights 2^(m_z - M), then
-// the sink, then the division. D / 4 lanes take a piece's outputs, so several
-// pieces are in flight at once. PRE: the pieces of the row's own positions,
-// then (from nsplit on) those of the prefix that its group in `pre` shares.
+// the sink, then the division. PRE: the pieces of the row's own positions,
+// then those of its group's prefix.
 template <typename T, int D, bool PRE>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a, Kv4Rows pre) {
-  constexpr uint32_t L = D / 4, GR = 64 / L;   // lanes a piece, pieces at once
+__global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a) {
   const uint32_t lane = threadIdx.x & 63;
   const uint64_t w = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const uint32_t row = (uint32_t)(w / a.hq), hd = (uint32_t)(w % a.hq);
@@ -1138,42 +1229,18 @@ __global__ __launch_bounds__(256) void k_kv4_join(Kv4Attend a, Kv4Rows pre) {
   if (a.r.off && (row < a.r.off[0] || row >= a.r.off[a.r.n])) return;
   if (nz > a.nsplit) return;
   const uint32_t own = nz;
-  if constexpr (PRE) {
-    bool has = pre.n != 0;
-    if (has && pre.off) {
-      const uint32_t g = find_seq(pre.off, pre.n, row);
-      has = row >= pre.off[g] && row < pre.off[g + 1] && pre.off[g + 1] <= a.r.rows;
-    }
-    if (has && nz) nz += min(__builtin_bit_cast(uint32_t, part[a.nsplit * (D + kPartHead) + 2]), a.nz - a.nsplit);
-  }
+  if (PRE && nz) nz += prefix_pieces<D>(a, part, row);
   // where piece z is (the own pieces may be fewer than their places)
   auto piece = [&](uint32_t z) { return part + (PRE && z >= own ? z - own + a.nsplit : z) * (D + kPartHead); };
-  float M = -INFINITY;
-  for (uint32_t z = lane; z < nz; z += 64) M = fmaxf(M, piece(z)[0]);
-  M = wmax(M);
-  const uint32_t g = lane / L, d = lane % L * 4;
-  float l = 0.0f;
-  f32x4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (uint32_t z = g; z < nz; z += GR) {
-    const float* p = piece(z);
-    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(p + kPartHead + d);
-    const float m = p[0];
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - M);
-    l += p[1] * f;
-    o += y * f;
-  }
-#pragma unroll
-  for (uint32_t mk = L; mk < 64; mk <<= 1) {
-    l += __shfl_xor(l, mk, 64);
-#pragma unroll
-    for (int e = 0; e < 4; e++) o[e] += __shfl_xor(o[e], mk, 64);
-  }
+  float M, l;
+  f32x4_t o;
+  sum_pieces<D>(nz, piece, lane, M, l, o);
+  const uint32_t d = lane % (D / 4) * 4;
   float f;
   const float den = finish_sum(M, l, a.sink, hd, &f);
   const float inv = nz && den != 0.0f ? f / den : 0.0f;
   T* out = (T*)a.o.p + (uint64_t)row * a.o.row + (uint64_t)hd * a.o.head + d;
-  if (g == 0) {
+  if (lane < D / 4) {
 #pragma unroll
     for (int e = 0; e < 4; e++) out[e] = (T)(nz ? o[e] * inv : 0.0f);
   }
@@ -1265,7 +1332,7 @@ bool attend_fits(const Kv4Attend& a) {
          kv4_attend_groups(a.c.heads, a.r.n, a.r.rows, a.r.off != nullptr, a.hq) <= kKv4MaxGroups;
 }
 // the sequences' own positions: the outputs, or what the join takes
-template <typename T, int D>
+template <typename T, int D, bool PRE>
 void launch_own(const Kv4Attend& a, hipStream_t st) {
   const uint32_t vec = on16<T>(a.q) && on16<T>(a.o);
   const uint32_t G = a.hq / a.c.heads;
@@ -1274,8 +1341,8 @@ void launch_own(const Kv4Attend& a, hipStream_t st) {
   const bool wide = !a.r.off && G * NC <= 16;
   const uint32_t ncol = a.r.off ? 1 : (G + 15) / 16;
   const dim3 grid(a.r.n * a.c.heads * ncol, a.nsplit);
-  if (wide) hipLaunchKernelGGL((k_kv4_few<T, D, NC>), grid, dim3(256), 0, st, a, vec, 1u);
-  else hipLaunchKernelGGL((k_kv4_few<T, D, 1>), grid, dim3(256), 0, st, a, vec, ncol);
+  if (wide) hipLaunchKernelGGL((k_kv4_few<T, D, NC, PRE>), grid, dim3(256), 0, st, a, vec, 1u);
+  else hipLaunchKernelGGL((k_kv4_few<T, D, 1, PRE>), grid, dim3(256), 0, st, a, vec, ncol);
   if (a.r.off) {
     constexpr uint32_t PW = Many<T, D>::pairs;
     const uint32_t gx = (uint32_t)(((uint64_t)a.r.rows * G + PW - 1) / PW) + a.r.n;
@@ -1283,8 +1350,8 @@ void launch_own(const Kv4Attend& a, hipStream_t st) {
   }
 }
 template <typename T, int D, bool PRE>
-void launch_join(const Kv4Attend& a, const Kv4Rows& pre, hipStream_t st) {
-  hipLaunchKernelGGL((k_kv4_join<T, D, PRE>), dim3((uint32_t)(((uint64_t)a.r.rows * a.hq + 3) / 4)), dim3(256), 0, st, a, pre);
+void launch_join(const Kv4Attend& a, hipStream_t st) {
+  hipLaunchKernelGGL((k_kv4_join<T, D, PRE>), dim3((uint32_t)(((uint64_t)a.r.rows * a.hq + 3) / 4)), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -1293,14 +1360,14 @@ hipError_t launch_kv4_attend(const Kv4Attend& call, int type, hipStream_t st) {
   Kv4Attend a = call;
   a.nz = a.nsplit;
   a.z0 = 0;
-  a.raw = false;
+  a.shared = false;
   if (!attend_fits(a) || (a.nsplit > 1 && !a.part)) return hipErrorInvalidValue;
   if (a.r.rows == 0 || a.r.n == 0) return hipSuccess;
   return by_type(type, a.c.hd, [&](auto t, auto d) -> hipError_t {
     using T = decltype(t);
     constexpr int D = decltype(d)::value;
-    launch_own<T, D>(a, st);
-    if (a.nsplit > 1) launch_join<T, D, false>(a, Kv4Rows{}, st);
+    launch_own<T, D, false>(a, st);
+    if (a.nsplit > 1) launch_join<T, D, false>(a, st);
     return hipGetLastError();
   });
 }
@@ -1309,8 +1376,14 @@ uint64_t kv4_prefix_groups(uint32_t heads, uint32_t n, uint32_t rows, uint32_t h
   return ((uint64_t)rows * (hq / heads) / 64 + 1 + n) * heads;
 }
 
+// A prefix's pieces, at most: as kv4_split's for ragged calls, but of two tiles
+// or more, so that a short prefix of few rows is spread too (12 heads of 64,
+// f32: 8 rows behind 700 positions 13.1 us in pieces of eight tiles, 6.3 so; 64
+// behind 1400 13.6 and 9.8; of one tile 5.9 and 13.2).
 uint32_t kv4_prefix_split(const Kv4& pc, uint32_t n, uint32_t rows, uint32_t hq, uint64_t live) {
-  return kv4_split(pc, n, rows, true, hq, live);
+  const uint64_t tiles = ((live ? std::min<uint64_t>(live, pc.slots) : pc.slots) + 31) / 32;
+  const uint64_t parts = std::max<uint64_t>(std::min(n, rows), ((uint64_t)rows * (hq / pc.heads) + 127) / 128);
+  return (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({768 / std::max<uint64_t>(parts * pc.heads, 1), 128, tiles / kPrefixTiles}));
 }
 
 hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const Kv4Rows& pre, uint32_t psplit, int type,
@@ -1318,7 +1391,8 @@ hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const 
   Kv4Attend a = call;
   a.nz = a.nsplit + psplit;
   a.z0 = 0;
-  a.raw = true;
+  a.shared = true;
+  a.pre = pre;
   if (!attend_fits(a) || !a.part || !pc.data || pc.slots == 0 || pc.heads != a.c.heads || pc.hd != a.c.hd || !pre.pos ||
       psplit == 0 || psplit > 65535 || (!pre.off && pre.n != 1) || pre.rows != a.r.rows ||
       kv4_prefix_groups(pc.heads, pre.n, pre.rows, a.hq) > kKv4MaxGroups)
@@ -1335,8 +1409,8 @@ hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const 
     const uint32_t gx = (uint32_t)(((uint64_t)pre.rows * (a.hq / pc.heads) + PW - 1) / PW) + (pre.off ? pre.n : 0);
     hipLaunchKernelGGL((k_kv4_many<T, D, true>), dim3(gx * pc.heads, psplit), dim3(256), 0, st, p,
                        (uint32_t)(on16<T>(a.q) && on16<T>(a.o)));
-    launch_own<T, D>(a, st);
-    launch_join<T, D, true>(a, pre, st);
+    launch_own<T, D, true>(a, st);
+    if (a.nsplit > 1) launch_join<T, D, true>(a, st);
     return hipGetLastError();
   });
 }
