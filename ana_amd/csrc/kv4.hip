@@ -1393,7 +1393,7 @@ hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const 
   a.z0 = 0;
   a.shared = true;
   a.pre = pre;
-  if (!attend_fits(a) || !a.part || !pc.data || pc.slots == 0 || pc.heads != a.c.heads || pc.hd != a.c.hd || !pre.pos ||
+  if (!attend_fits(a) || !a.part || !pc.data || pc.slots == 0 || pc.heads != a.c.heads || pc.hd != a.c.hd || (pre.n && !pre.pos) ||
       psplit == 0 || psplit > 65535 || (!pre.off && pre.n != 1) || pre.rows != a.r.rows ||
       kv4_prefix_groups(pc.heads, pre.n, pre.rows, a.hq) > kKv4MaxGroups)
     return hipErrorInvalidValue;

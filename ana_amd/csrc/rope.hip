@@ -220,8 +220,11 @@ hipError_t launch_rope(const RopeArgs& a, int type, hipStream_t st) {
     constexpr int L = decltype(l)::value, U = sizeof(T) == 4 ? 4 : 2;
     const uint32_t H = a.hq + a.hk, step = U * 256 / L;   // heads a workgroup takes at a time
     const uint32_t vec = on16<T>(a.q) && on16<T>(a.qo) && (!a.hk || (on16<T>(a.k) && on16<T>(a.ko)));
+    // Rows a workgroup: as many as give each thread two turns, while there are two
+    // workgroups a CU; single rows are cut into the heads of one turn. (And as many as
+    // keep the grid's threads below 2^32.)
     uint32_t R = std::min(kRopeRows, std::max(1u, 2 * step / H)), hy = H;
-    R = std::min(R, std::max(1u, a.r.rows / 512));
+    R = std::max(std::min(R, std::max(1u, a.r.rows / 512)), (a.r.rows + (1u << 23) - 1) >> 23);
     if (R == 1) hy = std::min(H, step);
     const dim3 grid((a.r.rows + R - 1) / R, (H + hy - 1) / hy);
     hipLaunchKernelGGL((k_qk_rope<T, L, U>), grid, dim3(256), 0, st, a, R, hy, vec);
@@ -231,8 +234,9 @@ hipError_t launch_rope(const RopeArgs& a, int type, hipStream_t st) {
     const uint32_t n = a.hd * sizeof(t) / 32;   // lanes that a head takes
     if (n <= 4) return go(t, std::integral_constant<int, 4>{});
     if (n <= 8) return go(t, std::integral_constant<int, 8>{});
-    if (n <= 16) return go(t, std::integral_constant<int, 16>{});
-    return go(t, std::integral_constant<int, 32>{});
+    if constexpr (sizeof(t) == 4)
+      if (n > 16) return go(t, std::integral_constant<int, 32>{});
+    return go(t, std::integral_constant<int, 16>{});
   };
   switch (type) {
     case ET_F32: return by_hd(float{});

@@ -17,9 +17,10 @@
 // (43.6 octaves: all that has a mass). Where a running mass is reached is
 // then a bin, whose few tokens go to LDS and are told apart there; the
 // likeliest 300 or so have been noted on the way, so that a nucleus of
-// few tokens needs no pass more. A top-k of up to 64 needs no masses but its
+// few tokens needs no pass more. A top-k of up to 256 needs no masses but its
 // own: the k-th largest of 64 group maxima is a bound that at least k logits
-// reach and few more do.
+// reach and few more do, and the least of them one that some 300 reach, k
+// among them mostly.
 //
 // Each pass reads the row again, from the caches mostly: a row held in
 // registers (64 of them for 32768 f32 logits, 512 threads) leaves too few for
@@ -43,6 +44,7 @@ constexpr uint32_t kBins = kSampleBins, kBinsOctave = 47, BT = kBins / NT;   // 
 constexpr uint32_t kList = NT;     // tokens that LDS takes, one a thread
 constexpr uint32_t kWave = 64;     // of them, a wave's
 constexpr uint32_t kFew = 64;      // those that one wave tells apart
+constexpr uint32_t kTop = 256;     // a top-k that is looked for among the likeliest alone
 constexpr double kUnit = 0x1p-42;  // of a mass
 static_assert(kBins == 4 * NT && kBins / kBinsOctave >= 43, "all that has a mass is in a bin");
 
@@ -236,7 +238,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     gm = gm == INFINITY ? 0.0f : -INFINITY;
     m = 0.0f;
   }
-  const bool greedy = !(t > 0.0f) || k == 1, short_k = k && k <= kFew;
+  const bool greedy = !(t > 0.0f) || k == 1, short_k = k && k <= kTop;
   if (STEP == kMass && (greedy || k)) return;   // (those rows need none, or not all)
   if (greedy) {
     uint32_t at = ~0u;
@@ -323,52 +325,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     return uni(all);
   };
 
-  if (short_k) {
-    // the k-th largest group maximum: the least that fewer than k are above
-    uint32_t above = 0;
-#pragma unroll 4
-    for (int i = 0; i < 64; i++) above += lane_f(gm, i) > gm;
-    const float bound = uni(-wmax(above < k ? -gm : -INFINITY));
-    uint32_t cnt = 0;
-    each(two, [&](const float (&v)[4], uint32_t i) {
-      note_four(v, i, [&](float x) { return x >= bound; }, [](u64) { return true; }, cnt);
-    });
-    const uint32_t nc = count_all(cnt);
-    if (nc <= kList) {
-      close_up(lane < cnt, lane < cnt ? list[tid] : 0);
-      if (tid < nc) {
-        const u64 mine = list[tid];
-        uint32_t over = 0;
-#pragma unroll 4
-        for (uint32_t o = 0; o < nc; o++) over += list[o] > mine ? 1u : 0u;
-        if (over < k) sub[over] = mine;
-      }
-      __syncthreads();
-      if (wv) return;
-      const bool in = lane < min(k, nc);
-      const u64 key = in ? sub[lane] : 0;
-      const double wd = in ? weight(value(key)) : 0.0;
-      const u64 w = units_of(wd), incl = wave_scan(w);
-      const u64 sum = lane_64(incl, 63);
-      const bool keep = in && (!nucleus || lane == 0 || incl - w < share_of(p, sum)) && (wd >= (double)q || lane == 0);
-      const uint32_t last = 63 - __clzll(__ballot(keep));
-      const u64 C = lane_64(incl, last), want = draw_of(a.u[r], C);
-      if (incl >= want && incl - w < want) answer(key, lp_of(key, C));
-      return;
-    }
-    __syncthreads();
-  }
-
-  // ---- the masses of all
-  const float cb = uni(fminf((float)(c * kBinsOctave), 3.0e38f));
-  // Where a logit is, in bins; what has no mass is past them (a NaN too), at a
-  // place of its lane's, so that few meet there.
-  const float none = (float)(kBins + lane);
-  auto place_of = [&](float v) { return fminf((m - v) * cb, none); };
-  // below it a weight is less than 2^-43
-  const float light = uni(m - fminf((float)(44.0 / c), 3.0e38f));
-  u64 cut = 0;   // keys below it are out (top-k)
-
   // the sum over the threads up to this one, and of all
   auto scan = [&](u64 v, u64* total) {
     v = wave_scan(v);
@@ -385,6 +341,66 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     *total = uni(all);
     return base + v;
   };
+
+  if (short_k) {
+    // the k-th largest group maximum, or the least: the least that fewer than k are above
+    uint32_t above = 0;
+#pragma unroll 4
+    for (int i = 0; i < 64; i++) above += lane_f(gm, i) > gm;
+    const float bound = uni(-wmax(above < k ? -gm : -INFINITY));
+    uint32_t cnt = 0;
+    each(two, [&](const float (&v)[4], uint32_t i) {
+      note_four(v, i, [&](float x) { return x >= bound; }, [](u64) { return true; }, cnt);
+    });
+    const uint32_t nc = count_all(cnt);
+    if (nc <= kList && (nc >= k || bound == -INFINITY)) {
+      close_up(lane < cnt, lane < cnt ? list[tid] : 0);
+      if (tid < nc) {
+        const u64 mine = list[tid];
+        uint32_t over = 0;
+#pragma unroll 4
+        for (uint32_t o = 0; o < nc; o++) over += list[o] > mine ? 1u : 0u;
+        if (over < k) sub[over] = mine;
+      }
+      __syncthreads();
+      const bool in = tid < min(k, nc);
+      const u64 key = in ? sub[tid] : 0;
+      const double wd = in ? weight(value(key)) : 0.0;
+      const u64 w = units_of(wd);
+      if (k <= 64) {
+        if (wv) return;
+        const u64 incl = wave_scan(w), sum = lane_64(incl, 63);
+        const bool keep = in && (!nucleus || lane == 0 || incl - w < share_of(p, sum)) && (wd >= (double)q || lane == 0);
+        const uint32_t last = 63 - __clzll(__ballot(keep));
+        const u64 C = lane_64(incl, last), want = draw_of(a.u[r], C);
+        if (incl >= want && incl - w < want) answer(key, lp_of(key, C));
+        return;
+      }
+      u64 sum;
+      const u64 incl = scan(w, &sum);
+      // (what is kept is a beginning: its last token's sum is the largest)
+      const bool keep = in && (!nucleus || tid == 0 || incl - w < share_of(p, sum)) && (wd >= (double)q || tid == 0);
+      if (tid == 0) hi_s = 0;
+      __syncthreads();
+      if (keep) atomicMax(&hi_s, incl);
+      __syncthreads();
+      const u64 C = uni(hi_s), want = draw_of(a.u[r], C);
+      if (in && incl >= want && incl - w < want) answer(key, lp_of(key, C));
+      return;
+    }
+    __syncthreads();
+  }
+
+  // ---- the masses of all
+  const float cb = uni(fminf((float)(c * kBinsOctave), 3.0e38f));
+  // Where a logit is, in bins; what has no mass is past them (a NaN too), at a
+  // place of its lane's, so that few meet there.
+  const float none = (float)(kBins + lane);
+  auto place_of = [&](float v) { return fminf((m - v) * cb, none); };
+  // below it a weight is less than 2^-43
+  const float light = uni(m - fminf((float)(44.0 / c), 3.0e38f));
+  u64 cut = 0;   // keys below it are out (top-k)
+
   // hist as running sums
   auto run_up = [&]() -> u64 {
     __syncthreads();

@@ -245,14 +245,12 @@ def qk_rope(q: torch.Tensor, k, pos: torch.Tensor, freq: torch.Tensor, off=None,
     qm = _mat(q, (rows, hq, hd), dtype, dev, "q")
     km = None if k is None else _mat(k, (rows, hk, hd), dtype, dev, "k")
     if out is None:
-        # (one allocation: 2 us a call less than two)
-        both = torch.empty(rows * (hq + hk) * hd, dtype=dtype, device=dev)
-        qo, ko = both.split_with_sizes((rows * hq * hd, rows * hk * hd))
-        qo, ko = qo.view(rows, hq, hd), None if k is None else ko.view(rows, hk, hd)
+        qo, ko = q.new_empty((rows, hq, hd)), None if k is None else k.new_empty((rows, hk, hd))
+        qom, kom = _Mat(qo.data_ptr(), hq * hd, hd), None if k is None else _Mat(ko.data_ptr(), hk * hd, hd)
     else:
         qo, ko = out
-    qom = _mat(qo, (rows, hq, hd), dtype, dev, "q's output")
-    kom = None if k is None else _mat(ko, (rows, hk, hd), dtype, dev, "k's output")
+        qom = _mat(qo, (rows, hq, hd), dtype, dev, "q's output")
+        kom = None if k is None else _mat(ko, (rows, hk, hd), dtype, dev, "k's output")
     _check(lib().ana_qk_rope(dev.index, hd, C.byref(r), _TYPES.get(dtype, -1), C.byref(f), hq, C.byref(qm), C.byref(qom),
                              hk, None if km is None else C.byref(km), None if kom is None else C.byref(kom),
                              _stream(dev.index)))

@@ -439,8 +439,8 @@ typedef struct {
 } ana_rope;
 
 /* Queries q [rows][hq][hd] and keys k [rows][hk][hd], normed and turned, to qo
- * and ko (which may be q and k themselves: the same address and strides),
- * in one pass; hd a multiple of 16 up to 256, either of hq and hk may be 0
+ * and ko (which may be q and k themselves: the same address and strides; else
+ * they lie apart from them), in one pass; hd a multiple of 16 up to 256, either of hq and hk may be 0
  * (its tensors are not looked at). r->seq is not read. A sequence whose first
  * position is none has zeros; rows of no sequence are left as they were.
  * Angles are right to f32's last bit at every position. Up to 2^26 rows and

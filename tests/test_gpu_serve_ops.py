@@ -253,6 +253,17 @@ def test_shared_long_prefix(ops, typ, rows):
     assert torch.isnan(got.float()).all()
 
 
+def test_shared_without_groups(ops):
+    """No prefix for any row: the attention of the rows' own rings."""
+    rs = np.random.RandomState(18)
+    cache = filled(ops, rs, 3, 70, 2, 64)
+    q, _ = rand(rs, (3, 4, 64), "f32")
+    pos = dev([5, 69, 200])
+    want = ops.kv4_attend(q, cache, pos)
+    got = ops.kv4_attend_shared(q, cache, pos, cache, dev([]), poff=dev([0]))
+    assert torch.equal(got, want)
+
+
 def test_shared_is_attention_over_copies(ops):
     """A prefix of 128 tokens and 70 own ones, against rings that hold both."""
     rs = np.random.RandomState(9)
@@ -307,7 +318,8 @@ def check_sample(ops, x, u, t=1.0, k=0, p=1.0, q=0.0):
 
 SETTINGS = [dict(), dict(t=0.0), dict(t=0.7, k=1), dict(t=0.8, k=40, p=0.95), dict(k=64, q=0.05), dict(t=1.3, k=65, p=0.7),
             dict(t=0.5, k=1000), dict(p=0.9), dict(t=1.7, p=0.99, q=0.01), dict(q=0.2), dict(p=0.0), dict(q=1.0),
-            dict(t=2.0, k=3000, p=0.9, q=1e-4)]
+            dict(t=2.0, k=3000, p=0.9, q=1e-4), dict(k=100), dict(t=1.5, k=256, p=0.8), dict(k=257, q=0.02),
+            dict(t=0.9, k=200, p=0.99, q=0.001)]
 
 
 @pytest.mark.parametrize("typ", list(TYPES))
