@@ -155,7 +155,8 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   const uint32_t e0 = STEP == kMax || STEP == kMass ? (blockIdx.x % S) * piece : 0;
   const uint32_t cnt_e = STEP == kMax || STEP == kMass ? min(piece, a.vocab - e0) : a.vocab;
   const T* row = (const T*)a.logits + (uint64_t)r * a.ld + e0;
-  const float t = a.ts ? a.ts[r] : a.t, p = a.ps ? a.ps[r] : a.p, q = a.qs ? a.qs[r] : a.q;
+  const float t = a.ts ? a.ts[r] : a.t, p = a.ps ? a.ps[r] : a.p, q_ = a.qs ? a.qs[r] : a.q;
+  const float q = q_ > 0.0f ? fminf(q_, 1.0f) : 0.0f;   // (above 1 is 1: what is as likely as the first stays; NaN is 0)
   const uint32_t k_ = a.ks ? a.ks[r] : a.k, k = k_ < a.vocab ? k_ : 0;   // (0: all)
   const uint32_t nvec = cnt_e / W;
   u64* const ghist = a.part + (uint64_t)r * sample_part_words(S);   // a split row's masses, then its pieces' group maxima

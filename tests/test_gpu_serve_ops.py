@@ -345,6 +345,23 @@ def test_sample_settings_of_each_row(ops):
                  q=pick([0.0, 0.1, 1e-3, 1.0, -1.0]))
 
 
+@pytest.mark.parametrize("vocab", [700, 9000, 100001])
+def test_sample_min_p_outside_0_to_1(ops, vocab):
+    """A row's min-p above 1 is 1 (what is as likely as the first stays), one
+    that is not above 0, or NaN, is 0."""
+    rs = np.random.RandomState(16)
+    given, meant = [2.0, 1.0001, math.inf, math.nan, -1.0, -math.inf, 1.0], [1.0, 1.0, 1.0, 0.0, 0.0, 0.0, 1.0]
+    x = torch.tensor(np.minimum(np.round(rs.randn(7, vocab)), 1.0), dtype=torch.float32).cuda()   # (many alike, the likeliest too)
+    for s in (dict(), dict(top_k=20), dict(top_k=100), dict(top_k=600), dict(top_p=0.9), dict(top_k=50, top_p=0.9)):
+        u = rs.rand(7).astype(np.float32)
+        u[0] = 0.97
+        tok, lp = ops.sample(x, dev(u, torch.float32), min_p=dev(given, torch.float32), **s)
+        for r in range(7):
+            want, wlp = sref.sample(host(x)[r], float(u[r]), 1.0, s.get("top_k", 0), float(np.float32(s.get("top_p", 1.0))), meant[r])
+            assert int(tok[r]) == want, (s, r)
+            assert abs(float(lp[r]) - wlp) <= 2.0 ** -24 * abs(wlp) + 2.0 ** -32, (s, r)   # (as in check_sample)
+
+
 @pytest.mark.parametrize("typ", ["f32", "bf16"])
 @pytest.mark.parametrize("vocab", [300, 20000, 70001])
 def test_sample_ties(ops, typ, vocab):
