@@ -440,11 +440,11 @@ typedef struct {
 
 /* Queries q [rows][hq][hd] and keys k [rows][hk][hd], normed and turned, to qo
  * and ko (which may be q and k themselves: the same address and strides; else
- * they lie apart from them), in one pass; hd a multiple of 16 up to 256, either of hq and hk may be 0
- * (its tensors are not looked at). r->seq is not read. A sequence whose first
- * position is none has zeros; rows of no sequence are left as they were.
- * Angles are right to f32's last bit at every position. Up to 2^26 rows and
- * sequences. */
+ * they lie apart from them), in one pass; hd a multiple of 16 up to 256, either
+ * of hq and hk may be 0 (its tensors are not looked at). r->seq is not read. A
+ * sequence whose first position is none has zeros; rows of no sequence are left
+ * as they were. Angles are right to f32's last bit at every position. Up to 2^26
+ * rows and sequences. */
 int ana_qk_rope(int device, uint32_t hd, const ana_kv4_rows* r, int type, const ana_rope* f, uint32_t hq, const ana_mat* q,
                 const ana_mat* qo, uint32_t hk, const ana_mat* k, const ana_mat* ko, void* stream);
 
