@@ -203,6 +203,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   };
   constexpr std::integral_constant<uint32_t, 2> two{};
   constexpr std::integral_constant<uint32_t, 8 * sizeof(T) / 4> many{};   // (for passes that do little)
+  constexpr std::integral_constant<uint32_t, STEP == kRest ? 8 * sizeof(T) / 4 : 2> noting{};   // (alone on its CU)
   auto answer = [&](u64 key, float lp) {
     a.tok[r] = 0xFFFFFFFFu - (uint32_t)key;
     a.lp[r] = lp;
@@ -350,7 +351,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     for (int i = 0; i < 64; i++) above += lane_f(gm, i) > gm;
     const float bound = uni(-wmax(above < k ? -gm : -INFINITY));
     uint32_t cnt = 0;
-    each(two, [&](const float (&v)[4], uint32_t i) {
+    each(noting, [&](const float (&v)[4], uint32_t i) {
       note_four(v, i, [&](float x) { return x >= bound; }, [](u64) { return true; }, cnt);
     });
     const uint32_t nc = count_all(cnt);
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
         y0 = (float)b + (float)part / NT;
         y1 = (float)b + (float)(part + 1) / NT;
         cnt = 0;
-        each(two, [&](const float (&v)[4], uint32_t i) { note_four(v, i, here, of_keys, cnt); });
+        each(noting, [&](const float (&v)[4], uint32_t i) { note_four(v, i, here, of_keys, cnt); });
         nc = count_all(cnt);
         if (nc <= kList) nc = close_up(lane < cnt, lane < cnt ? list[tid] : 0);
       } else {
@@ -512,7 +513,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
           }
         }
         cnt = 0;
-        each(two, [&](const float (&v)[4], uint32_t i) {
+        each(noting, [&](const float (&v)[4], uint32_t i) {
           note_four(v, i, [&](float x) { return here(x) || of_bins(x, b1, b2); }, of_keys, cnt);
         });
         nc = count_all(cnt);
@@ -602,7 +603,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
       });
       narrow(least, most, each_key);
       cnt = 0;
-      each(two, [&](const float (&v)[4], uint32_t i) { note_four(v, i, here, of_keys, cnt); });
+      each(noting, [&](const float (&v)[4], uint32_t i) { note_four(v, i, here, of_keys, cnt); });
       nc = count_all(cnt);
       if (nc <= kList) nc = close_up(lane < cnt, lane < cnt ? list[tid] : 0);
     }
