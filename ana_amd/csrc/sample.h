@@ -26,9 +26,10 @@ struct SampleArgs {
   float* lp;          // [n]
   u64* part;          // sample_ws_words words
 };
-// a split row's words in `part`: its bins, the mass of min-p's tokens, S pieces' group maxima
-constexpr uint32_t kSampleBins = 2048;
-__host__ __device__ inline uint64_t sample_part_words(uint32_t S) { return kSampleBins + 1 + 32 * (uint64_t)S; }
+// a split row's words in `part`: its bins, the mass of min-p's tokens, how many
+// tokens were gathered, S pieces' group maxima, the gathered tokens
+constexpr uint32_t kSampleBins = 2048, kSampleGather = 8192;
+__host__ __device__ inline uint64_t sample_part_words(uint32_t S) { return kSampleBins + 2 + 32 * (uint64_t)S + kSampleGather; }
 // the words of workspace a call takes (0 for none)
 uint64_t sample_ws_words(uint32_t n, uint32_t vocab);
 // (type: kv4.h's ElemType)

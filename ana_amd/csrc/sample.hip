@@ -133,12 +133,17 @@ __device__ __forceinline__ u64 share_of(float p, u64 S) {
 }
 
 // What a launch does: whole rows (kWhole), or, where rows are few and long, a
-// row in S pieces: their group maxima, then their masses, to `part`, and the
-// rest by one workgroup.
-enum Step { kWhole, kMax, kMass, kRest };
+// row in S pieces: their group maxima, then their masses, to `part`, then the
+// tokens of the bins that the nucleus' end and the draw can be in, and the rest
+// by one workgroup, which goes over those alone (or over the row, where they are
+// more than there is room for, or a top-k is asked for). (Four rows of 200003 f32
+// with a nucleus: 31 us; 116 when that workgroup went over the row itself, each
+// time 10 us. The lambdas that take others are inlined by force: one that is
+// not puts all they refer to in memory, 59 us.)
+enum Step { kWhole, kMax, kMass, kGather, kRest };
 
 template <typename T, Step STEP>
-__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_sample(SampleArgs a, uint32_t S, uint32_t piece) {
+__global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(STEP == kRest ? 2 : 4))) void k_sample(SampleArgs a, uint32_t S, uint32_t piece) {
   constexpr uint32_t W = 16 / sizeof(T);
   typedef T vec_t __attribute__((ext_vector_type(W)));
   // (a row may start on any element's border)
@@ -150,17 +155,19 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   __shared__ uint32_t nlist, bin_s, bin2_s[2], found[NW];
   __shared__ u64 before_s, key_s, incl_s, lo_s, hi_s;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wv = tid >> 6;
-  const uint32_t r = STEP == kMax || STEP == kMass ? blockIdx.x / S : blockIdx.x;
+  constexpr bool kPiece = STEP == kMax || STEP == kMass || STEP == kGather;
+  const uint32_t r = kPiece ? blockIdx.x / S : blockIdx.x;
   // the elements e0 .. of the row that this workgroup looks at
-  const uint32_t e0 = STEP == kMax || STEP == kMass ? (blockIdx.x % S) * piece : 0;
-  const uint32_t cnt_e = STEP == kMax || STEP == kMass ? min(piece, a.vocab - e0) : a.vocab;
+  const uint32_t e0 = kPiece ? (blockIdx.x % S) * piece : 0;
+  const uint32_t cnt_e = kPiece ? min(piece, a.vocab - e0) : a.vocab;
   const T* row = (const T*)a.logits + (uint64_t)r * a.ld + e0;
   const float t = a.ts ? a.ts[r] : a.t, p = a.ps ? a.ps[r] : a.p, q_ = a.qs ? a.qs[r] : a.q;
   const float q = q_ > 0.0f ? fminf(q_, 1.0f) : 0.0f;   // (above 1 is 1: what is as likely as the first stays; NaN is 0)
   const uint32_t k_ = a.ks ? a.ks[r] : a.k, k = k_ < a.vocab ? k_ : 0;   // (0: all)
   const uint32_t nvec = cnt_e / W;
-  u64* const ghist = a.part + (uint64_t)r * sample_part_words(S);   // a split row's masses, then its pieces' group maxima
-  float* const gmaxs = (float*)(ghist + kBins + 1);
+  u64* const ghist = a.part + (uint64_t)r * sample_part_words(S);   // a split row's words
+  float* const gmaxs = (float*)(ghist + kBins + 2);
+  u64* const gtok = ghist + kBins + 2 + 32 * S;
 
   bool inf = false;   // +inf is the largest: those are alike, the others nothing
   auto load = [&](uint32_t v) {
@@ -180,10 +187,28 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   // the elements after the last whole vector, one each for the first threads
   const uint32_t ie = nvec * W + tid;
   float xe = ie < cnt_e ? (float)row[ie] : -INFINITY;
-  // f(values, index of the first) over the thread's share in groups of four, U
+  uint32_t ntok = ~0u;   // the gathered tokens, where those do for the row
+  // f(values, their indices) over the thread's share in groups of four, U
   // vectors of loads at a time; places without a logit hold -inf
-  auto each = [&](auto vecs, auto&& f) {
+  auto each = [&](auto vecs, auto&& f) __attribute__((always_inline)) {
     constexpr uint32_t U = decltype(vecs)::value;
+    if constexpr (STEP == kRest) {
+      if (ntok != ~0u) {
+#pragma unroll 1
+        for (uint32_t i = tid; i - tid < ntok; i += 4 * NT) {
+          u64 key[4];
+          float v[4];
+#pragma unroll
+          for (uint32_t e = 0; e < 4; e++) key[e] = i + e * NT < ntok ? gtok[i + e * NT] : 0;
+#pragma unroll
+          for (uint32_t e = 0; e < 4; e++) v[e] = key[e] ? value_of((uint32_t)(key[e] >> 32)) : -INFINITY;
+          f(v, [&](uint32_t e) {
+            return 0xFFFFFFFFu - (uint32_t)(e == 0 ? key[0] : e == 1 ? key[1] : e == 2 ? key[2] : key[3]);
+          });
+        }
+        return;
+      }
+    }
 #pragma unroll 1
     for (uint32_t i = tid; i - tid < nvec; i += U * NT) {
       vec_t y[U];
@@ -194,12 +219,13 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
 #pragma unroll
         for (uint32_t e = 0; e < W; e += 4) {
           const float v[4] = {(float)y[u][e], (float)y[u][e + 1], (float)y[u][e + 2], (float)y[u][e + 3]};
-          f(v, e0 + (i + u * NT) * W + e);
+          const uint32_t at = e0 + (i + u * NT) * W + e;
+          f(v, [at](uint32_t o) { return at + o; });
         }
       }
     }
     const float v[4] = {xe, -INFINITY, -INFINITY, -INFINITY};
-    f(v, e0 + ie);
+    f(v, [&](uint32_t o) { return e0 + ie + o; });
   };
   constexpr std::integral_constant<uint32_t, 2> two{};
   constexpr std::integral_constant<uint32_t, 8 * sizeof(T) / 4> many{};   // (for passes that do little)
@@ -213,7 +239,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   float gm = -INFINITY;
   if constexpr (STEP == kWhole || STEP == kMax) {
     float m = -INFINITY;
-    each(many, [&](const float (&v)[4], uint32_t) { m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))); });
+    each(many, [&](const float (&v)[4], auto) { m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]))); });
     tmax[wv][lane] = m;
     __syncthreads();
     gm = tmax[0][lane];
@@ -226,12 +252,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   if constexpr (STEP == kMax) {
     if (wv == 0) gmaxs[(blockIdx.x % S) * 64 + lane] = gm;
     // (and the masses' places cleared for the next step)
-    for (uint32_t i = (blockIdx.x % S) * NT + tid; i <= kBins; i += S * NT) ghist[i] = 0;
+    for (uint32_t i = (blockIdx.x % S) * NT + tid; i < kBins + 2; i += S * NT) ghist[i] = 0;
     return;
   }
   float m = wmax(gm);
   if (m == -INFINITY) {   // no number above it
-    if (STEP != kMass && tid == 0) answer(~0ull << 32, __builtin_nanf(""));
+    if (!kPiece && tid == 0) answer(~0ull << 32, __builtin_nanf(""));
     return;
   }
   if (m == INFINITY) {
@@ -241,12 +267,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     m = 0.0f;
   }
   const bool greedy = !(t > 0.0f) || k == 1, short_k = k && k <= kTop;
-  if (STEP == kMass && (greedy || k)) return;   // (those rows need none, or not all)
+  if ((STEP == kMass || STEP == kGather) && (greedy || k)) return;   // (those rows need none, or not all)
   if (greedy) {
     uint32_t at = ~0u;
-    each(many, [&](const float (&v)[4], uint32_t i) {
+    each(many, [&](const float (&v)[4], auto i) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) at = v[e] == m ? min(at, i + e) : at;
+      for (int e = 0; e < 4; e++) at = v[e] == m ? min(at, i(e)) : at;
     });
 #pragma unroll
     for (int s = 32; s >= 1; s >>= 1) at = min(at, (uint32_t)__shfl_xor(at, s, 64));
@@ -285,7 +311,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     cnt += __popcll(mask);
   };
   // of four, those that in(value) (the cheap test, which most fail) and keep(key) hold for
-  auto note_four = [&](const float (&v)[4], uint32_t i, auto&& in, auto&& keep, uint32_t& cnt) {
+  auto note_four = [&](const float (&v)[4], auto&& i, auto&& in, auto&& keep, uint32_t& cnt) __attribute__((always_inline)) {
     unsigned long long on[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) on[e] = __ballot(in(v[e]));
@@ -293,7 +319,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       if (!on[e]) continue;
-      const u64 key = key_of(v[e], i + e);
+      const u64 key = key_of(v[e], i(e));
       note((on[e] >> lane & 1) && v[e] > -INFINITY && keep(key), key, cnt);
     }
   };
@@ -351,7 +377,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     for (int i = 0; i < 64; i++) above += lane_f(gm, i) > gm;
     const float bound = uni(-wmax(above < k ? -gm : -INFINITY));
     uint32_t cnt = 0;
-    each(noting, [&](const float (&v)[4], uint32_t i) {
+    each(noting, [&](const float (&v)[4], auto i) {
       note_four(v, i, [&](float x) { return x >= bound; }, [](u64) { return true; }, cnt);
     });
     const uint32_t nc = count_all(cnt);
@@ -440,7 +466,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   };
   // The key at which the running sum reaches R (1 .. the sum of all), and the
   // sum up to it. also0, also1: sums that will be asked for next.
-  auto find = [&](u64 R, u64 also0, u64 also1, u64* incl) -> u64 {
+  auto find = [&](u64 R, u64 also0, u64 also1, u64* incl) __attribute__((always_inline)) -> u64 {
     reaching(R, [&](uint32_t i) { bin_s = i; });
     if (also0) {
       reaching(also0, [&](uint32_t i) { bin2_s[0] = i; });
@@ -488,19 +514,19 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
       };
       if (about(b, b) > kList * 0.6f) {
         // more than the list takes: its parts' sums first
-        each(two, [&](const float (&v)[4], uint32_t i) {
+        each(two, [&](const float (&v)[4], auto i) {
           if (!__any(here(v[0]) || here(v[1]) || here(v[2]) || here(v[3]))) return;
           double w[4] = {};
           if (!counts) weights(v, w);
 #pragma unroll
           for (int e = 0; e < 4; e++)
-            if (here(v[e]) && key_of(v[e], i + e) >= cut) atomicAdd(&sub[part_at(v[e])], counts ? 1 : units_of(w[e]));
+            if (here(v[e]) && key_of(v[e], i(e)) >= cut) atomicAdd(&sub[part_at(v[e])], counts ? 1 : units_of(w[e]));
         });
         const uint32_t part = part_of();
         y0 = (float)b + (float)part / NT;
         y1 = (float)b + (float)(part + 1) / NT;
         cnt = 0;
-        each(noting, [&](const float (&v)[4], uint32_t i) { note_four(v, i, here, of_keys, cnt); });
+        each(noting, [&](const float (&v)[4], auto i) { note_four(v, i, here, of_keys, cnt); });
         nc = count_all(cnt);
         if (nc <= kList) nc = close_up(lane < cnt, lane < cnt ? list[tid] : 0);
       } else {
@@ -513,7 +539,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
           }
         }
         cnt = 0;
-        each(noting, [&](const float (&v)[4], uint32_t i) {
+        each(noting, [&](const float (&v)[4], auto i) {
           note_four(v, i, [&](float x) { return here(x) || of_bins(x, b1, b2); }, of_keys, cnt);
         });
         nc = count_all(cnt);
@@ -555,7 +581,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     }
     // The keys of `members` into NT parts, the highest first: the part that the
     // sum reaches R in (its keys are lo .. hi then).
-    auto narrow = [&](u64 least, u64 most, auto&& members) {
+    auto narrow = [&](u64 least, u64 most, auto&& members) __attribute__((always_inline)) {
       // the extent of the members' keys
 #pragma unroll
       for (int s = 32; s >= 1; s >>= 1) {
@@ -587,12 +613,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
 #pragma unroll 1
     while (nc > kList) {
       u64 least = ~0ull, most = 0;
-      auto each_key = [&](auto&& f) {
-        each(two, [&](const float (&v)[4], uint32_t i) {
+      auto each_key = [&](auto&& f) __attribute__((always_inline)) {
+        each(two, [&](const float (&v)[4], auto i) {
 #pragma unroll 1
           for (uint32_t e = 0; e < 4; e++) {
             const float x = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
-            const u64 key = key_of(x, i + e);
+            const u64 key = key_of(x, i(e));
             if (here(x) && x > -INFINITY && of_keys(key)) f(key);
           }
         });
@@ -603,7 +629,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
       });
       narrow(least, most, each_key);
       cnt = 0;
-      each(noting, [&](const float (&v)[4], uint32_t i) { note_four(v, i, here, of_keys, cnt); });
+      each(noting, [&](const float (&v)[4], auto i) { note_four(v, i, here, of_keys, cnt); });
       nc = count_all(cnt);
       if (nc <= kList) nc = close_up(lane < cnt, lane < cnt ? list[tid] : 0);
     }
@@ -637,17 +663,17 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
 
   u64 sq = 0;   // the mass of those of weight q or more
   const double qd = uni((double)q);
-  auto masses = [&](auto all) {
+  auto masses = [&](auto all) __attribute__((always_inline)) {
     // (the least group maximum: some 300 reach it; no list is kept of pieces)
     const float likely = STEP == kWhole ? uni(-wmax(-gm)) : INFINITY;
     cnt = 0;
-    each(two, [&](const float (&v)[4], uint32_t i) {
+    each(two, [&](const float (&v)[4], auto i) {
       if (!__any(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) >= light)) return;
       double w[4];
       weights(v, w);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        if constexpr (!decltype(all)::value) w[e] = key_of(v[e], i + e) >= cut ? w[e] : 0.0;
+        if constexpr (!decltype(all)::value) w[e] = key_of(v[e], i(e)) >= cut ? w[e] : 0.0;
         // (past the bins w is anything, and no one looks)
         atomicAdd(&hist[(uint32_t)place_of(v[e])], units_of(w[e]));
       }
@@ -663,7 +689,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   u64 up = 0;
   if (counts) {
     clear();
-    each(two, [&](const float (&v)[4], uint32_t) {
+    each(two, [&](const float (&v)[4], auto) {
 #pragma unroll
       for (int e = 0; e < 4; e++) atomicAdd(&hist[(uint32_t)place_of(v[e])], 1ull);
     });
@@ -675,10 +701,14 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
   }
   clear();
   u64 heavy = 0;
-  if (STEP == kRest && k == 0) {
+  if (STEP == kGather || (STEP == kRest && k == 0)) {
 #pragma unroll
     for (uint32_t i = 0; i < BT; i++) hist[i * NT + tid] = ghist[i * NT + tid];
     heavy = ghist[kBins];
+    if constexpr (STEP == kRest) {
+      const u64 n = uni(ghist[kBins + 1]);
+      ntok = n <= kSampleGather ? (uint32_t)n : ~0u;
+    }
   } else {
     if (cut) masses(std::false_type{});
     else masses(std::true_type{});
@@ -705,6 +735,29 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(4))) void k_
     __syncthreads();
     least = draw_of(u, min(C, uni(lo_s) + 1));
     most = draw_of(u, min(C, uni(hi_s)));
+  }
+  if constexpr (STEP == kGather) {
+    // (R's bin, and behind a nucleus the bins that the draw can be in)
+    if (!nucleus) R = draw_of(u, C);
+    reaching(R, [&](uint32_t b) { bin_s = b; });
+    if (nucleus) {
+      reaching(least, [&](uint32_t b) { bin2_s[0] = b; });
+      reaching(most, [&](uint32_t b) { bin2_s[1] = b; });
+    }
+    __syncthreads();
+    const uint32_t b = uni(bin_s), i0 = nucleus ? uni(bin2_s[0]) : b, i1 = nucleus ? uni(bin2_s[1]) : b;
+    cnt = 0;
+    each(two, [&](const float (&v)[4], auto i) {
+      note_four(v, i, [&](float x) { return of_bins(x, b, b) || of_bins(x, i0, i1); }, [](u64) { return true; }, cnt);
+    });
+    const uint32_t n = count_all(cnt);
+    if (n <= kList) close_up(lane < cnt, lane < cnt ? list[tid] : 0);
+    // (a piece whose list is too short for them makes the count say so)
+    if (tid == 0) before_s = atomicAdd(&ghist[kBins + 1], n <= kList ? (u64)n : (u64)kSampleGather + 1);
+    __syncthreads();
+    const u64 at = uni(before_s) + tid;
+    if (n <= kList && tid < n && at < kSampleGather) gtok[at] = list[tid];
+    return;
   }
   // the nucleus' last token, then the one that is drawn
 #pragma unroll 1
@@ -755,7 +808,10 @@ hipError_t launch_sample(const SampleArgs& a, int type, hipStream_t st) {
       return;
     }
     hipLaunchKernelGGL((k_sample<T, kMax>), dim3(a.n * made), dim3(NT), 0, st, a, made, piece);
-    hipLaunchKernelGGL((k_sample<T, kMass>), dim3(a.n * made), dim3(NT), 0, st, a, made, piece);
+    if ((a.ts || a.t > 0.0f) && (a.ks || a.k == 0 || a.k >= a.vocab)) {   // (some row may ask for all masses)
+      hipLaunchKernelGGL((k_sample<T, kMass>), dim3(a.n * made), dim3(NT), 0, st, a, made, piece);
+      hipLaunchKernelGGL((k_sample<T, kGather>), dim3(a.n * made), dim3(NT), 0, st, a, made, piece);
+    }
     hipLaunchKernelGGL((k_sample<T, kRest>), dim3(a.n), dim3(NT), 0, st, a, made, piece);
   };
   switch (type) {

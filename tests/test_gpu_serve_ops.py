@@ -424,6 +424,20 @@ def test_sample_widest_vocabulary(ops):
         check_sample(ops, x, rs.rand(2), **s)
 
 
+@pytest.mark.parametrize("spread", [0.1, 0.17, 0.3, 0.6, 3.0])
+def test_sample_long_rows(ops, spread):
+    """One bin's tokens from more than a piece's list or all pieces' room takes
+    down to a few."""
+    rs = np.random.RandomState(17)
+    x = torch.tensor(rs.randn(2, 400003) * spread, dtype=torch.float32).cuda()
+    x[1, ::2] = x[0, 1::2].mean()
+    for s in (dict(), dict(p=0.9), dict(p=0.3, q=0.7), dict(k=400, p=0.9)):
+        check_sample(ops, x, rs.rand(2), **s)
+    k = dev([0, 400], torch.int32)
+    check_sample(ops, x, rs.rand(2), t=dev([0.7, 1.0], torch.float32), k=k, p=0.9)
+    check_sample(ops, x, rs.rand(2), t=dev([0.0, 1.3], torch.float32), k=k.flip(0), p=dev([0.5, 0.95], torch.float32))
+
+
 def test_sample_follows_the_probabilities(ops):
     """Evenly spaced numbers take each token as often as its probability says."""
     n = 4096
