@@ -777,10 +777,10 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(STEP == kRes
 }
 
 // How many pieces a row is cut into: where rows are few, as many as give every
-// CU one, of 8192 logits or more. (Whole distributions, f32: 64 rows of 131072
-// take 73.6 us by a workgroup each, 51.6 in four pieces; one row of 32768 with a
-// nucleus 17 and in four pieces 15.6, its likeliest token alone 8.7 and 15, so
-// rows that short stay whole.)
+// CU one, of 8192 logits or more. (f32: 64 rows of 131072 take 73.6 us by a
+// workgroup each for the whole distribution, 40.5 in four pieces. 16 rows of
+// 32768 with a nucleus 27.7 and in four pieces 26, with a top-k of 40 11 and 12.7,
+// their likeliest tokens 8.7 and 12.8: rows that short stay whole.)
 uint32_t pieces_of(uint32_t n, uint32_t vocab) {
   if (n == 0 || vocab < 65536) return 1;
   const uint32_t s = std::min(256 / n, vocab / 8192);
