@@ -286,6 +286,8 @@ __device__ __forceinline__ void split8(const float (&x)[8], bf16x8_t (&o)[N]) {
 }
 
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 // split8 for probabilities (never next to the largest float): a part of two
 // in one conversion, and what it leaves of each, x - part, in one dot product
 // of two with (-1, 0) or (0, -1), exact as every term is
@@ -349,6 +351,9 @@ __device__ __forceinline__ void load_v(Raw<D>& r, const uint8_t* rec, uint32_t l
 __device__ __forceinline__ uint32_t has255(uint32_t w) {
   return ((w & 0x7F7F7F7Fu) + 0x01010101u) & w & 0x80808080u;
 }
+// nonzero where some byte of w is not 108 .. 139 (a scale from 2^-19 to 2^12):
+// with 20 more those are 128 .. 159, and a byte that carries into the next is none of them
+__device__ __forceinline__ uint32_t past_f16(uint32_t w) { return ((w + 0x14141414u) & 0xE0E0E0E0u) ^ 0x80808080u; }
 __device__ __forceinline__ float scale_of(uint32_t w, int byte) {
   return __builtin_bit_cast(float, ((w >> (8 * byte)) & 0xFFu) << 23);
 }
@@ -363,13 +368,19 @@ __device__ __forceinline__ bf16x8_t key_op(const Raw<D>& r, int h, int s, float 
   const u32x4_t o = {two_of<0>(w, sc), two_of<1>(w, sc), two_of<2>(w, sc), two_of<3>(w, sc)};
   return __builtin_bit_cast(bf16x8_t, o);
 }
-// the value operands of dims m D / 16 + 2 u and + 1 over the lane's eight slots
-template <int D, int U>
+// two codes as f16: exact for scales from 2^-23 to 2^13
+template <int B>
+__device__ __forceinline__ uint32_t two_f16_of(uint32_t w, float s) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, s, B));
+}
+// the value operands of dims m D / 16 + 2 u and + 1 over the lane's eight
+// slots (F16: of that type, in the same registers)
+template <int D, int U, bool F16 = false>
 __device__ __forceinline__ void val_ops(const uint32_t (&w)[D / 16], const float (&sc)[8], bf16x8_t& a, bf16x8_t& b) {
   uint32_t x[8];
   static_for<8>([&](auto e_) {
     constexpr int e = decltype(e_)::value, byte = e * (D / 32) + U;
-    x[e] = two_of<byte % 4>(w[byte / 4], sc[e]);
+    x[e] = F16 ? two_f16_of<byte % 4>(w[byte / 4], sc[e]) : two_of<byte % 4>(w[byte / 4], sc[e]);
   });
   u32x4_t lo, hi;
 #pragma unroll
@@ -440,6 +451,13 @@ __device__ __forceinline__ uint32_t pieces_of(uint32_t tiles, uint32_t per) { re
 // base 2): probabilities then reach 2^kSlack, which costs f32 and bf16 no
 // digit, and most tiles rescale nothing.
 constexpr float kSlack = 10.0f;
+// Probabilities in f16 are held 2^kLift times as large (mx is that much below the
+// largest score) and reach 2^15, so that what is lost below f16's steps is 2^-32 of the largest one at most. (10 and a
+// slack of 5: 1% more time.)
+constexpr float kLift = 7.0f, kLiftSlack = 8.0f;
+// the bit of a wave's mode that makes numbers past f16's largest that one
+// (infinities and NaN stay)
+constexpr int kF16Largest = 1 | 23 << 6;   // MODE, from bit 23, one bit
 
 // The queries' scale: f32 queries carry it (times log2 e) into their parts,
 // 16-bit ones enter as they are and only take its sign
@@ -889,12 +907,18 @@ struct Many {
 // bf16 behind 32001 positions, 8 heads: 170 us, the matrix units busy 39% of it
 // and the vector units 58%, hardly at once; 5000 rows of 16 over 4 heads behind
 // three prefixes of 4668 to 8000, 395.)
+// A bf16 output's probabilities and values are f16 there: as many matrix
+// instructions as in bf16, but right to 2^-11, so that an output's error is its
+// own rounding's (1.7e-3 of the outputs' size, 2.3e-3 with bf16 ones; both calls
+// above 1 to 2% longer). From its first tile on with a value scale beyond f16, below
+// 2^-19 or above 2^12, a piece goes on in bf16, a probability in two parts.
 template <typename T, int D, bool PRE>
 __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend a, uint32_t vec) {
   constexpr int NP = Parts<T>::q, NPP = Many<T, D>::NPP, NQ = Many<T, D>::NQ;
   constexpr uint32_t PW = Many<T, D>::pairs;
   constexpr int KS = D / 32, OPS = D / 16;     // steps of a key operand, operands of a tile's keys (values)
   constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool FINE = PRE && NPP == 1;       // one f16 for a probability, or two bf16
   constexpr uint32_t OR = D + 4;               // a row of outputs in LDS
   constexpr size_t LDS = std::max<size_t>(2 * 2 * OPS * 64 * 16, 4 * 16 * OR * 4);
   __shared__ __align__(16) char lds[LDS];
@@ -970,7 +994,9 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
     rs[0] = t.x;
     rs[1] = t.y;
   };
-  auto stage = [&](uint32_t tile, uint32_t buf) {
+  // (half_: the values in f16; flag says where they have scales that are beyond it, or no numbers)
+  auto stage = [&](uint32_t tile, uint32_t buf, auto half_) __attribute__((always_inline)) {
+    constexpr bool F16 = decltype(half_)::value;
     bool bad;
     if (keys) {
       const uint32_t s0 = rs[0], s1 = rs[1], b8 = ((krow & 2 ? s1 : s0) >> ((krow & 1) * 16 + half * 8)) & 0xFF;
@@ -983,15 +1009,16 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
         ops[buf][0][half * KS + d][lane] = __builtin_bit_cast(bf16x8_t, o);
       }
     } else {
-      bad = __any(has255(rs[0]) | has255(rs[1]));
-      if (bad || tile * 32 + 32 > view.live) quiet_values(rs, tile, view.live, j);
+      if constexpr (F16) bad = __any(past_f16(rs[0]) | past_f16(rs[1]));
+      else bad = __any(has255(rs[0]) | has255(rs[1]));
+      if ((!F16 && bad) || tile * 32 + 32 > view.live) quiet_values(rs, tile, view.live, j);
       float vsc[8];
 #pragma unroll
       for (int e = 0; e < 8; e++) vsc[e] = scale_of(rs[e / 4], e % 4);
       static_for<KS>([&](auto u_) {
         constexpr int u = decltype(u_)::value;
         if (half == u * 2 / KS)
-          val_ops<D, u>(rw, vsc, ops[buf][1][2 * u][lane], ops[buf][1][2 * u + 1][lane]);
+          val_ops<D, u, F16>(rw, vsc, ops[buf][1][2 * u][lane], ops[buf][1][2 * u + 1][lane]);
       });
     }
     if (lane == 0) flag[buf][wv] = bad;
@@ -1025,121 +1052,177 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
     l[n] = 0.0f;
     nan[n] = 0;
   }
-  uint32_t buf = 0;
-  if (t0 < t1) stage(t0, 0);
+  uint32_t buf = 0, tile = t0;
+  if (t0 < t1) stage(t0, 0, std::integral_constant<bool, FINE>{});
   __syncthreads();
+  // (half_: up to the first tile that is not in f16)
+  auto go_over = [&](auto half_) __attribute__((always_inline)) {
+    constexpr bool F16 = decltype(half_)::value;
+    constexpr int PP = FINE && !F16 ? 2 : NPP;   // parts of a probability
 #pragma unroll 1
-  for (uint32_t tile = t0; tile < t1; tile++) {
-    const bool more = tile + 1 < t1;
-    if (more) load(tile + 1);
-    // (past every position of the wave's pairs: nothing to do)
-    if (PRE ? w0 < all : !flat || tile * 32 <= wave_hi) {
-      const bool whole = view.whole(tile, PRE ? 0 : len - 1 - t_lo);
-      const bool bad_k = flag[buf][0] | flag[buf][1], bad = flag[buf][2] | flag[buf][3];
-      // (f32 scores come out less their pair's maximum: the products start from it)
-      f32x4_t s[NQ][2];
+    for (; tile < t1; tile++) {
+      const bool more = tile + 1 < t1;
+      if (more) load(tile + 1);
+      // (past every position of the wave's pairs: nothing to do)
+      if (PRE ? w0 < all : !flat || tile * 32 <= wave_hi) {
+        const bool whole = view.whole(tile, PRE ? 0 : len - 1 - t_lo);
+        const bool bad_k = flag[buf][0] | flag[buf][1], bad = flag[buf][2] | flag[buf][3];
+        // (f32 scores come out less their pair's maximum: the products start from it)
+        f32x4_t s[NQ][2];
 #pragma unroll
-      for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = less[n];
+        for (int n = 0; n < NQ; n++) s[n][0] = s[n][1] = less[n];
 #pragma unroll
-      for (int d = 0; d < KS; d++)
+        for (int d = 0; d < KS; d++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          const bf16x8_t ko = ops[buf][0][h * KS + d][lane];
+          for (int h = 0; h < 2; h++) {
+            const bf16x8_t ko = ops[buf][0][h * KS + d][lane];
 #pragma unroll
-          for (int u = 0; u < NP; u++)
+            for (int u = 0; u < NP; u++)
 #pragma unroll
-            for (int n = 0; n < NQ; n++)
-              s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ko, qo[n][u][d], s[n][h], 0, 0, 0);
-        }
-      bf16x8_t po[NQ][NPP];
-      float x[NQ][8];
-      bool raise = false;
-      float top[NQ];
-#pragma unroll
-      for (int n = 0; n < NQ; n++)
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[n][e] = s[n][e / 4][e % 4];
-      if (bad_k) {
-        // (such a key has made its own slot's scores anything)
-        const uint32_t nk = nan_keys<D>(base + (uint64_t)tile * (34 * D), j);
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-#pragma unroll
-          for (int n = 0; n < NQ; n++) x[n][e] = (nk >> e) & 1 ? __builtin_nanf("") : x[n][e];
-      }
-      if (!whole) {
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const uint32_t slot = tile * 32 + 16 * (e / 4) + 4 * j + e % 4, back = view.back(slot);
-          const bool live = slot < view.live;
-#pragma unroll
-          for (int n = 0; n < NQ; n++) x[n][e] = live && back >= ago[n] ? x[n][e] : -INFINITY;
-        }
-      }
-      if (bad) {
-#pragma unroll 1
-        for (int n = 0; n < NQ; n++) {
-          const uint32_t t = nan_blocks<D>(base + (uint64_t)tile * (34 * D), tile, view, n ? ago[NQ - 1] : ago[0], j);
-          if (n == 0) nan[0] |= t;
-          else nan[NQ - 1] |= t;
-        }
-      }
-#pragma unroll
-      for (int n = 0; n < NQ; n++) {
-        top[n] = x[n][0];
-#pragma unroll
-        for (int e = 1; e < 8; e++) top[n] = fmaxf(top[n], x[n][e]);
-        if constexpr (F32) raise |= top[n] > (mx[n] == -INFINITY ? mx[n] : kSlack);
-        else raise |= top[n] * sf > mx[n] + kSlack;
-      }
-      if (__any(raise)) {
-#pragma unroll
-        for (int n = 0; n < NQ; n++) {
-          const float was = mx[n] == -INFINITY ? 0.0f : mx[n];
-          const float v = fmaxf(mx[n], F32 ? pair_max(top[n]) + was : pair_max(top[n]) * sf);
-          const float f = v == mx[n] ? 1.0f : __builtin_amdgcn_exp2f(mx[n] - v);
-          mx[n] = v;
-          if constexpr (F32) {
-            const float b = v == -INFINITY ? 0.0f : v;
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[n][e] -= b - was;
-            less[n] = f32x4_t{-b, -b, -b, -b};
+              for (int n = 0; n < NQ; n++)
+                s[n][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ko, qo[n][u][d], s[n][h], 0, 0, 0);
           }
-          l[n] *= f;
+        if (F16 && __builtin_amdgcn_readfirstlane(bad)) return;
+        bf16x8_t po[NQ][PP];
+        float x[NQ][8];
+        bool raise = false;
+        float top[NQ];
 #pragma unroll
-          for (int d = 0; d < OPS; d++) o[n][d] *= f;
+        for (int n = 0; n < NQ; n++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[n][e] = s[n][e / 4][e % 4];
+        if (bad_k) {
+          // (such a key has made its own slot's scores anything)
+          const uint32_t nk = nan_keys<D>(base + (uint64_t)tile * (34 * D), j);
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+#pragma unroll
+            for (int n = 0; n < NQ; n++) x[n][e] = (nk >> e) & 1 ? __builtin_nanf("") : x[n][e];
         }
+        if (!whole) {
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const uint32_t slot = tile * 32 + 16 * (e / 4) + 4 * j + e % 4, back = view.back(slot);
+            const bool live = slot < view.live;
+#pragma unroll
+            for (int n = 0; n < NQ; n++) x[n][e] = live && back >= ago[n] ? x[n][e] : -INFINITY;
+          }
+        }
+        if (!F16 && bad) {
+#pragma unroll 1
+          for (int n = 0; n < NQ; n++) {
+            const uint32_t t = nan_blocks<D>(base + (uint64_t)tile * (34 * D), tile, view, n ? ago[NQ - 1] : ago[0], j);
+            if (n == 0) nan[0] |= t;
+            else nan[NQ - 1] |= t;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+          top[n] = x[n][0];
+#pragma unroll
+          for (int e = 1; e < 8; e++) top[n] = fmaxf(top[n], x[n][e]);
+          if constexpr (F32) raise |= top[n] > (mx[n] == -INFINITY ? mx[n] : kSlack);
+          else if constexpr (F16) raise |= fmaf(top[n], sf, -mx[n]) > kLift + kLiftSlack;   // (as the exponents are formed)
+          else raise |= top[n] * sf > mx[n] + kSlack;
+        }
+        if (__any(raise)) {
+#pragma unroll
+          for (int n = 0; n < NQ; n++) {
+            const float was = mx[n] == -INFINITY ? 0.0f : mx[n];
+            float v = F32 ? pair_max(top[n]) + was : pair_max(top[n]) * sf;
+            if constexpr (F16) {
+              // kLift below the largest, but for its own step, and never above it:
+              // where that step is past f16's range, the largest are f16's largest
+              const float t = pair_max(top[n]);
+              v = fmaf(t, sf, -kLift);
+              if (fmaf(t, sf, -v) < 0.0f) v = fmaf(fabsf(v), -0x1p-24f, v);
+            }
+            v = fmaxf(mx[n], v);
+            const float f = v == mx[n] ? 1.0f : __builtin_amdgcn_exp2f(mx[n] - v);
+            mx[n] = v;
+            if constexpr (F32) {
+              const float b = v == -INFINITY ? 0.0f : v;
+#pragma unroll
+              for (int e = 0; e < 8; e++) x[n][e] -= b - was;
+              less[n] = f32x4_t{-b, -b, -b, -b};
+            }
+            l[n] *= f;
+#pragma unroll
+            for (int d = 0; d < OPS; d++) o[n][d] *= f;
+          }
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+          const float b = mx[n] == -INFINITY ? 0.0f : mx[n];
+#pragma unroll
+          for (int e = 0; e < 8; e++) x[n][e] = __builtin_amdgcn_exp2f(F32 ? x[n][e] : fmaf(x[n][e], sf, -b));
+          if constexpr (F16) {
+            const f16x2_t one = {(_Float16)1.0f, (_Float16)1.0f};
+            f16x8_t h;
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) {
+              const f16x2_t t = __builtin_convertvector((f32x2_t{x[n][e], x[n][e + 1]}), f16x2_t);
+              h[e] = t[0];
+              h[e + 1] = t[1];
+              l[n] = __builtin_amdgcn_fdot2(t, one, l[n], false);
+            }
+            po[n][0] = __builtin_bit_cast(bf16x8_t, h);
+            continue;
+          }
+          split8_p(x[n], po[n]);
+          if constexpr (PP == 1) {
+            const bf16x2_t one = {(__bf16)1.0f, (__bf16)1.0f};
+#pragma unroll
+            for (int e = 0; e < 8; e += 2)
+              l[n] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{po[n][0][e], po[n][0][e + 1]}, one, l[n], false);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) l[n] += x[n][e];
+          }
+        }
+#pragma unroll
+        for (int t = 0; t < OPS; t++) {
+          const bf16x8_t vo = ops[buf][1][t][lane];
+#pragma unroll
+          for (int u = 0; u < PP; u++)
+#pragma unroll
+            for (int n = 0; n < NQ; n++) {
+              if constexpr (F16)
+                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, vo), __builtin_bit_cast(f16x8_t, po[n][u]),
+                                                                 o[n][t], 0, 0, 0);
+              else
+                o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, po[n][u], o[n][t], 0, 0, 0);
+            }
+        }
+      } else if (F16 && __builtin_amdgcn_readfirstlane(flag[buf][2] | flag[buf][3])) {
+        return;
       }
+      if (more) stage(tile + 1, buf ^ 1, half_);
+      __syncthreads();
+      buf ^= 1;
+    }
+  };
+  if constexpr (FINE) {
+    __builtin_amdgcn_s_setreg(kF16Largest, 1);
+    go_over(std::true_type{});
+    if (tile < t1) {
+      // this tile again, in the buffer that no wave reads; without the lift, for
+      // which values next to f32's largest leave no room
+      load(tile);
+      buf ^= 1;
+      stage(tile, buf, std::false_type{});
+      __syncthreads();
 #pragma unroll
       for (int n = 0; n < NQ; n++) {
-        const float b = mx[n] == -INFINITY ? 0.0f : mx[n];
+        constexpr float f = 1.0f / (1 << (int)kLift);
+        mx[n] += kLift;
+        l[n] *= f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[n][e] = __builtin_amdgcn_exp2f(F32 ? x[n][e] : fmaf(x[n][e], sf, -b));
-        split8_p(x[n], po[n]);
-        if constexpr (NPP == 1) {
-          const bf16x2_t one = {(__bf16)1.0f, (__bf16)1.0f};
-#pragma unroll
-          for (int e = 0; e < 8; e += 2)
-            l[n] = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{po[n][0][e], po[n][0][e + 1]}, one, l[n], false);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; e++) l[n] += x[n][e];
-        }
-      }
-#pragma unroll
-      for (int t = 0; t < OPS; t++) {
-        const bf16x8_t vo = ops[buf][1][t][lane];
-#pragma unroll
-        for (int u = 0; u < NPP; u++)
-#pragma unroll
-          for (int n = 0; n < NQ; n++)
-            o[n][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vo, po[n][u], o[n][t], 0, 0, 0);
+        for (int d = 0; d < OPS; d++) o[n][d] *= f;
       }
     }
-    if (more) stage(tile + 1, buf ^ 1);
-    __syncthreads();
-    buf ^= 1;
   }
+  go_over(std::false_type{});
   // the outputs, 16 pairs at a time through the wave's part of LDS, so that a
   // store's lanes write whole rows
   float(*rows)[OR] = reinterpret_cast<float(*)[OR]>(lds + wv * (16 * OR * 4));

@@ -416,8 +416,9 @@ uint64_t ana_kv4_attend_ws(const ana_kv4* c, const ana_kv4_rows* r, uint32_t hq,
  * own positions alone; a sequence whose place in c is none has zeros. pc has
  * c's heads and head size, and may be c. pre->off as r->off; up to 2^26
  * groups. plive as live, of the prefixes. bf16 outputs' probabilities over a
- * prefix are each rounded to bf16, over the own positions as there. ws:
- * ana_kv4_attend_shared_ws bytes for the same arguments, on a 16-byte border. */
+ * prefix are taken to 2^-11, or 2^-32 of the largest one, over the own positions
+ * as there. Scores are to be below 2^29 in size. ws: ana_kv4_attend_shared_ws bytes for the same arguments, on a
+ * 16-byte border. */
 int ana_kv4_attend_shared(const ana_kv4* c, const ana_kv4_rows* r, const ana_kv4* pc, const ana_kv4_rows* pre, int type,
                           const ana_mat* q, uint32_t hq, float scale, const float* sink, const ana_mat* o, uint64_t live,
                           uint64_t plive, void* ws, uint64_t ws_bytes, void* stream);

@@ -297,6 +297,98 @@ def test_shared_in_place_and_strided(ops):
             assert torch.equal(ops.kv4_attend_shared(q, cache, dev(pos), prefix, dev([150])), want)
 
 
+def check_fine(ops, cache, prefix, q, q64, pos, off, plen, poff, sink, vmax=0.0):
+    """check_shared of bf16 with what f16 probabilities allow: each is off by
+    at most half a step, 2^-11 of itself, or 2^-32 of the largest one (vmax: of
+    the values), in the sum and in the denominator."""
+    got = check_shared(ops, cache, prefix, q, q64, "bf16", pos, None, off, plen, None, poff, sink)
+    n = len(pos)
+    o, pv, big, cnt = sref.attend_shared(q64, cache.data.cpu().numpy(), cache.slots, pos, list(range(n)), off,
+                                         prefix.data.cpu().numpy(), prefix.slots, plen, list(range(len(plen))), poff, sink,
+                                         cache.hd ** -0.5)
+    tol = ref.attend_tolerance("bf16", o, pv, big, cnt, cache.hd) + 2 * 2.0 ** -11 * pv + 2 * cnt * 2.0 ** -32 * vmax
+    far = np.abs(host(got) - o) - tol
+    assert (far <= 0).all(), far.max()
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("sink", [False, True])
+def test_shared_bf16_probabilities(ops, hd, sink):
+    """Few positions of like weight and values that cancel: a probability's
+    rounding is what shows in a bf16 output, not the output's own."""
+    rs = np.random.RandomState(21)
+    cache, prefix = filled(ops, rs, 64, 3, 2, hd), filled(ops, rs, 3, 40, 2, hd)
+    q, q64 = rand(rs, (64, 8, hd), "bf16")
+    sk = rs.randn(8) if sink else None
+    check_fine(ops, cache, prefix, q, q64, [0] * 64, None, [3], None, sk)
+    check_fine(ops, cache, prefix, q, q64, [0] * 64, None, [2, 33, 5], [0, 30, 31, 64], sk)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+def test_shared_values_of_any_scale(ops, hd):
+    """Blocks of values beyond f16 (and zeros as the cache holds them, and such
+    that are not finite) in some tiles, in all, in the last alone."""
+    rs = np.random.RandomState(22)
+    for at in ([5], [0], [9], [3, 4, 7], list(range(10))):
+        cache, prefix = filled(ops, rs, 20, 40, 1, hd), filled(ops, rs, 1, 310, 1, hd)
+        for t in at:
+            for lo, hi in ((60, 108), (140, 180), (2, 4)):
+                n = rs.randint(1, 12)
+                prefix.data[0, 0, t, dev(33 * hd + rs.randint(0, hd, n), torch.int64)] = dev(rs.randint(lo, hi, n), torch.uint8)
+        q, q64 = rand(rs, (20, 3, hd), "bf16")
+        check_fine(ops, cache, prefix, q, q64, rs.randint(0, 40, 20).tolist(), None, [310], None, None)
+    q, q64 = rand(rs, (1, 3, hd), "bf16")
+    for t, byte in ((2, 255), (9, 255), (2, 250), (2, 0)):
+        prefix = filled(ops, rs, 1, 310, 1, hd)
+        prefix.data[0, 0, t, 33 * hd] = byte     # (slot 32 t, the first dims)
+        got = host(ops.kv4_attend_shared(q, cache, dev([3]), prefix, dev([310])))
+        if byte == 255:
+            assert np.isnan(got[..., :32]).all() and np.isfinite(got[..., 32:]).all()
+        else:
+            check_fine(ops, cache, prefix, q, q64, [3], None, [310], None, None)
+
+
+@pytest.mark.parametrize("gap", [5.0, 9.0, 16.0, 20.0, 30.0])
+def test_shared_many_light_positions(ops, gap):
+    """One position of a prefix far above thousands of others whose weights
+    add up, at the start, in the middle and at the end; its value is zero."""
+    rs = np.random.RandomState(23)
+    hd, n = 64, 8000
+    for slot in (0, 4005, 7999):
+        cache, prefix = filled(ops, rs, 5, 3, 1, hd), filled(ops, rs, 1, n, 1, hd)
+        prefix.data[..., 32 * hd:33 * hd] = 117
+        cache.data[..., 32 * hd:33 * hd] = 117
+        ref_data = prefix.data.cpu().numpy()
+        ref.put(ref_data, 0, 0, slot, [7] * hd, [126] * 2, [0] * hd, [127] * 2)    # keys of 3, values of 0
+        prefix.data.copy_(torch.tensor(ref_data))
+        q = torch.full((5, 2, hd), gap / 24, device="cuda").bfloat16()            # (a score of gap, the others next to 0)
+        check_fine(ops, cache, prefix, q, host(q), [0] * 5, None, [n], None, None, vmax=6.0)
+
+
+@pytest.mark.parametrize("typ", list(TYPES))
+def test_shared_scores_of_any_size(ops, typ):
+    """Scores whose own steps are more than a weight's range: the likeliest
+    position has all, whether behind the prefix or the row's own."""
+    rs = np.random.RandomState(24)
+    hd, n, rows = 64, 300, 40
+    cache, prefix = filled(ops, rs, rows, 5, 1, hd), filled(ops, rs, 1, n, 1, hd)
+    K, V = ref.get(prefix.data.cpu().numpy(), 0, 0, n)
+    for big in (1e4,) if typ == "f16" else (1e4, 1e6, 1e7, 3e7, 1e8):
+        q, q64 = rand(rs, (rows, 2, hd), typ, big)
+        got = host(ops.kv4_attend_shared(q, cache, dev([2] * rows), prefix, dev([n])))
+        assert np.isfinite(got).all()
+        for r in range(rows):
+            own = ref.get(cache.data[r:r + 1].cpu().numpy(), 0, 0, 5)
+            k, v = np.concatenate([K, own[0][:3]]), np.concatenate([V, own[1][:3]])
+            for h in range(2):
+                x = k @ q64[r, h] * hd ** -0.5
+                at = np.argsort(x)
+                # (a score is off by 3 hd 2^-24 of its terms, in two of them, and 40 is a weight of nothing)
+                if x[at[-1]] - x[at[-2]] > 40 + 4 * 3 * hd * 2.0 ** -24 * (np.abs(k) @ np.abs(q64[r, h])).max() * hd ** -0.5:
+                    # (e^-40 of the others' values, and a few roundings of the quotient)
+                    assert np.abs(got[r, h] - v[at[-1]]).max() <= 6 * 2.0 ** -20, (big, r, h)
+
+
 # ---------------------------------------------------------------- sampling
 
 def check_sample(ops, x, u, t=1.0, k=0, p=1.0, q=0.0):
