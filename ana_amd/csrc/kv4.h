@@ -68,10 +68,9 @@ struct Kv4Attend {
   float* part;         // partials [rows][hq][nsplit][kKv4PartHead + hd], when nsplit > 1
   uint32_t nsplit;     // pieces that a sequence's slots are cut into at most
   // (set by the launches) a pair's places in `part` and the first of this
-  // kernel's pieces; whether groups of the rows share prefixes, and theirs, whose
-  // pieces come after the nsplit of a row's own
+  // kernel's pieces; the groups of rows that share prefixes, whose pieces come
+  // after the nsplit of a row's own
   uint32_t nz, z0;
-  bool shared;
   Kv4Rows pre;
 };
 // the pieces of a call (live: the most positions a sequence holds after it,

@@ -901,8 +901,8 @@ struct Many {
   static constexpr uint32_t pairs = 64 * NQ;
 };
 
-// PRE: the sequences are groups of rows, and what they see is a prefix that
-// they share: the first pos[i] positions of the group's place, all of them for
+// What the rows see: their sequences' own positions, or these beside a prefix
+// that groups of rows share, or (the sequences being the groups) the prefix: the first pos[i] positions of the group's place, all of them for
 // every row. Groups of any size are taken. (256 rows of 32 query heads of 128 in
 // bf16 behind 32001 positions, 8 heads: 170 us, the matrix units busy 39% of it
 // and the vector units 58%, hardly at once; 5000 rows of 16 over 4 heads behind
@@ -912,12 +912,13 @@ struct Many {
 // own rounding's (1.7e-3 of the outputs' size, 2.3e-3 with bf16 ones; both calls
 // above 1 to 2% longer). From its first tile on with a value scale beyond f16, below
 // 2^-19 or above 2^12, a piece goes on in bf16, a probability in two parts.
-template <typename T, int D, bool PRE>
+enum Seen { kAlone, kOwn, kPrefix };
+template <typename T, int D, Seen SEEN>
 __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend a, uint32_t vec) {
   constexpr int NP = Parts<T>::q, NPP = Many<T, D>::NPP, NQ = Many<T, D>::NQ;
   constexpr uint32_t PW = Many<T, D>::pairs;
   constexpr int KS = D / 32, OPS = D / 16;     // steps of a key operand, operands of a tile's keys (values)
-  constexpr bool F32 = sizeof(T) == 4;
+  constexpr bool F32 = sizeof(T) == 4, PRE = SEEN == kPrefix;
   constexpr bool FINE = PRE && NPP == 1;       // one f16 for a probability, or two bf16
   constexpr uint32_t OR = D + 4;               // a row of outputs in LDS
   constexpr size_t LDS = std::max<size_t>(2 * 2 * OPS * 64 * 16, 4 * 16 * OR * 4);
@@ -1235,7 +1236,7 @@ __global__ __launch_bounds__(256, (Many<T, D>::waves)) void k_kv4_many(Kv4Attend
     const bool on = c < all;
     const uint32_t row = on ? row0 + c / G : row0, hq = on ? head * G + c % G : 0;
     float* part = a.part + (((uint64_t)row * a.hq + hq) * a.nz + a.z0 + z) * (D + kPartHead);
-    if (!PRE && a.shared && !split && ok && on) {
+    if (SEEN == kOwn && !split && ok && on) {
       // what the row sees of its group's prefix
       const uint32_t np = prefix_pieces<D>(a, part, row);
       const float* p = part + a.nsplit * (D + kPartHead);
@@ -1431,7 +1432,7 @@ void launch_own(const Kv4Attend& a, hipStream_t st) {
   if (a.r.off) {
     constexpr uint32_t PW = Many<T, D>::pairs;
     const uint32_t gx = (uint32_t)(((uint64_t)a.r.rows * G + PW - 1) / PW) + a.r.n;
-    hipLaunchKernelGGL((k_kv4_many<T, D, false>), dim3(gx * a.c.heads, a.nsplit), dim3(256), 0, st, a, vec);
+    hipLaunchKernelGGL((k_kv4_many<T, D, PRE ? kOwn : kAlone>), dim3(gx * a.c.heads, a.nsplit), dim3(256), 0, st, a, vec);
   }
 }
 template <typename T, int D, bool PRE>
@@ -1445,7 +1446,6 @@ hipError_t launch_kv4_attend(const Kv4Attend& call, int type, hipStream_t st) {
   Kv4Attend a = call;
   a.nz = a.nsplit;
   a.z0 = 0;
-  a.shared = false;
   if (!attend_fits(a) || (a.nsplit > 1 && !a.part)) return hipErrorInvalidValue;
   if (a.r.rows == 0 || a.r.n == 0) return hipSuccess;
   return by_type(type, a.c.hd, [&](auto t, auto d) -> hipError_t {
@@ -1476,7 +1476,6 @@ hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const 
   Kv4Attend a = call;
   a.nz = a.nsplit + psplit;
   a.z0 = 0;
-  a.shared = true;
   a.pre = pre;
   if (!attend_fits(a) || !a.part || !pc.data || pc.slots == 0 || pc.heads != a.c.heads || pc.hd != a.c.hd || (pre.n && !pre.pos) ||
       psplit == 0 || psplit > 65535 || (!pre.off && pre.n != 1) || pre.rows != a.r.rows ||
@@ -1492,7 +1491,7 @@ hipError_t launch_kv4_attend_shared(const Kv4Attend& call, const Kv4& pc, const 
     p.nsplit = psplit;
     p.z0 = a.nsplit;
     const uint32_t gx = (uint32_t)(((uint64_t)pre.rows * (a.hq / pc.heads) + PW - 1) / PW) + (pre.off ? pre.n : 0);
-    hipLaunchKernelGGL((k_kv4_many<T, D, true>), dim3(gx * pc.heads, psplit), dim3(256), 0, st, p,
+    hipLaunchKernelGGL((k_kv4_many<T, D, kPrefix>), dim3(gx * pc.heads, psplit), dim3(256), 0, st, p,
                        (uint32_t)(on16<T>(a.q) && on16<T>(a.o)));
     launch_own<T, D, true>(a, st);
     if (a.nsplit > 1) launch_join<T, D, true>(a, st);
