@@ -286,9 +286,18 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(STEP == kRes
   }
 
   const double c = uni(1.4426950408889634 / (double)t), md = uni((double)m);
+  // below it a weight is less than 2^-43
+  const float light = uni(m - fminf((float)(44.0 / c), 3.0e38f));
+  // A temperature below 2^-121: bins as narrow as f32 makes them hold weights
+  // below 2^-1022 too, which exp2_of does not take.
+  const bool steep = c * kBinsOctave > 3.0e38;
   auto weights = [&](const float (&v)[4], double (&w)[4]) {
     const double z[4] = {((double)v[0] - md) * c, ((double)v[1] - md) * c, ((double)v[2] - md) * c, ((double)v[3] - md) * c};
     exp2_of(z, w);
+    if (steep) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) w[e] = v[e] >= light ? w[e] : 0.0;
+    }
   };
   auto weight = [&](float v) {
     const double z = __builtin_fmax(((double)v - md) * c, -64.0), four[4] = {z, z, z, z};   // (-64 for a NaN)
@@ -425,8 +434,6 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(STEP == kRes
   // place of its lane's, so that few meet there.
   const float none = (float)(kBins + lane);
   auto place_of = [&](float v) { return fminf((m - v) * cb, none); };
-  // below it a weight is less than 2^-43
-  const float light = uni(m - fminf((float)(44.0 / c), 3.0e38f));
   u64 cut = 0;   // keys below it are out (top-k)
 
   // hist as running sums

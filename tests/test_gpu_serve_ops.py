@@ -498,6 +498,20 @@ def test_sample_temperatures(ops):
             check_sample(ops, torch.tensor(x).cuda(), rs.rand(3), t=t, **s)
 
 
+@pytest.mark.parametrize("vocab", [2, 3001, 70001])
+def test_sample_temperatures_next_to_zero(ops, vocab):
+    """Temperatures down to f32's least number over logits as small as they are:
+    next to each other in f32, and far apart for e^x."""
+    rs = np.random.RandomState(25)
+    x = rs.randn(4, vocab) * np.array([[1e-37], [1e-36], [1e-40], [1e-43]])
+    x[0, 0], x[0, 1] = 0.0, -1e-37
+    x[1, ::2] -= 1e-35
+    x = x.astype(np.float32)
+    for t in (1e-45, 1e-43, 1e-40, 1e-38, 2e-37, 2.4e-37, 1e-36):
+        for s in (dict(), dict(p=0.8), dict(k=20), dict(k=300, p=0.9), dict(q=0.3, p=0.99)):
+            check_sample(ops, torch.tensor(x).cuda(), rs.rand(4), t=t, **s)
+
+
 def test_sample_numbers_at_the_borders(ops):
     """Masses and numbers that are exact: u at a border takes the next token."""
     x = torch.zeros((9, 8), device="cuda")
