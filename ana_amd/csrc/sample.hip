@@ -287,7 +287,7 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(STEP == kRes
 
   const double c = uni(1.4426950408889634 / (double)t), md = uni((double)m);
   // below it a weight is less than 2^-43
-  const float light = uni(m - fminf((float)(44.0 / c), 3.0e38f));
+  const float light = uni((float)(md - 44.0 / c));
   // A temperature below 2^-121: bins as narrow as f32 makes them hold weights
   // below 2^-1022 too, which exp2_of does not take.
   const bool steep = c * kBinsOctave > 3.0e38;

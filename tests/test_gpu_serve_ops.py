@@ -512,6 +512,21 @@ def test_sample_temperatures_next_to_zero(ops, vocab):
             check_sample(ops, torch.tensor(x).cuda(), rs.rand(4), t=t, **s)
 
 
+@pytest.mark.parametrize("typ", ["f32", "bf16"])
+@pytest.mark.parametrize("vocab", [3001, 70001])
+def test_sample_temperatures_next_to_none(ops, typ, vocab):
+    """At a temperature past every logit tokens at the type's lowest value are
+    as likely as the others, whole stretches of them too."""
+    rs = np.random.RandomState(26)
+    x = torch.tensor(rs.randn(3, vocab)).to(TYPES[typ])
+    x[0, 600:] = torch.finfo(TYPES[typ]).min
+    x[1, :vocab - 700] = torch.finfo(TYPES[typ]).min
+    x[2, 1::2] = -math.inf
+    for t in (math.inf, 3e38, 1e38, 1e37):
+        for s in (dict(), dict(p=0.8), dict(k=2000), dict(q=0.5)):
+            check_sample(ops, x.cuda(), [0.3, 0.9, 0.6], t=t, **s)
+
+
 def test_sample_numbers_at_the_borders(ops):
     """Masses and numbers that are exact: u at a border takes the next token."""
     x = torch.zeros((9, 8), device="cuda")
