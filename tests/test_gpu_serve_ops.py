@@ -253,6 +253,53 @@ def test_shared_long_prefix(ops, typ, rows):
     assert torch.isnan(got.float()).all()
 
 
+def own_pieces(ops, cache, rows, hq, pos, off=None):
+    """Whether kv4_attend of such a call cuts a sequence's own positions."""
+    r = ops._rows(cache, rows, dev(pos), None, None if off is None else dev(off))
+    return ops.lib().ana_kv4_attend_ws(cache._p, ops.C.byref(r), hq, 0) > 0
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("typ", list(TYPES))
+def test_shared_own_positions_in_pieces(ops, typ, hd):
+    """Single rows whose own positions are one piece and many in one call,
+    wrapped ones too, behind prefixes of one piece and many, of no length, without
+    a place, and of no group; with and without sinks."""
+    rs = np.random.RandomState(31)
+    pos = [650, 3, 127, 128, 255, 256, 699, 1500, 40, 700, 511, 0]
+    cache, prefix = filled(ops, rs, 13, 700, 2, hd), filled(ops, rs, 3, 400, 2, hd)
+    q, q64 = rand(rs, (12, 4, hd), typ)
+    assert own_pieces(ops, cache, 12, 4, pos)
+    seq = rs.permutation(13)[:12].tolist()
+    seq[6] = 13                                                        # (no place: zeros)
+    poff, pseq, plen = [1, 4, 6, 6, 8, 10], [2, 0, 1, 1, 7], [400, 17, 30, 0, 60]
+    for sink in (None, rs.randn(4)):
+        got = check_shared(ops, cache, prefix, q, q64, typ, pos, seq, None, plen, pseq, poff, sink)
+        assert (got[6] == 0).all()
+        check_shared(ops, cache, prefix, q, q64, typ, pos, seq, None, [333], [1], None, sink)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("typ", list(TYPES))
+def test_shared_ragged_own_positions_in_pieces(ops, typ, hd):
+    """Sequences of few rows and of many (16 pairs of a key head and more) over
+    one piece of their own positions and over several, rows before, between and
+    after the groups and of no sequence."""
+    rs = np.random.RandomState(32)
+    off = [2, 42, 45, 45, 65, 66, 68, 100, 109]
+    pos = [1500, 3, 9, 700, 1540, 255, 20, 1700]
+    cache, prefix = filled(ops, rs, 8, 1600, 1, hd), filled(ops, rs, 2, 400, 1, hd)
+    q, q64 = rand(rs, (111, 2, hd), typ)
+    assert own_pieces(ops, cache, 111, 2, pos, off)
+    seq = rs.permutation(8).tolist()
+    poff, pseq, plen = [0, 30, 43, 67, 104], [1, 0, 0, 1], [400, 33, 0, 150]
+    for sink in (None, rs.randn(2)):
+        out = torch.full_like(q, 7.5)
+        check_shared(ops, cache, prefix, q, q64, typ, pos, seq, off, plen, pseq, poff, sink, out=out)
+        assert (out[:2] == 7.5).all() and (out[109:] == 7.5).all()
+        check_shared(ops, cache, prefix, q, q64, typ, pos, seq, off, [399], [0], None, sink)
+
+
 def test_shared_without_groups(ops):
     """No prefix for any row: the attention of the rows' own rings."""
     rs = np.random.RandomState(18)
