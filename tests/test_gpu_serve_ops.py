@@ -628,6 +628,25 @@ def test_sample_rows_do_not_depend_on_each_other(ops):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+@pytest.mark.parametrize("typ", list(TYPES))
+def test_sample_long_rows_alone_and_in_a_batch(ops, typ):
+    """A row in pieces takes the token that it takes whole, to the bit of its
+    log probability."""
+    rs = np.random.RandomState(33)
+    n, vocab = 100, 70001
+    x, _ = rand(rs, (n, vocab), typ, 2.0)
+    x[3] = 1.0
+    x[4, ::3] = -math.inf
+    u = dev(rs.rand(n), torch.float32)
+    assert ops.lib().ana_row_sample_ws(1, vocab) > 0 and ops.lib().ana_row_sample_ws(n, vocab) == 0
+    for s in (dict(), dict(top_p=0.9), dict(temperature=0.0), dict(top_k=40), dict(top_k=500, top_p=0.9), dict(min_p=0.05),
+              dict(temperature=2.0, top_p=0.99, min_p=0.001)):
+        a = ops.sample(x, u, **s)
+        for r0, r1 in ((0, 1), (3, 5), (60, 100)):
+            b = ops.sample(x[r0:r1], u[r0:r1], **s)
+            assert torch.equal(a[0][r0:r1], b[0]) and torch.equal(a[1][r0:r1], b[1]), (s, r0)
+
+
 # ---------------------------------------------------------------- a served step of all of them
 
 class Step:
@@ -709,6 +728,69 @@ def test_served_steps_captured_and_side_by_side(ops):
         for s, t, out, w in zip(steps, twins, outs, want):
             assert torch.equal(s.cache.data, t.cache.data), i
             assert all(torch.equal(a, b) for a, b in zip(out, w)), i
+
+
+class LongStep(Step):
+    """A Step whose every launch there is takes part: own positions in pieces with
+    the join, rows of logits in pieces with their bins in a workspace."""
+
+    def __init__(self, ops, typ, seed=0, slots=700, **kw):
+        super().__init__(ops, typ, seed=seed, vocab=66001, **kw)
+        rs = np.random.RandomState(seed)
+        self.cache = filled(ops, rs, self.n, slots, self.cache.heads, self.hd)
+        self.pos = dev(rs.randint(0, 2 * slots, self.n))
+        self.head = self.head * 0.2
+
+    def run(self):
+        o = self.ops
+        q, k = o.qk_rope(self.q, self.k, self.pos + self.plen, self.freq, gq=self.gq, gk=self.gk)
+        o.kv4_write(self.cache, k, self.v, self.pos)
+        att = o.kv4_attend_shared(q, self.cache, self.pos, self.prefix, self.length)
+        logits = att.flatten(1).float() @ self.head.float()
+        tok, lp = o.sample(logits, self.u, 1.3, 0, 0.95, 1e-4)
+        return q, k, att, logits, tok, lp
+
+
+def test_long_steps_captured_and_side_by_side(ops):
+    """As test_served_steps_captured_and_side_by_side, of the launches that hand
+    counters, bins and pieces on: two graphs of their own workspaces, replayed on
+    two streams with other inputs each time."""
+    make = lambda: [LongStep(ops, "f32", seed=1), LongStep(ops, "bf16", n=9, plen=96, seed=2)]  # noqa: E731
+    steps, twins = make(), make()
+    for s in twins:
+        assert own_pieces(ops, s.cache, s.n, 4, [0] * s.n) and ops.lib().ana_row_sample_ws(s.n, 66001) > 0
+        s.run()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in steps:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(s.run())
+        graphs.append(g)
+    streams = [torch.cuda.Stream() for _ in steps]
+    rs = np.random.RandomState(34)
+    for i in range(5):
+        want = []
+        for s, t in zip(steps, twins):
+            fresh, u = rand(rs, tuple(s.x.shape), s.typ)[0], dev(rs.rand(s.n), torch.float32)
+            for y in (s, t):
+                y.x.copy_(fresh)
+                y.u.copy_(u)
+                y.pos.add_(37)
+            t.cache.data.copy_(s.cache.data)
+            want.append(t.run())
+        torch.cuda.synchronize()
+        for g, st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        for s, t, out, w in zip(steps, twins, outs, want):
+            assert torch.equal(s.cache.data, t.cache.data), i
+            assert all(torch.equal(a, b) for a, b in zip(out, w)), i
+            for r in range(s.n):
+                tok, lp = sref.sample(host(out[3])[r], float(s.u[r]), float(np.float32(1.3)), 0, float(np.float32(0.95)),
+                                      float(np.float32(1e-4)))
+                assert int(out[4][r]) == tok and abs(float(out[5][r]) - lp) <= 2.0 ** -24 * abs(lp) + 1e-9
 
 
 def test_calls_of_none(ops):
