@@ -905,9 +905,9 @@ struct Many {
 // prefix that groups of rows share), or, the sequences being the groups, that
 // prefix: the first pos[i] positions of the group's place, all of them for every
 // row. Groups of any size are taken. (256 rows of 32 query heads of 128 in bf16
-// behind 32001 positions, 8 heads: 170 us, the matrix units busy 39% of it and the
-// vector units 58%, hardly at once; 5000 rows of 16 over 4 heads behind three
-// prefixes of 4668 to 8000, 395.)
+// behind 32001 positions, 8 heads: 172 us, the matrix units busy 39% of it and the
+// vector units 56%, hardly at once; 5000 rows of 16 over 4 heads behind three
+// prefixes of 4668 to 8000, 396.)
 // A bf16 output's probabilities and values over a prefix are f16: as many matrix
 // instructions as in bf16, but right to 2^-11, so that an output's error is its
 // own rounding's (1.7e-3 of the outputs' size, 2.3e-3 with bf16 ones; both calls

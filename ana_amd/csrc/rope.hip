@@ -27,7 +27,8 @@ constexpr uint32_t kRopeRows = 16;   // rows a workgroup, at most
 
 // cos and sin of p f. The angle in quarter turns is the exact product of 56
 // bits times 2 / pi in twice 53, so that the part after the whole turns is
-// right to f32's last bit at every position below 2^32 (in f32 the angle of
+// right to f32's last bits at every position below 2^32, for frequencies
+// up to 256 in size and some way past (in f32 the angle of
 // position 10^6 is off by 0.03); then the series of sin and cos on a quarter
 // turn about 0, cut where the next term is below 2^-28.
 __device__ __forceinline__ float2 cos_sin(uint32_t p, float f) {

@@ -784,10 +784,12 @@ __global__ __launch_bounds__(NT) __attribute__((amdgpu_waves_per_eu(STEP == kRes
 }
 
 // How many pieces a row is cut into: where rows are few, as many as give every
-// CU one, of 8192 logits or more. (f32: 64 rows of 131072 take 73.6 us by a
-// workgroup each for the whole distribution, 40.5 in four pieces. 16 rows of
-// 32768 with a nucleus 27.7 and in four pieces 26, with a top-k of 40 11 and 12.7,
-// their likeliest tokens 8.7 and 12.8: rows that short stay whole.)
+// CU one, of 8192 logits or more, and three at least. In pieces and whole (f32, us; a
+// nucleus of 0.9 / the likeliest alone): 64 rows of 131072 46 and 76 / 18 and 14, 85
+// of 65536 in three 39 and 46 / 15 and 9. In two, which are left out: 128 of 131072 71
+// and 91 / 26 and 22, 128 of 65536 45 and 47 / 16 and 9. (16 rows of 32768 with a
+// nucleus 27.7 and in four pieces 26, with a top-k of 40 11 and 12.7, their likeliest
+// 8.7 and 12.8: rows that short stay whole.)
 uint32_t pieces_of(uint32_t n, uint32_t vocab) {
   if (n == 0 || vocab < 65536) return 1;
   const uint32_t s = std::min(256 / n, vocab / 8192);

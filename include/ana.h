@@ -444,8 +444,10 @@ typedef struct {
  * they lie apart from them), in one pass; hd a multiple of 16 up to 256, either
  * of hq and hk may be 0 (its tensors are not looked at). r->seq is not read. A
  * sequence whose first position is none has zeros; rows of no sequence are left
- * as they were. Angles are right to f32's last bit at every position. Up to 2^26
- * rows and sequences. */
+ * as they were. Angles are right to f32's last bits at every position for
+ * frequencies up to 256 in size. A norm's squares are summed in f32: a head where
+ * they pass its largest number (values next to 2^64) comes out as zeros. Up to
+ * 2^26 rows and sequences. */
 int ana_qk_rope(int device, uint32_t hd, const ana_kv4_rows* r, int type, const ana_rope* f, uint32_t hq, const ana_mat* q,
                 const ana_mat* qo, uint32_t hk, const ana_mat* k, const ana_mat* ko, void* stream);
 
@@ -473,7 +475,7 @@ typedef struct {
  * the sums are exact in units of 2^-42 of it, so that a row's token does not
  * depend on the other rows or on how the work is split. -inf and NaN are never
  * drawn; tokens at +inf are alike and have all; with no number above -inf tok
- * is 2^32 - 1 and lp NaN. Up to 2^21 logits and 2^22 - 1 rows. ws:
+ * is 2^32 - 1 and lp NaN. Finite logits are to be within 2^128 of each other. Up to 2^21 logits and 2^22 - 1 rows. ws:
  * ana_row_sample_ws bytes, on an 8-byte border (0 bytes but for few long rows). */
 int ana_row_sample(int device, int type, const void* logits, uint64_t ld, uint32_t n, uint32_t vocab, const float* u,
                    const ana_draw* s, uint32_t* tok, float* lp, void* ws, uint64_t ws_bytes, void* stream);
