@@ -344,11 +344,15 @@ def test_shared_in_place_and_strided(ops):
             assert torch.equal(ops.kv4_attend_shared(q, cache, dev(pos), prefix, dev([150])), want)
 
 
-def check_fine(ops, cache, prefix, q, q64, pos, off, plen, poff, sink, vmax=0.0):
-    """check_shared of bf16 with what f16 probabilities allow: each is off by
-    at most half a step, 2^-11 of itself, or 2^-32 of the largest one (vmax: of
-    the values), in the sum and in the denominator."""
-    got = check_shared(ops, cache, prefix, q, q64, "bf16", pos, None, off, plen, None, poff, sink)
+def check_fine(ops, cache, prefix, q, q64, pos, off, plen, poff, sink, vmax=0.0, **kw):
+    """bf16 outputs behind a prefix, with what f16 probabilities allow. Each is
+    off by at most half a step: 2^-11 of itself, or, where f16's steps no longer
+    shrink with it, 2^-25, the largest being 2^7 at least there, so 2^-32 of the
+    largest. That counts in the sum, times a value of the tiles that are in f16
+    (vmax at most), and in the denominator."""
+    d = lambda a: None if a is None else dev(a)  # noqa: E731
+    got = ops.kv4_attend_shared(q, cache, dev(pos), prefix, dev(plen), poff=d(poff), off=d(off),
+                                sink=None if sink is None else dev(sink, torch.float32), **kw)
     n = len(pos)
     o, pv, big, cnt = sref.attend_shared(q64, cache.data.cpu().numpy(), cache.slots, pos, list(range(n)), off,
                                          prefix.data.cpu().numpy(), prefix.slots, plen, list(range(len(plen))), poff, sink,
@@ -393,6 +397,24 @@ def test_shared_values_of_any_scale(ops, hd):
             assert np.isnan(got[..., :32]).all() and np.isfinite(got[..., 32:]).all()
         else:
             check_fine(ops, cache, prefix, q, q64, [3], None, [310], None, None)
+
+
+@pytest.mark.parametrize("hd", [32, 64, 128])
+@pytest.mark.parametrize("rows", [3, 50])
+def test_shared_values_of_any_scale_in_one_piece(ops, hd, rows):
+    """A prefix gone over in one piece, in f16 and from some tile on in bf16, its
+    scores rising and falling from tile to tile before that and after."""
+    rs = np.random.RandomState(27)
+    n = 700
+    for first in (0, 1, 9, 20, 21, 22):        # (22: none)
+        cache, prefix = filled(ops, rs, rows, 40, 1, hd), filled(ops, rs, 1, n, 1, hd)
+        for t in range(22):
+            prefix.data[0, 0, t, 32 * hd:33 * hd] = int(rs.randint(120, 130))
+        for t in (first, 21 if first < 21 else first):
+            if t < 22:
+                prefix.data[0, 0, t, dev(33 * hd + rs.randint(0, hd, 5), torch.int64)] = dev(rs.randint(140, 160, 5), torch.uint8)
+        q, q64 = rand(rs, (rows, 2, hd), "bf16")
+        check_fine(ops, cache, prefix, q, q64, rs.randint(0, 40, rows).tolist(), None, [n], None, rs.randn(2), vmax=6.0, plive=32)
 
 
 @pytest.mark.parametrize("gap", [5.0, 9.0, 16.0, 20.0, 30.0])
